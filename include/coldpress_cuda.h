@@ -8,8 +8,9 @@
  *     16-byte aligned.  `stream` is a cudaStream_t passed as void* (NULL = legacy stream).
  *   - Calls only enqueue work; they return before it finishes.  The return value is a
  *     CP_* status (0 = ok); CP_ERR_CUDA carries the CUDA message in cp_last_error().
- *   - Types are GGML type ids: Q8_0 = 8, Q2_K = 10, Q3_K = 11, Q4_K = 12, Q5_K = 13, Q6_K = 14.
- *   - Weights are float32 [nrow, n] with n a multiple of 256 (32 for Q8_0); imatrix vectors
+ *   - Types are GGML type ids: Q8_0 = 8, Q2_K = 10, Q3_K = 11, Q4_K = 12, Q5_K = 13, Q6_K = 14,
+ *     MXFP4 = 39, NVFP4 = 40 (the last as an operand of cp_mx4_* only).
+ *   - Weights are float32 [nrow, n] with n a multiple of 256 (32 for Q8_0 and MXFP4); imatrix vectors
  *     are float32 [n] and apply to every row; packed rows are n/256 * cp_block_bytes(type).
  *   - Output bytes are identical to the reference numpy codec (coldpress/kquant.py) for the
  *     same float32 inputs; inputs containing NaN or Inf are outside that guarantee.
@@ -271,6 +272,56 @@ int cp_xtx_inject_stall(int skip_step, int64_t wait_ns);
  * CP_ERR_TIMEOUT when a wait inside an earlier cp_xtx_accumulate ran out (its H is then
  * incomplete). */
 int cp_xtx_status(void* workspace, void* stream);
+
+/* ---------------------------------------------------------------- microscaled 4-bit operands
+ * No counterpart in the reference.  Values are e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign) times a
+ * block scale: MXFP4 (type 39) blocks of 32 with an e8m0 scale, NVFP4 (type 40) blocks of 16 with
+ * an e4m3 scale, times one tensor scale that the caller keeps.  MXFP4 also has a GGUF container
+ * (17-byte blocks), which cp_kquant_encode, cp_kquant_decode, their grouped forms and
+ * cp_weighted_err[_batch] accept; NaN and infinities make their block decode to NaN.
+ *
+ * An operand is two arrays.  codes: [rows][P/2], P = n rounded up to 256, element 2j of a row in
+ * the low half of byte j.  scales: tiles of 128 rows x 4 blocks, [rows/128][blocks of P/4][512],
+ * byte 16 r + 4 j + k of a tile for row 32 j + r and block k.  Both are zero past n. */
+#define CP_MXFP4 39
+#define CP_NVFP4 40
+#define CP_MX4_BF16 0
+#define CP_MX4_F16 1
+#define CP_MX4_F32 2
+
+int64_t cp_mx4_codes_bytes(int64_t rows, int64_t n);
+int64_t cp_mx4_scales_bytes(int format, int64_t rows, int64_t n);
+
+/* x [rows, n] of `dtype`, rows ld elements apart -> an operand.  tensor_scale: a power of two (1
+ * for MXFP4).  qw (float32 [n], non-negative) or NULL: with it every block tries several scales
+ * and keeps the least sum of qw (x - value)^2. */
+int cp_mx4_quantize(int format, int dtype, const void* x, int64_t rows, int64_t n, int64_t ld, const float* qw,
+                    float tensor_scale, uint8_t* codes, uint8_t* scales, void* stream);
+/* The values of an operand, [rows, n] of `dtype`. */
+int cp_mx4_dequantize(int format, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t n,
+                      float tensor_scale, int dtype, void* out, void* stream);
+/* GGUF MXFP4 bytes [nrow, n/32 * 17] -> an MXFP4 operand with the same values. */
+int cp_mx4_from_gguf(const uint8_t* raw, int64_t nrow, int64_t n, uint8_t* codes, uint8_t* scales, void* stream);
+
+/* y[t][r] = alpha * sum_k a[t][k] w[r][k], y [a_rows, w_rows] of `dtype`; both operands of one
+ * format and of n columns. */
+int cp_mx4_matmul(int format, const uint8_t* a_codes, const uint8_t* a_scales, int64_t a_rows, const uint8_t* w_codes,
+                  const uint8_t* w_scales, int64_t w_rows, int64_t n, float alpha, int dtype, void* y, void* stream);
+
+/* transpose == 0: y[t][r] = alpha * sum_k x[t][k] w[r][k], x [T, n], y [T, rows].
+ * transpose == 1: y[t][k] = alpha * sum_r x[t][r] w[r][k], x [T, rows], y [T, n] (the first
+ * form's gradient with respect to x).  x and y are of `dtype`, x's rows ld elements apart.
+ * workspace >= cp_mx4_linear_workspace_bytes of the same arguments (it may be 0). */
+size_t cp_mx4_linear_workspace_bytes(int dtype, const void* x, int64_t T, int64_t ld, int64_t rows, int64_t n,
+                                     int transpose);
+int cp_mx4_linear(int format, int dtype, const void* x, int64_t T, int64_t ld, const uint8_t* codes,
+                  const uint8_t* scales, int64_t rows, int64_t n, float alpha, int transpose, void* y,
+                  void* workspace, size_t ws_bytes, void* stream);
+
+/* Synchronises `stream`, reads and clears the current device's status word: CP_OK, or
+ * CP_ERR_TIMEOUT when a wait inside an earlier cp_mx4_matmul or cp_mx4_linear ran out (its
+ * result is then incomplete). */
+int cp_mx4_status(void* stream);
 
 #ifdef __cplusplus
 }

@@ -13,11 +13,14 @@ LIB_PATH = os.path.join(_HERE, "libcoldpress_cuda.so")
 
 CP_OK, CP_ERR_TYPE, CP_ERR_SHAPE, CP_ERR_NOT_PD, CP_ERR_CUDA, CP_ERR_ARG, CP_ERR_WORKSPACE, CP_ERR_TIMEOUT = range(8)
 CP_XTX_BF16, CP_XTX_F32 = 0, 1
+MX4_ID = {"MXFP4": 39, "NVFP4": 40}
+CP_MX4_BF16, CP_MX4_F16, CP_MX4_F32 = 0, 1, 2
 
-TYPE_ID = {"Q8_0": 8, "Q2_K": 10, "Q3_K": 11, "Q4_K": 12, "Q5_K": 13, "Q6_K": 14}
+TYPE_ID = {"Q8_0": 8, "Q2_K": 10, "Q3_K": 11, "Q4_K": 12, "Q5_K": 13, "Q6_K": 14, "MXFP4": 39}
 K_TYPES = ("Q2_K", "Q3_K", "Q4_K", "Q5_K", "Q6_K")
-BYTES_PER_BLOCK = {"Q2_K": 84, "Q3_K": 110, "Q4_K": 144, "Q5_K": 176, "Q6_K": 210, "Q8_0": 34}
-BLOCK_ELEMS = {"Q2_K": 256, "Q3_K": 256, "Q4_K": 256, "Q5_K": 256, "Q6_K": 256, "Q8_0": 32}
+BYTES_PER_BLOCK = {"Q2_K": 84, "Q3_K": 110, "Q4_K": 144, "Q5_K": 176, "Q6_K": 210, "Q8_0": 34,
+                   "MXFP4": 17}
+BLOCK_ELEMS = {"Q2_K": 256, "Q3_K": 256, "Q4_K": 256, "Q5_K": 256, "Q6_K": 256, "Q8_0": 32, "MXFP4": 32}
 # (sub-block width, code lo, code hi, has a min), coldpress/ef.py:87-127
 GRID = {"Q2_K": (16, 0, 3, True), "Q3_K": (16, -4, 3, False), "Q4_K": (32, 0, 15, True),
         "Q5_K": (32, 0, 31, True), "Q6_K": (16, -32, 31, False)}
@@ -77,6 +80,7 @@ def lib():
                             f"(the encoder has no CPU fallback)")
     L = ctypes.CDLL(LIB_PATH)
     P, I64, I, D, SZ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_double, ctypes.c_size_t
+    F = ctypes.c_float
     sig = {
         "cp_version": ([], I),
         "cp_last_error": ([], ctypes.c_char_p),
@@ -116,6 +120,15 @@ def lib():
         "cp_fetch_host": ([P, P, I64, P], I),
         "cp_gather_f32": ([P, I64, P, I64, P, I64, P, P], I),
         "cp_col_sqdiff": ([P, P, I64, I64, I64, P, P], I),
+        "cp_mx4_codes_bytes": ([I64, I64], I64),
+        "cp_mx4_scales_bytes": ([I, I64, I64], I64),
+        "cp_mx4_quantize": ([I, I, P, I64, I64, I64, P, F, P, P, P], I),
+        "cp_mx4_dequantize": ([I, P, P, I64, I64, F, I, P, P], I),
+        "cp_mx4_from_gguf": ([P, I64, I64, P, P, P], I),
+        "cp_mx4_matmul": ([I, P, P, I64, P, P, I64, I64, F, I, P, P], I),
+        "cp_mx4_linear_workspace_bytes": ([I, P, I64, I64, I64, I64, I], SZ),
+        "cp_mx4_linear": ([I, I, P, I64, I64, P, P, I64, I64, F, I, P, P, SZ, P], I),
+        "cp_mx4_status": ([P], I),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)

@@ -24,7 +24,7 @@ ROOT = os.path.dirname(HERE)
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
           "-I", os.path.join(ROOT, "include"), "-I", CSRC]
-EXACT_UNITS = {"kquant_encode.cu", "kquant_decode.cu", "ef_sweep.cu"}
+EXACT_UNITS = {"kquant_encode.cu", "kquant_decode.cu", "ef_sweep.cu", "mx4_quant.cu"}
 
 
 def nvcc():

@@ -1,6 +1,7 @@
 // extern "C" entry points of libcoldpress_cuda.so (declared in include/coldpress_cuda.h).
 // Argument checks and workspace carving live here; the kernels are in the other units.
 #include <cuda_runtime.h>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <vector>
@@ -10,6 +11,7 @@
 #include "kquant_kernels.h"
 #include "xtx_kernels.h"
 #include "layout_kernels.h"
+#include "mx4_kernels.h"
 
 static_assert(cpk::kNoAllocScratchBytes == CP_NOALLOC_SCRATCH_BYTES,
               "the public no-allocation limit must equal the scratch array's size");
@@ -44,10 +46,10 @@ int check_rc(int rc, const char* what) {
 
 bool is_k_type(int t) { return t == cpk::kQ2_K || t == cpk::kQ3_K || t == cpk::kQ4_K || t == cpk::kQ5_K || t == cpk::kQ6_K; }
 
-int check_shape(int t, int64_t nrow, int64_t n, bool allow_q80) {
-  if (!(is_k_type(t) || (allow_q80 && t == cpk::kQ8_0)))
-    return set_err(CP_ERR_TYPE, "unsupported ggml type (k-quants Q2_K..Q6_K, and Q8_0 where noted)");
-  const int64_t blk = (t == cpk::kQ8_0) ? 32 : 256;
+int check_shape(int t, int64_t nrow, int64_t n, bool allow_q80, bool allow_mx4 = false) {
+  if (!(is_k_type(t) || (allow_q80 && t == cpk::kQ8_0) || (allow_mx4 && t == cpk::kMXFP4)))
+    return set_err(CP_ERR_TYPE, "unsupported ggml type (k-quants Q2_K..Q6_K, and Q8_0 and MXFP4 where noted)");
+  const int64_t blk = (t == cpk::kQ8_0 || t == cpk::kMXFP4) ? 32 : 256;
   if (nrow < 0 || n <= 0 || n % blk) return set_err(CP_ERR_SHAPE, "n must be a positive multiple of the block size");
   if (nrow > (int64_t)1 << 31 || n > (int64_t)1 << 30) return set_err(CP_ERR_SHAPE, "tensor too large");
   return CP_OK;
@@ -151,17 +153,23 @@ const char* cp_last_error(void) { return g_err; }
 int cp_block_bytes(int ggml_type) { return cpk::block_bytes(ggml_type); }
 
 int cp_kquant_encode(int t, const float* x, int64_t nrow, int64_t n, const float* qw, uint8_t* out, void* stream) {
-  if (int rc = check_shape(t, nrow, n, true)) return rc;
+  if (int rc = check_shape(t, nrow, n, true, true)) return rc;
   if ((!x || !out) && nrow > 0) return set_err(CP_ERR_ARG, "null pointer");
   if (((uintptr_t)x | (uintptr_t)qw) & 15) return set_err(CP_ERR_ARG, "x and qw must be 16-byte aligned");
   if (t != cpk::kQ8_0 && ((uintptr_t)out & 15)) return set_err(CP_ERR_ARG, "out must be 16-byte aligned");
   ProfScope ps(kProfFit, (cudaStream_t)stream);
+  if (t == cpk::kMXFP4)
+    return check_rc(cpk::launch_mx4_encode(x, nrow, n, qw, out, (cudaStream_t)stream), "cp_kquant_encode");
   return check_rc(cpk::launch_quantize(t, x, nrow, n, qw, out, (cudaStream_t)stream), "cp_kquant_encode");
 }
 
 int cp_kquant_decode(int t, const uint8_t* raw, int64_t nrow, int64_t n, float* out, void* stream) {
-  if (int rc = check_shape(t, nrow, n, true)) return rc;
+  if (int rc = check_shape(t, nrow, n, true, true)) return rc;
   if ((!raw || !out) && nrow > 0) return set_err(CP_ERR_ARG, "null pointer");
+  if (t == cpk::kMXFP4) {
+    if (((uintptr_t)raw | (uintptr_t)out) & 15) return set_err(CP_ERR_ARG, "raw and out must be 16-byte aligned");
+    return check_rc(cpk::launch_mx4_decode(raw, nrow, n, out, (cudaStream_t)stream), "cp_kquant_decode");
+  }
   return check_rc(cpk::launch_dequantize(t, raw, nrow, n, out, (cudaStream_t)stream), "cp_kquant_decode");
 }
 
@@ -185,8 +193,13 @@ int cp_kquant_repack(int t, uint8_t* raw, const int8_t* codes, int64_t nrow, int
 
 int cp_weighted_err(int t, const uint8_t* raw, const float* x, const float* w, int64_t nrow, int64_t n, double* out,
                     void* stream) {
-  if (int rc = check_shape(t, nrow, n, false)) return rc;
+  if (int rc = check_shape(t, nrow, n, false, true)) return rc;
   if (!out || ((!raw || !x) && nrow > 0)) return set_err(CP_ERR_ARG, "null pointer");
+  if (t == cpk::kMXFP4) {
+    if ((uintptr_t)raw & 15) return set_err(CP_ERR_ARG, "raw must be 16-byte aligned");
+    if (cudaMemsetAsync(out, 0, sizeof(double), (cudaStream_t)stream) != cudaSuccess) return check_launch("cp_weighted_err");
+    return check_rc(cpk::launch_mx4_weighted_err(raw, x, w, nrow, n, out, (cudaStream_t)stream), "cp_weighted_err");
+  }
   return check_rc(cpk::launch_weighted_err(t, raw, x, w, nrow, n, out, (cudaStream_t)stream), "cp_weighted_err");
 }
 
@@ -330,8 +343,13 @@ int cp_ef_encode(int t, const float* x, int64_t nrow, int64_t n, const int32_t* 
 
 int cp_kquant_encode_batch(int t, const cp_fit_job* jobs, int count, void* stream) {
   if (count < 0 || (count > 0 && !jobs)) return set_err(CP_ERR_ARG, "bad job list");
-  if (!is_k_type(t)) return set_err(CP_ERR_TYPE, "grouped fits support the k-quant types");
   cudaStream_t s = (cudaStream_t)stream;
+  if (t == cpk::kMXFP4) {   // one launch per tensor: a block's fit is short, so nothing is gained by grouping
+    for (int i = 0; i < count; i++)
+      if (int rc = cp_kquant_encode(t, jobs[i].x, jobs[i].nrow, jobs[i].n, jobs[i].qw, jobs[i].out, stream)) return rc;
+    return CP_OK;
+  }
+  if (!is_k_type(t)) return set_err(CP_ERR_TYPE, "grouped fits support the k-quant types and MXFP4");
   for (int pass = 0; pass < 2; pass++) {  // imatrix jobs, then reference-path jobs
     static thread_local cpk::FitBatch b;
     b.count = 0;
@@ -380,8 +398,15 @@ static int block_batch(int op, const cp_block_job* jobs, int count, void* stream
     }
     if (i == count) break;
     const cp_block_job& j = jobs[i];
-    if (int rc = check_shape(j.ggml_type, j.nrow, j.n, false)) return rc;
+    if (int rc = check_shape(j.ggml_type, j.nrow, j.n, false, op == 2)) return rc;
     if (j.nrow == 0) continue;
+    if (j.ggml_type == cpk::kMXFP4) {
+      if (!j.raw || !j.x || !j.err || ((uintptr_t)j.raw & 15))
+        return set_err(CP_ERR_ARG, "null or unaligned pointer in a block job");
+      ProfScope ps(kProfOther, s);
+      if (int rc = check_rc(cpk::launch_mx4_weighted_err(j.raw, j.x, j.w, j.nrow, j.n, j.err, s), what)) return rc;
+      continue;
+    }
     const bool ok = op == 0 ? (j.raw && j.dl) : op == 1 ? (j.raw_out && j.codes) : (j.raw && j.x && j.err);
     if (!ok) return set_err(CP_ERR_ARG, "null pointer in a block job");
     if (op == 0 && j.grid_pitch != 0 && j.grid_pitch < j.nrow) return set_err(CP_ERR_ARG, "grid_pitch < nrow");
@@ -619,6 +644,129 @@ int cp_xtx_status(void* workspace, void* stream) {
   if (cudaMemsetAsync(workspace, 0, 4, s) != cudaSuccess || cudaStreamSynchronize(s) != cudaSuccess)
     return check_launch("cp_xtx_status");
   return set_err(CP_ERR_TIMEOUT, "a bounded wait in cp_xtx_accumulate ran out; H is incomplete");
+}
+
+// ---------------------------------------------------------------------------- 4-bit operands
+
+static int check_mx4(int fmt, int64_t rows, int64_t n) {
+  if (fmt != CP_MXFP4 && fmt != CP_NVFP4) return set_err(CP_ERR_TYPE, "format must be CP_MXFP4 or CP_NVFP4");
+  if (rows < 0 || n <= 0) return set_err(CP_ERR_SHAPE, "rows must not be negative and n must be positive");
+  if (rows > (int64_t)1 << 30 || n > (int64_t)1 << 30 || rows * ((n + 255) / 256) > (int64_t)1 << 34)
+    return set_err(CP_ERR_SHAPE, "operand too large");
+  return CP_OK;
+}
+
+static int check_mx4_dtype(int dtype) {
+  if (dtype != CP_MX4_BF16 && dtype != CP_MX4_F16 && dtype != CP_MX4_F32)
+    return set_err(CP_ERR_TYPE, "dtype must be CP_MX4_BF16, CP_MX4_F16 or CP_MX4_F32");
+  return CP_OK;
+}
+
+static size_t mx4_elem(int dtype) { return dtype == CP_MX4_F32 ? 4 : 2; }
+
+int64_t cp_mx4_codes_bytes(int64_t rows, int64_t n) { return rows > 0 && n > 0 ? rows * cpk::mx4_pitch(n) : 0; }
+
+int64_t cp_mx4_scales_bytes(int fmt, int64_t rows, int64_t n) {
+  return rows > 0 && n > 0 && (fmt == CP_MXFP4 || fmt == CP_NVFP4) ? cpk::mx4_scale_bytes(fmt, rows, n) : 0;
+}
+
+int cp_mx4_quantize(int fmt, int dtype, const void* x, int64_t rows, int64_t n, int64_t ld, const float* qw,
+                    float tensor_scale, uint8_t* codes, uint8_t* scales, void* stream) {
+  if (int rc = check_mx4(fmt, rows, n)) return rc;
+  if (int rc = check_mx4_dtype(dtype)) return rc;
+  if (rows > 1 && ld < n) return set_err(CP_ERR_SHAPE, "cp_mx4_quantize: ld smaller than a row");
+  int e = 0;
+  if (!(tensor_scale > 0.0f) || std::frexp(tensor_scale, &e) != 0.5f || e < -100 || e > 100)
+    return set_err(CP_ERR_ARG, "cp_mx4_quantize: tensor_scale must be a power of two, 2^-100 .. 2^99");
+  if (fmt == CP_MXFP4 && tensor_scale != 1.0f) return set_err(CP_ERR_ARG, "cp_mx4_quantize: MXFP4 has no tensor scale");
+  if (rows == 0) return CP_OK;
+  if (!x || !codes || !scales) return set_err(CP_ERR_ARG, "null pointer");
+  if (((uintptr_t)codes | (uintptr_t)scales) & 15) return set_err(CP_ERR_ARG, "codes and scales must be 16-byte aligned");
+  if ((uintptr_t)x % mx4_elem(dtype) || ((uintptr_t)qw & 3)) return set_err(CP_ERR_ARG, "x or qw is misaligned");
+  ProfScope ps(kProfFit, (cudaStream_t)stream);
+  return check_rc(cpk::launch_mx4_quantize(fmt, dtype, x, rows, n, ld, qw, 1.0f / tensor_scale, codes, scales,
+                                           (cudaStream_t)stream),
+                  "cp_mx4_quantize");
+}
+
+int cp_mx4_dequantize(int fmt, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t n,
+                      float tensor_scale, int dtype, void* out, void* stream) {
+  if (int rc = check_mx4(fmt, rows, n)) return rc;
+  if (int rc = check_mx4_dtype(dtype)) return rc;
+  if (rows == 0) return CP_OK;
+  if (!codes || !scales || !out) return set_err(CP_ERR_ARG, "null pointer");
+  if (((uintptr_t)codes | (uintptr_t)scales) & 15) return set_err(CP_ERR_ARG, "codes and scales must be 16-byte aligned");
+  if ((uintptr_t)out % mx4_elem(dtype)) return set_err(CP_ERR_ARG, "out is misaligned");
+  const cpk::Mx4View v{codes, scales, rows, n, fmt};
+  return check_rc(cpk::launch_mx4_dequantize(v, tensor_scale, dtype, out, (cudaStream_t)stream), "cp_mx4_dequantize");
+}
+
+int cp_mx4_from_gguf(const uint8_t* raw, int64_t nrow, int64_t n, uint8_t* codes, uint8_t* scales, void* stream) {
+  if (int rc = check_mx4(CP_MXFP4, nrow, n)) return rc;
+  if (n % 32) return set_err(CP_ERR_SHAPE, "n must be a positive multiple of the block size");
+  if (nrow == 0) return CP_OK;
+  if (!raw || !codes || !scales) return set_err(CP_ERR_ARG, "null pointer");
+  if (((uintptr_t)codes | (uintptr_t)scales) & 15) return set_err(CP_ERR_ARG, "codes and scales must be 16-byte aligned");
+  return check_rc(cpk::launch_mx4_unpack(raw, nrow, n, codes, scales, (cudaStream_t)stream), "cp_mx4_from_gguf");
+}
+
+int cp_mx4_matmul(int fmt, const uint8_t* a_codes, const uint8_t* a_scales, int64_t a_rows, const uint8_t* w_codes,
+                  const uint8_t* w_scales, int64_t w_rows, int64_t n, float alpha, int dtype, void* y, void* stream) {
+  if (int rc = check_mx4(fmt, a_rows, n)) return rc;
+  if (int rc = check_mx4(fmt, w_rows, n)) return rc;
+  if (int rc = check_mx4_dtype(dtype)) return rc;
+  if (a_rows == 0 || w_rows == 0) return CP_OK;
+  if (!a_codes || !a_scales || !w_codes || !w_scales || !y) return set_err(CP_ERR_ARG, "null pointer");
+  if (((uintptr_t)a_codes | (uintptr_t)a_scales | (uintptr_t)w_codes | (uintptr_t)w_scales) & 15)
+    return set_err(CP_ERR_ARG, "codes and scales must be 16-byte aligned");
+  if ((uintptr_t)y % mx4_elem(dtype)) return set_err(CP_ERR_ARG, "y is misaligned");
+  ProfScope ps(kProfOther, (cudaStream_t)stream);
+  const cpk::Mx4View a{a_codes, a_scales, a_rows, n, fmt}, w{w_codes, w_scales, w_rows, n, fmt};
+  return check_rc(cpk::launch_mx4_matmul(a, w, alpha, dtype, y, (cudaStream_t)stream), "cp_mx4_matmul");
+}
+
+static int mx4_x_aligned(int dtype, const void* x, int64_t ld) {
+  return ((uintptr_t)x & 15) == 0 && (ld * (int64_t)mx4_elem(dtype)) % 16 == 0;
+}
+
+size_t cp_mx4_linear_workspace_bytes(int dtype, const void* x, int64_t T, int64_t ld, int64_t rows, int64_t n,
+                                     int transpose) {
+  if (T <= 0 || rows <= 0 || n <= 0) return 0;
+  return cpk::mx4_linear_workspace_bytes(dtype, T, rows, n, ld, mx4_x_aligned(dtype, x, ld), transpose);
+}
+
+int cp_mx4_linear(int fmt, int dtype, const void* x, int64_t T, int64_t ld, const uint8_t* codes,
+                  const uint8_t* scales, int64_t rows, int64_t n, float alpha, int transpose, void* y,
+                  void* workspace, size_t ws_bytes, void* stream) {
+  if (int rc = check_mx4(fmt, rows, n)) return rc;
+  if (int rc = check_mx4(fmt, T, transpose ? rows + 1 : n)) return rc;
+  if (int rc = check_mx4_dtype(dtype)) return rc;
+  if (T > 1 && ld < (transpose ? rows : n)) return set_err(CP_ERR_SHAPE, "cp_mx4_linear: ld smaller than a row of x");
+  if (T == 0 || (rows == 0 && !transpose)) return CP_OK;
+  if (rows == 0) {   // a sum over no rows
+    if (!y) return set_err(CP_ERR_ARG, "null pointer");
+    if (cudaMemsetAsync(y, 0, (size_t)T * n * mx4_elem(dtype), (cudaStream_t)stream) != cudaSuccess)
+      return check_launch("cp_mx4_linear");
+    return CP_OK;
+  }
+  if (!x || !codes || !scales || !y) return set_err(CP_ERR_ARG, "null pointer");
+  if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)workspace) & 15)
+    return set_err(CP_ERR_ARG, "codes, scales and workspace must be 16-byte aligned");
+  if ((uintptr_t)x % mx4_elem(dtype) || (uintptr_t)y % mx4_elem(dtype)) return set_err(CP_ERR_ARG, "x or y is misaligned");
+  const size_t need = cp_mx4_linear_workspace_bytes(dtype, x, T, ld, rows, n, transpose);
+  if (ws_bytes < need || (need && !workspace))
+    return set_err(CP_ERR_WORKSPACE, "workspace smaller than cp_mx4_linear_workspace_bytes()");
+  ProfScope ps(kProfOther, (cudaStream_t)stream);
+  const cpk::Mx4View w{codes, scales, rows, n, fmt};
+  return check_rc(cpk::launch_mx4_linear(dtype, x, T, ld, w, alpha, transpose, y, workspace, (cudaStream_t)stream),
+                  "cp_mx4_linear");
+}
+
+int cp_mx4_status(void* stream) {
+  int st = 0;
+  if (cpk::mx4_read_status((cudaStream_t)stream, &st) != 0) return check_launch("cp_mx4_status");
+  if (st == 0) return CP_OK;
+  return set_err(CP_ERR_TIMEOUT, "a bounded wait in a 4-bit product ran out; its result is incomplete");
 }
 
 }  // extern "C"

@@ -16,7 +16,7 @@ enum TypeId : int { kQ8_0 = 8, kQ2_K = 10, kQ3_K = 11, kQ4_K = 12, kQ5_K = 13, k
 
 __host__ __device__ constexpr int block_bytes(int t) {
   return t == kQ2_K ? 84 : t == kQ3_K ? 110 : t == kQ4_K ? 144 : t == kQ5_K ? 176
-       : t == kQ6_K ? 210 : t == kQ8_0 ? 34 : 0;
+       : t == kQ6_K ? 210 : t == kQ8_0 ? 34 : t == 39 ? 17 /* MXFP4 */ : 0;
 }
 
 // nearest_int (kquant.py:25-28): magic add, low 23 bits, re-centre.  A NaN sum is treated

@@ -1,0 +1,466 @@
+// Quantisation to microscaled 4-bit operands and back (layout and rounding: mx4_format.cuh), and
+// the GGUF MXFP4 container.
+//
+// Bound by memory: a bf16 activation matrix costs 2 bytes a value to read and 17/32 or 9/16 to
+// write.  One warp takes 256 columns (a lane 8 of them, so loads and code stores are whole
+// 128-byte lines) of up to four rows 32 apart: those rows' scale bytes are neighbours in the scale
+// tile, so a group of four blocks leaves as one 16-byte store, and the four rows' loads are in
+// flight together.
+//
+// Importance-weighted scales.  For weights with column weights qw a block tries several scales
+// and keeps the one with the least sum of qw (x - q s)^2: MXFP4 the exponents e, e + 1 and
+// e - 1, NVFP4 the codes c, c + 1, c - 1, c + 2, c - 2, c + 3, c + 4, c + 5 (c + 4 and c + 5
+// map the maximum to 4 instead of 6).  Ties go to the first.  The choice is defined by the sums in 64
+// bits; float32 sums decide it unless two candidates are within 2^-16 of each other (their
+// error is below 2^-19), and only then are the sums formed again in 64 bits.
+#include <cuda_runtime.h>
+#include "kquant_kernels.h"
+#include "mx4_format.cuh"
+
+namespace cpk {
+namespace {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+
+// Eight consecutive values of a row; left = values of the row from here on (may be <= 0).
+template <typename T> __device__ __forceinline__ void load8(const T* p, int64_t left, bool vec, float (&v)[8]) {
+  if (vec && left >= 8) {
+    constexpr int W = sizeof(T) * 8 / 16;
+    uint4 w[W];
+#pragma unroll
+    for (int i = 0; i < W; i++) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = to_f32(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = i < left ? to_f32(p[i]) : 0.0f;
+  }
+}
+
+template <int FMT> __host__ __device__ constexpr int mx_candidates() { return FMT == kMXFP4 ? 3 : 8; }
+template <int FMT> __device__ __forceinline__ int mx_candidate(int first, int c) {
+  constexpr int kMx[3] = {0, 1, -1};
+  constexpr int kNv[8] = {0, 1, -1, 2, -2, 3, 4, 5};
+  const int b = first + (FMT == kMXFP4 ? kMx[c < 3 ? c : 0] : kNv[c]);
+  return min(max(b, 0), FMT == kMXFP4 ? 253 : 126);
+}
+
+// Sum over the lanes of a block.
+template <int FMT, typename T> __device__ __forceinline__ T block_sum(T e) {
+  e += __shfl_xor_sync(0xffffffffu, e, 1);
+  if (FMT == kMXFP4) e += __shfl_xor_sync(0xffffffffu, e, 2);
+  return e;
+}
+
+// Scale byte and codes of a block (8 values per lane; v already divided by the tensor scale).
+template <int FMT, bool IMAT>
+__device__ __forceinline__ uint32_t quantize_block(const float (&v)[8], const float (&w)[8], int& byte) {
+  const uint32_t m = mx_block_max<FMT>(v);
+  byte = mx_first_scale<FMT>(m);
+  const bool finite = m < 0x7F800000u;   // else the scale byte is NaN and the block decodes to NaN
+  uint32_t code = mx_codes<FMT>(v, byte);
+  if constexpr (IMAT) {
+    constexpr int C = mx_candidates<FMT>();
+    const int first = byte;
+    // differences in units of the block's maximum, so that their squares neither vanish nor overflow
+    const int mexp = max((int)(m >> 23), 1);
+    const float unit = __uint_as_float((uint32_t)min(max(254 - mexp, 1), 253) << 23);
+    float err[C];
+    uint32_t codes[C];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      const int b = mx_candidate<FMT>(first, c);
+      const float s = mx_scale_value<FMT>(b);
+      codes[c] = c == 0 ? code : mx_codes<FMT>(v, b);
+      float e = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float2 q = e2m1x2_value(codes[c] >> (8 * i));
+        const float d0 = __fmul_rn(__fmaf_rn(-q.x, s, v[2 * i]), unit);
+        const float d1 = __fmul_rn(__fmaf_rn(-q.y, s, v[2 * i + 1]), unit);
+        e = __fadd_rn(e, __fmul_rn(w[2 * i], __fmul_rn(d0, d0)));
+        e = __fadd_rn(e, __fmul_rn(w[2 * i + 1], __fmul_rn(d1, d1)));
+      }
+      err[c] = block_sum<FMT>(e);
+    }
+    int pick = 0;
+    float best = err[0];
+#pragma unroll
+    for (int c = 1; c < C; c++)
+      if (err[c] < best) best = err[c], pick = c;
+    // near: some other candidate is as good as the float32 sums can tell, or the sums are out of
+    // float32's range
+    bool near = !(best > 1e-30f && best < 1e30f);
+#pragma unroll
+    for (int c = 0; c < C; c++) near |= c != pick && err[c] <= best * 1.0000153f;
+    near = near && first > 0 && finite;
+    if (__any_sync(0xffffffffu, near)) {
+      double bd = 0.0;
+      int pd = 0;
+#pragma unroll 1
+      for (int c = 0; c < C; c++) {
+        const int b = mx_candidate<FMT>(first, c);
+        const double s = (double)mx_scale_value<FMT>(b);
+        const uint32_t cw = mx_codes<FMT>(v, b);
+        double e = 0.0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float2 q = e2m1x2_value(cw >> (8 * i));
+          const double d0 = (double)v[2 * i] - (double)q.x * s, d1 = (double)v[2 * i + 1] - (double)q.y * s;
+          e += (double)w[2 * i] * (d0 * d0);
+          e += (double)w[2 * i + 1] * (d1 * d1);
+        }
+        e = block_sum<FMT>(e);
+        if (c == 0 || e < bd) bd = e, pd = c;
+      }
+      if (near) pick = pd;
+    }
+    if (first > 0 && finite) {   // scale byte 0 (an all but empty block) is not searched
+      byte = mx_candidate<FMT>(first, pick);
+#pragma unroll
+      for (int c = 0; c < C; c++)
+        if (c == pick) code = codes[c];
+    }
+  }
+  return finite ? code : 0;
+}
+
+constexpr int kWarps = 8;
+
+// Units (row lane r of a row tile, 256-column chunk), one per warp.
+template <typename T, int FMT, bool IMAT>
+__global__ void __launch_bounds__(32 * kWarps)
+    quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t n, int64_t ld, const float* __restrict__ qw,
+                    float inv_scale, int chunks, int64_t units, bool vec, uint8_t* __restrict__ codes,
+                    uint8_t* __restrict__ scales) {
+  const int64_t unit = blockIdx.x * (int64_t)kWarps + threadIdx.x / 32;
+  if (unit >= units) return;
+  const int lane = threadIdx.x % 32;
+  const int64_t rl = unit / chunks;                 // 32 row lanes per tile of 128 rows
+  const int chunk = (int)(unit - rl * chunks);
+  const int64_t row0 = (rl >> 5) * 128 + (rl & 31);
+  const int64_t col = (int64_t)chunk * 256 + lane * 8, left = n - col;
+  float v[4][8], w[8];
+#pragma unroll
+  for (int j = 0; j < 4; j++) load8(x + (row0 + 32 * j) * ld + col, row0 + 32 * j < rows ? left : 0, vec, v[j]);
+  if constexpr (IMAT) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = i < left ? __ldg(qw + col + i) : 0.0f;
+  }
+  constexpr int LB = mx_block<FMT>() / 8;   // lanes per block
+  uint32_t sb[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    if (FMT == kNVFP4) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[j][i] = __fmul_rn(v[j][i], inv_scale);
+    }
+    int byte;
+    const uint32_t code = quantize_block<FMT, IMAT>(v[j], w, byte);
+    if (row0 + 32 * j < rows)
+      *reinterpret_cast<uint32_t*>(codes + (row0 + 32 * j) * (int64_t)chunks * 128 + chunk * 128 + lane * 4) = code;
+    // the four bytes of a group of four blocks, gathered into its first lane
+    uint32_t b = (uint32_t)byte;
+    b |= __shfl_down_sync(0xffffffffu, b, LB) << 8;
+    b |= __shfl_down_sync(0xffffffffu, b, 2 * LB) << 16;
+    sb[j] = b;
+  }
+  if (lane % (4 * LB) == 0) {
+    const int64_t groups = (int64_t)chunks * (256 / (32 * LB));
+    const int64_t g = (int64_t)chunk * (256 / (32 * LB)) + lane / (4 * LB);
+    *reinterpret_cast<uint4*>(scales + ((row0 >> 7) * groups + g) * 512 + (row0 & 31) * 16) =
+        make_uint4(sb[0], sb[1], sb[2], sb[3]);
+  }
+}
+
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+
+template <typename T, int FMT>
+__global__ void __launch_bounds__(32 * kWarps)
+    dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows, int64_t n,
+                      float scale, int chunks, int64_t units, bool vec, T* __restrict__ out) {
+  const int64_t unit = blockIdx.x * (int64_t)kWarps + threadIdx.x / 32;
+  if (unit >= units) return;
+  const int lane = threadIdx.x % 32;
+  const int64_t rl = unit / chunks;
+  const int chunk = (int)(unit - rl * chunks);
+  const int64_t row0 = (rl >> 5) * 128 + (rl & 31);
+  const int64_t col = (int64_t)chunk * 256 + lane * 8, left = n - col;
+  if (left <= 0) return;
+  constexpr int LB = mx_block<FMT>() / 8;
+  const int64_t groups = (int64_t)chunks * (256 / (32 * LB));
+  const int64_t g = (int64_t)chunk * (256 / (32 * LB)) + lane / (4 * LB);
+  const uint4 sw = __ldg(reinterpret_cast<const uint4*>(scales + ((row0 >> 7) * groups + g) * 512 + (row0 & 31) * 16));
+  const uint32_t sj[4] = {sw.x, sw.y, sw.z, sw.w};
+  uint32_t c[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    c[j] = row0 + 32 * j < rows ? __ldg(reinterpret_cast<const uint32_t*>(
+                                      codes + (row0 + 32 * j) * (int64_t)chunks * 128 + chunk * 128 + lane * 4))
+                                : 0;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int64_t row = row0 + 32 * j;
+    if (row >= rows) break;
+    const float s = mx_scale_value<FMT>((sj[j] >> (8 * (lane / LB % 4))) & 0xFF);
+    T o[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 q = e2m1x2_value(c[j] >> (8 * i));
+      // q s is exact, so the tensor scale's product is the only rounding before the type's own
+      put(o + 2 * i, __fmul_rn(__fmul_rn(q.x, s), scale));
+      put(o + 2 * i + 1, __fmul_rn(__fmul_rn(q.y, s), scale));
+    }
+    T* p = out + row * n + col;
+    if (vec && left >= 8) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(o)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (i < left) p[i] = o[i];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------- GGUF container
+// Blocks of 32: the scale byte, then 16 bytes whose low halves are values 0-15 and whose high
+// halves are values 16-31.  Blocks follow one another through the whole tensor, so the kernels
+// take them flat, 256 per CTA: 4352 bytes, staged in shared memory and moved 16 bytes at a time.
+constexpr int kBlkBytes = 17, kCtaBlocks = 256;
+
+// Nibbles of a and b interleaved into bytes a_i | b_i << 4, for i = 0..3 (lo) and 4..7 (hi).
+__device__ __forceinline__ uint32_t spread16(uint32_t h) {   // 4 nibbles -> 4 bytes
+  h = (h | (h << 8)) & 0x00FF00FFu;
+  return (h | (h << 4)) & 0x0F0F0F0Fu;
+}
+
+template <bool IMAT>
+__global__ void __launch_bounds__(256) encode_kernel(const float* __restrict__ x, int64_t nblk, int nb_row,
+                                                     const float* __restrict__ qw, uint8_t* __restrict__ out) {
+  __shared__ __align__(16) uint8_t stage[kCtaBlocks * kBlkBytes];
+  const int64_t b0 = (int64_t)blockIdx.x * kCtaBlocks;
+  const int t = threadIdx.x, l4 = t & 3;
+  float v[4][8];
+#pragma unroll
+  for (int p = 0; p < 4; p++) {
+    const int64_t b = b0 + p * 64 + (t >> 2);
+    load8(x + b * 32 + l4 * 8, b < nblk ? 8 : 0, true, v[p]);
+  }
+#pragma unroll
+  for (int p = 0; p < 4; p++) {
+    const int lb = p * 64 + (t >> 2);
+    const int64_t b = b0 + lb;
+    float w[8];
+    if constexpr (IMAT) load8(qw + (b % nb_row) * 32 + l4 * 8, b < nblk ? 8 : 0, true, w);
+    int byte;
+    const uint32_t c = quantize_block<kMXFP4, IMAT>(v[p], w, byte);
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, c, 2);   // values 16 further (lanes 0, 1)
+    if (l4 < 2) {
+      const uint32_t lo = spread16(c & 0xFFFF) | spread16(other & 0xFFFF) << 4;
+      const uint32_t hi = spread16(c >> 16) | spread16(other >> 16) << 4;
+      uint8_t* q = stage + lb * kBlkBytes + 1 + l4 * 8;
+#pragma unroll
+      for (int i = 0; i < 4; i++) q[i] = (uint8_t)(lo >> (8 * i)), q[4 + i] = (uint8_t)(hi >> (8 * i));
+      if (l4 == 0) stage[lb * kBlkBytes] = (uint8_t)byte;
+    }
+  }
+  __syncthreads();
+  const int64_t left = nblk - b0;
+  const int bytes = (int)(left < kCtaBlocks ? left : kCtaBlocks) * kBlkBytes;
+  uint8_t* dst = out + b0 * kBlkBytes;
+  for (int i = t; i < bytes / 16; i += 256) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(stage)[i];
+  if (t < bytes % 16) dst[bytes / 16 * 16 + t] = stage[bytes / 16 * 16 + t];
+}
+
+// Brings a CTA's blocks into shared memory.
+__device__ __forceinline__ int load_blocks(const uint8_t* __restrict__ raw, int64_t nblk, int64_t b0, uint8_t* stage) {
+  const int64_t left = nblk - b0;
+  const int bytes = (int)(left < kCtaBlocks ? left : kCtaBlocks) * kBlkBytes;
+  const uint8_t* src = raw + b0 * kBlkBytes;
+  for (int i = threadIdx.x; i < bytes / 16; i += 256)
+    reinterpret_cast<uint4*>(stage)[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+  if ((int)threadIdx.x < bytes % 16) stage[bytes / 16 * 16 + threadIdx.x] = src[bytes / 16 * 16 + threadIdx.x];
+  __syncthreads();
+  return bytes / kBlkBytes;
+}
+
+// Values 8 l4 .. 8 l4 + 7 of a staged block.
+__device__ __forceinline__ void block_values(const uint8_t* blk, int l4, float (&v)[8]) {
+  const float s = e8m0_value(blk[0]);
+  const uint8_t* q = blk + 1 + (l4 & 1) * 8;
+  const int sh = l4 >= 2 ? 4 : 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] = __fmul_rn(e2m1x2_value((q[i] >> sh) & 15).x, s);
+}
+
+__global__ void __launch_bounds__(256) decode_kernel(const uint8_t* __restrict__ raw, int64_t nblk,
+                                                     float* __restrict__ out) {
+  __shared__ __align__(16) uint8_t stage[kCtaBlocks * kBlkBytes];
+  const int64_t b0 = (int64_t)blockIdx.x * kCtaBlocks;
+  const int n = load_blocks(raw, nblk, b0, stage);
+  const int t = threadIdx.x;
+#pragma unroll
+  for (int p = 0; p < 4; p++) {
+    const int lb = p * 64 + (t >> 2);
+    if (lb >= n) break;
+    float v[8];
+    block_values(stage + lb * kBlkBytes, t & 3, v);
+    float4* dst = reinterpret_cast<float4*>(out + (b0 + lb) * 32 + (t & 3) * 8);
+    dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+    dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+// *err += sum of w (x - value)^2 in 64 bits, one atomic per CTA.
+__global__ void __launch_bounds__(256) weighted_err_kernel(const uint8_t* __restrict__ raw, const float* __restrict__ x,
+                                                           const float* __restrict__ w, int64_t nblk, int nb_row,
+                                                           double* __restrict__ err) {
+  __shared__ __align__(16) uint8_t stage[kCtaBlocks * kBlkBytes];
+  __shared__ double part[8];
+  const int64_t b0 = (int64_t)blockIdx.x * kCtaBlocks;
+  const int n = load_blocks(raw, nblk, b0, stage);
+  const int t = threadIdx.x;
+  double e = 0.0;
+  for (int p = 0; p < 4; p++) {
+    const int lb = p * 64 + (t >> 2);
+    if (lb >= n) break;
+    float v[8];
+    block_values(stage + lb * kBlkBytes, t & 3, v);
+    const int64_t b = b0 + lb;
+    for (int i = 0; i < 8; i++) {
+      const int k = (t & 3) * 8 + i;
+      const double d = (double)v[i] - (double)x[b * 32 + k];
+      e += d * d * (w ? (double)w[(b % nb_row) * 32 + k] : 1.0);
+    }
+  }
+  for (int o = 16; o; o >>= 1) e += __shfl_down_sync(0xffffffffu, e, o);
+  if (t % 32 == 0) part[t / 32] = e;
+  __syncthreads();
+  if (t == 0) {
+    for (int i = 1; i < 8; i++) e += part[i];
+    atomicAdd(err, e);
+  }
+}
+
+// Container -> operand: one thread per block of the padded row (blocks past n: zero).
+__global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* __restrict__ raw, int64_t nrow, int nb_row, int nb_pad,
+                                                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  const int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x;
+  if (i >= nrow * nb_pad) return;
+  const int64_t row = i / nb_pad;
+  const int b = (int)(i - row * nb_pad);
+  uint32_t o[4] = {0, 0, 0, 0};
+  uint8_t s = 0;
+  if (b < nb_row) {
+    const uint8_t* src = raw + (row * nb_row + b) * kBlkBytes;
+    s = src[0];
+#pragma unroll
+    for (int j = 0; j < 16; j++) {   // value j: low half, nibble j of the row; value j + 16: high half
+      const uint32_t q = src[1 + j];
+      o[j >> 3] |= (q & 15) << (4 * (j & 7));
+      o[2 + (j >> 3)] |= (q >> 4) << (4 * (j & 7));
+    }
+  }
+  *reinterpret_cast<uint4*>(codes + i * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+  scales[mx_scale_offset(row, b, nb_pad / 4)] = s;
+}
+
+int64_t row_lanes(int64_t rows) { return rows / 128 * 32 + (rows % 128 < 32 ? rows % 128 : 32); }
+
+template <typename T>
+int quantize_typed(int fmt, const T* x, int64_t rows, int64_t n, int64_t ld, const float* qw, float inv_scale,
+                   uint8_t* codes, uint8_t* scales, cudaStream_t stream) {
+  const int chunks = (int)((n + 255) / 256);
+  const int64_t units = row_lanes(rows) * chunks;
+  const unsigned grid = (unsigned)((units + kWarps - 1) / kWarps);
+  const bool vec = ((uintptr_t)x & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
+#define CPK_Q(F, I) \
+  quantize_kernel<T, F, I><<<grid, 32 * kWarps, 0, stream>>>(x, rows, n, ld, qw, inv_scale, chunks, units, vec, codes, scales)
+  if (fmt == kMXFP4) {
+    if (qw) CPK_Q(kMXFP4, true);
+    else CPK_Q(kMXFP4, false);
+  } else {
+    if (qw) CPK_Q(kNVFP4, true);
+    else CPK_Q(kNVFP4, false);
+  }
+#undef CPK_Q
+  note_launch();
+  return 0;
+}
+
+template <typename T> int dequantize_typed(const Mx4View& v, float scale, T* out, cudaStream_t stream) {
+  const int chunks = (int)((v.n + 255) / 256);
+  const int64_t units = row_lanes(v.rows) * chunks;
+  const unsigned grid = (unsigned)((units + kWarps - 1) / kWarps);
+  const bool vec = ((uintptr_t)out & 15) == 0 && (v.n * sizeof(T)) % 16 == 0;
+  if (v.fmt == kMXFP4)
+    dequantize_kernel<T, kMXFP4><<<grid, 32 * kWarps, 0, stream>>>(v.codes, v.scales, v.rows, v.n, scale, chunks, units, vec, out);
+  else
+    dequantize_kernel<T, kNVFP4><<<grid, 32 * kWarps, 0, stream>>>(v.codes, v.scales, v.rows, v.n, scale, chunks, units, vec, out);
+  note_launch();
+  return 0;
+}
+
+}  // namespace
+
+int launch_mx4_quantize(int fmt, int dtype, const void* x, int64_t rows, int64_t n, int64_t ld, const float* qw,
+                        float inv_scale, uint8_t* codes, uint8_t* scales, cudaStream_t stream) {
+  if (rows == 0) return 0;
+  if (dtype == kMxBF16)
+    return quantize_typed(fmt, static_cast<const __nv_bfloat16*>(x), rows, n, ld, qw, inv_scale, codes, scales, stream);
+  if (dtype == kMxF16)
+    return quantize_typed(fmt, static_cast<const __half*>(x), rows, n, ld, qw, inv_scale, codes, scales, stream);
+  return quantize_typed(fmt, static_cast<const float*>(x), rows, n, ld, qw, inv_scale, codes, scales, stream);
+}
+
+int launch_mx4_dequantize(const Mx4View& v, float scale, int dtype, void* out, cudaStream_t stream) {
+  if (v.rows == 0) return 0;
+  if (dtype == kMxBF16) return dequantize_typed(v, scale, static_cast<__nv_bfloat16*>(out), stream);
+  if (dtype == kMxF16) return dequantize_typed(v, scale, static_cast<__half*>(out), stream);
+  return dequantize_typed(v, scale, static_cast<float*>(out), stream);
+}
+
+int launch_mx4_encode(const float* x, int64_t nrow, int64_t n, const float* qw, uint8_t* out, cudaStream_t stream) {
+  const int64_t nblk = nrow * (n / 32);
+  if (nblk == 0) return 0;
+  const unsigned grid = (unsigned)((nblk + kCtaBlocks - 1) / kCtaBlocks);
+  if (qw) encode_kernel<true><<<grid, 256, 0, stream>>>(x, nblk, (int)(n / 32), qw, out);
+  else encode_kernel<false><<<grid, 256, 0, stream>>>(x, nblk, (int)(n / 32), qw, out);
+  note_launch();
+  return 0;
+}
+
+int launch_mx4_decode(const uint8_t* raw, int64_t nrow, int64_t n, float* out, cudaStream_t stream) {
+  const int64_t nblk = nrow * (n / 32);
+  if (nblk == 0) return 0;
+  decode_kernel<<<(unsigned)((nblk + kCtaBlocks - 1) / kCtaBlocks), 256, 0, stream>>>(raw, nblk, out);
+  note_launch();
+  return 0;
+}
+
+int launch_mx4_weighted_err(const uint8_t* raw, const float* x, const float* w, int64_t nrow, int64_t n, double* err,
+                            cudaStream_t stream) {
+  const int64_t nblk = nrow * (n / 32);
+  if (nblk == 0) return 0;
+  weighted_err_kernel<<<(unsigned)((nblk + kCtaBlocks - 1) / kCtaBlocks), 256, 0, stream>>>(raw, x, w, nblk, (int)(n / 32), err);
+  note_launch();
+  return 0;
+}
+
+int launch_mx4_unpack(const uint8_t* raw, int64_t nrow, int64_t n, uint8_t* codes, uint8_t* scales,
+                      cudaStream_t stream) {
+  if (nrow == 0) return 0;
+  const int nb = (int)(n / 32), nbp = (int)((n + 255) / 256 * 8);
+  const int64_t total = nrow * nbp;
+  unpack_kernel<<<(unsigned)((total + 255) / 256), 256, 0, stream>>>(raw, nrow, nb, nbp, codes, scales);
+  note_launch();
+  return 0;
+}
+
+}  // namespace cpk

@@ -225,7 +225,7 @@ def encode_gguf(f16_path, target_path, hessdir, out_path, imatrix_path=None, per
             if p is not None:
                 fit_w = fit_w[p]
             plan.append((name, tt, "wRTN(attn0-diag)", qw, None, fit_w, p))
-        elif gguf_io.has_hessian(hessdir, name):
+        elif gguf_io.has_hessian(hessdir, name) and tt != "MXFP4":   # error feedback covers the k-quants
             if tt not in nat.K_TYPES:
                 raise ValueError(tt)  # ef.py:_grid_params supports the k-quants only
             plan.append((name, tt, "EF" if not unsafe_storage_order else "EF(storage-order)", qw, name, None, p))

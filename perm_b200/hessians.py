@@ -79,6 +79,7 @@ def build_name_map(model, arch, n_layers):
     """{module_name: gguf_base_name} through gguf's TensorNameMap, as hessians.py:64-82."""
     import gguf
     import torch.nn as nn
+    from .mx4 import Linear as Linear4
     inv = {v: k for k, v in gguf.MODEL_ARCH_NAMES.items()}
     enum = inv.get(arch)
     if enum is None:
@@ -87,7 +88,7 @@ def build_name_map(model, arch, n_layers):
     nm = gguf.get_tensor_name_map(enum, n_layers)
     out = {}
     for name, mod in model.named_modules():
-        if isinstance(mod, (nn.Linear, nn.Embedding)):
+        if isinstance(mod, (nn.Linear, nn.Embedding, Linear4)):
             g = nm.get_name(name)
             if g is not None:
                 out[name] = g
@@ -97,17 +98,20 @@ def build_name_map(model, arch, n_layers):
 def collect_hessians(model, batches, gguf_ne0, arch, n_layers, layer_lo=0, layer_hi=None,
                      progress_every=16, log=print, share_inputs=True):
     """Same contract as coldpress.hessians.collect_hessians; X^T X accumulates on the device.
+    Matmuls already encoded to 4 bits (mx4.Linear) are hooked like the others, so what follows
+    them is calibrated on the encoded model's activations.
 
     Returns ({gguf_name: {"H": float32 [d, d] numpy, "n": int}}, unmapped)."""
     import torch
     import torch.nn as nn
+    from .mx4 import Linear as Linear4
     if layer_hi is None:
         layer_hi = n_layers
     name_map = build_name_map(model, arch, n_layers)
     acc, cnt, alias = {}, {}, {}
     unmapped, mismatched, plan = [], [], []
     for mname, mod in model.named_modules():
-        if not isinstance(mod, (nn.Linear, nn.Embedding)):
+        if not isinstance(mod, (nn.Linear, nn.Embedding, Linear4)):
             continue
         base = name_map.get(mname)
         if base is None:
@@ -121,7 +125,7 @@ def collect_hessians(model, batches, gguf_ne0, arch, n_layers, layer_lo=0, layer
         in_shard = (layer_lo <= blk < layer_hi) if blk >= 0 else (layer_lo == 0)
         if not in_shard:
             continue
-        if isinstance(mod, nn.Linear) and mod.in_features != gguf_ne0[gname]:
+        if isinstance(mod, (nn.Linear, Linear4)) and mod.in_features != gguf_ne0[gname]:
             mismatched.append((mname, gname, mod.in_features, gguf_ne0[gname]))
             continue
         plan.append((mod, gname))

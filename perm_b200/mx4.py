@@ -1,0 +1,262 @@
+"""Microscaled 4-bit operands: quantisation, products with them, and the products' gradient.
+
+    from perm_b200 import mx4
+    w = mx4.quantize(W, "MXFP4", qw)           # frozen weights [out, n], importance-weighted scales
+    y = mx4.linear(x, w)                       # x bf16 / f16 / f32 [..., n] -> [..., out]; x gets a gradient
+    a = mx4.quantize(x, "MXFP4")               # activations in 4 bits
+    y = mx4.matmul(a, w, torch.bfloat16)       # both operands in 4 bits
+
+Values are e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign) times a block scale: "MXFP4" has blocks of
+32 with an e8m0 scale (a power of two), "NVFP4" blocks of 16 with an e4m3 scale and one tensor
+scale.  A block of MXFP4 takes the exponent floor(log2 max) - 2, one of NVFP4 the e4m3 nearest to
+max / 6 / tensor_scale; values round to nearest even and saturate at 6.  With column weights qw
+(as kquant's imatrix path has them) each block tries several scales and keeps the one with the
+least sum of qw (x - value)^2, formed in 64 bits.  A NaN or an infinity makes its block NaN.
+
+The GGUF container of MXFP4 is in kquant (QUANTIZE["MXFP4"], DEQUANTIZE["MXFP4"]); from_gguf
+turns its bytes into an operand.
+
+Calls only enqueue work on the current stream of the tensors' device, and every tensor of a call
+is on that device.  Products accumulate in float32 and round once.  Their kernels bound every
+wait; status() raises if one ran out.
+"""
+import math
+
+import torch
+
+from . import _native as nat
+
+BLOCK = {"MXFP4": 32, "NVFP4": 16}
+_DTYPE = {torch.bfloat16: nat.CP_MX4_BF16, torch.float16: nat.CP_MX4_F16, torch.float32: nat.CP_MX4_F32}
+
+
+class Mx4Tensor:
+    """A 4-bit operand [rows, n].
+
+    codes   uint8 [rows, P/2], P = n rounded up to 256: element 2j of a row in the low half of
+            byte j, zero past n
+    scales  uint8, tiles of 128 rows x 4 blocks, [ceil(rows/128), P/(4 block), 32, 4, 4]: entry
+            [i, g, r, j, k] is the scale of row 128 i + 32 j + r, block 4 g + k; zero past n
+    tensor_scale  a positive float that multiplies every value"""
+    __slots__ = ("codes", "scales", "fmt", "rows", "n", "tensor_scale")
+
+    def __init__(self, codes, scales, fmt, rows, n, tensor_scale=1.0):
+        if fmt not in BLOCK:
+            raise ValueError(f"unknown 4-bit format {fmt!r}")
+        pitch = (n + 255) // 256 * 128
+        if rows < 0 or n <= 0 or codes.dtype != torch.uint8 or codes.shape != (rows, pitch) or not codes.is_contiguous():
+            raise ValueError(f"codes must be a contiguous uint8 [{rows}, {pitch}]")
+        if scales.dtype != torch.uint8 or not scales.is_contiguous() or \
+                scales.numel() != (rows + 127) // 128 * 256 * pitch // BLOCK[fmt]:
+            raise ValueError(f"scales must be contiguous uint8 tiles of {rows} rows and {pitch * 2 // BLOCK[fmt]} blocks")
+        if codes.device != scales.device:
+            raise ValueError("codes and scales must be on one device")
+        if not (tensor_scale > 0.0 and math.isfinite(tensor_scale)):
+            raise ValueError("tensor_scale must be positive and finite")
+        self.codes, self.scales, self.fmt, self.rows, self.n = codes, scales, fmt, rows, n
+        self.tensor_scale = tensor_scale
+
+    @property
+    def shape(self):
+        return (self.rows, self.n)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def __repr__(self):
+        return f"Mx4Tensor({self.fmt}, [{self.rows}, {self.n}], tensor_scale={self.tensor_scale}, device={self.device})"
+
+
+def _need_cuda(t, what):
+    if not t.is_cuda:
+        raise nat.CudaPathError(f"{what}: tensors must be on a CUDA device")
+
+
+def _call(dev, fn, what, *args):
+    """fn(*args, stream) on `dev`'s current stream, with `dev` current."""
+    idx = dev.index
+    if idx == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(idx).cuda_stream)
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, torch.cuda.current_stream(idx).cuda_stream)
+    if rc:
+        nat.check(rc, what)
+
+
+def _empty_operand(fmt, rows, n, dev):
+    pitch = (n + 255) // 256 * 128
+    codes = torch.empty((rows, pitch), dtype=torch.uint8, device=dev)
+    scales = torch.empty(((rows + 127) // 128, pitch // (2 * BLOCK[fmt]), 32, 4, 4), dtype=torch.uint8, device=dev)
+    return codes, scales
+
+
+def tensor_scale_for(x):
+    """A power of two g for quantize(x, "NVFP4", tensor_scale=g): the least with
+    max |x| / (6 g) <= 448, so the largest block scale uses e4m3's range.  Reads x on the host."""
+    m = float(x.detach().abs().amax()) if x.numel() else 0.0
+    if not math.isfinite(m):
+        raise ValueError("tensor_scale_for: x has values that are not finite")
+    if m == 0.0:
+        return 1.0
+    f, e = math.frexp(m / (6.0 * 448.0))
+    return math.ldexp(1.0, max(-99, min(99, e - 1 if f == 0.5 else e)))
+
+
+def quantize(x, fmt, qw=None, tensor_scale=1.0):
+    """x [rows, n] (bf16, f16 or f32; any row stride) -> Mx4Tensor.  qw: non-negative column
+    weights [n], or None.  tensor_scale: a power of two (1 for MXFP4)."""
+    if fmt not in BLOCK:
+        raise ValueError(f"unknown 4-bit format {fmt!r}")
+    _need_cuda(x, "mx4.quantize")
+    dt = _DTYPE.get(x.dtype)
+    if dt is None or x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError("mx4.quantize expects a bf16, f16 or f32 matrix [rows, n], n > 0")
+    rows, n = x.shape
+    if x.stride(1) != 1 and n > 1 or rows > 1 and x.stride(0) < n:
+        x = x.contiguous()
+    if qw is not None:
+        if qw.shape != (n,) or qw.device != x.device:
+            raise ValueError(f"qw must hold {n} column weights on x's device")
+        qw = qw.to(torch.float32).contiguous()
+    codes, scales = _empty_operand(fmt, rows, n, x.device)
+    _call(x.device, nat.lib().cp_mx4_quantize, "mx4.quantize", nat.MX4_ID[fmt], dt, x.data_ptr(), rows, n, x.stride(0),
+          None if qw is None else qw.data_ptr(), tensor_scale, codes.data_ptr(), scales.data_ptr())
+    return Mx4Tensor(codes, scales, fmt, rows, n, tensor_scale)
+
+
+def dequantize(q, dtype=torch.float32):
+    """The values of an operand, [rows, n] in `dtype` (bf16, f16 or f32)."""
+    dt = _DTYPE.get(dtype)
+    if dt is None:
+        raise ValueError("mx4.dequantize: dtype must be bf16, f16 or f32")
+    _need_cuda(q.codes, "mx4.dequantize")
+    out = torch.empty((q.rows, q.n), dtype=dtype, device=q.device)
+    _call(q.device, nat.lib().cp_mx4_dequantize, "mx4.dequantize", nat.MX4_ID[q.fmt], q.codes.data_ptr(),
+          q.scales.data_ptr(), q.rows, q.n, q.tensor_scale, dt, out.data_ptr())
+    return out
+
+
+def from_gguf(raw, n):
+    """GGUF MXFP4 bytes (uint8 CUDA [rows, n/32 * 17], as kquant.QUANTIZE["MXFP4"] gives) -> Mx4Tensor."""
+    _need_cuda(raw, "mx4.from_gguf")
+    if n <= 0 or n % 32:
+        raise ValueError(f"cannot reshape a row of {n} values into 32-value blocks")
+    if raw.dtype != torch.uint8 or raw.dim() != 2 or raw.shape[1] != n // 32 * 17:
+        raise ValueError(f"raw must be uint8 [rows, {n // 32 * 17}]")
+    raw = raw.contiguous()
+    codes, scales = _empty_operand("MXFP4", raw.shape[0], n, raw.device)
+    _call(raw.device, nat.lib().cp_mx4_from_gguf, "mx4.from_gguf", raw.data_ptr(), raw.shape[0], n, codes.data_ptr(),
+          scales.data_ptr())
+    return Mx4Tensor(codes, scales, "MXFP4", raw.shape[0], n)
+
+
+def matmul(a, w, dtype=torch.bfloat16):
+    """a w^T for two operands of one format: a [T, n], w [out, n] -> [T, out] in `dtype`."""
+    dt = _DTYPE.get(dtype)
+    if dt is None:
+        raise ValueError("mx4.matmul: dtype must be bf16, f16 or f32")
+    if a.fmt != w.fmt or a.n != w.n:
+        raise ValueError(f"mx4.matmul: {a!r} and {w!r} must have one format and one n")
+    if a.device != w.device:
+        raise ValueError("mx4.matmul: operands must be on one device")
+    _need_cuda(a.codes, "mx4.matmul")
+    y = torch.empty((a.rows, w.rows), dtype=dtype, device=a.device)
+    _call(a.device, nat.lib().cp_mx4_matmul, "mx4.matmul", nat.MX4_ID[w.fmt], a.codes.data_ptr(), a.scales.data_ptr(),
+          a.rows, w.codes.data_ptr(), w.scales.data_ptr(), w.rows, w.n, a.tensor_scale * w.tensor_scale, dt, y.data_ptr())
+    return y
+
+
+def _product(x, w, transpose, what):
+    """x [..., K] times w^T (transpose: times w)."""
+    dt = _DTYPE.get(x.dtype)
+    K, out = (w.rows, w.n) if transpose else (w.n, w.rows)
+    if dt is None:
+        raise ValueError(f"{what} expects bf16, f16 or f32, not {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"{what}: the last dimension must be {K}, not {tuple(x.shape)}")
+    if x.device != w.device:
+        raise ValueError(f"{what}: the operands must be on one device")
+    _need_cuda(x, what)
+    x2 = x if x.dim() == 2 else x.reshape(x.numel() // K if K else math.prod(x.shape[:-1]), K)
+    T = x2.shape[0]
+    if x2.stride(1) != 1 and K > 1 or T > 1 and x2.stride(0) < K:
+        x2 = x2.contiguous()
+    ld = x2.stride(0) if T > 1 else (K + 7) // 8 * 8
+    L = nat.lib()
+    y = torch.empty((*x.shape[:-1], out), dtype=x.dtype, device=x.device)
+    p = x2.data_ptr()
+    need = L.cp_mx4_linear_workspace_bytes(dt, p, T, ld, w.rows, w.n, transpose)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _call(x.device, L.cp_mx4_linear, what, nat.MX4_ID[w.fmt], dt, p, T, ld, w.codes.data_ptr(), w.scales.data_ptr(),
+          w.rows, w.n, w.tensor_scale, transpose, y.data_ptr(), ws.data_ptr() if need else None, need)
+    return y
+
+
+class _Product(torch.autograd.Function):
+    """The product and its transpose are each other's gradient (the weights are frozen)."""
+
+    @staticmethod
+    def forward(ctx, x, w, transpose):
+        ctx.w, ctx.transpose = w, transpose
+        return _product(x, w, transpose, "mx4.linear_grad" if transpose else "mx4.linear")
+
+    @staticmethod
+    def backward(ctx, dy):
+        return _Product.apply(dy, ctx.w, 1 - ctx.transpose), None, None
+
+
+def linear(x, w):
+    """x w^T: x [..., n] (bf16, f16 or f32, taken at its own precision), w [out, n] -> [..., out] in
+    x's type.  x gets a gradient; the weights are frozen."""
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Product.apply(x, w, 0)
+    return _product(x, w, 0, "mx4.linear")
+
+
+def linear_grad(dy, w):
+    """The gradient of linear(x, w) with respect to x: dy w, dy [..., out] -> [..., n]."""
+    if dy.requires_grad and torch.is_grad_enabled():
+        return _Product.apply(dy, w, 1)
+    return _product(dy, w, 1, "mx4.linear_grad")
+
+
+def status(device=None):
+    """Raise CudaPathError if a bounded wait in an earlier product on `device` ran out (its result
+    is incomplete); synchronises the current stream."""
+    nat.torch_cuda()
+    dev = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index or 0)
+    _call(dev, nat.lib().cp_mx4_status, "mx4.status")
+
+
+class Linear(torch.nn.Module):
+    """torch.nn.Linear with frozen 4-bit weights (hessians.collect_hessians hooks it like one, so
+    the Hessians of later layers can be collected from an encoded model's own activations)."""
+
+    def __init__(self, weight, bias=None):
+        super().__init__()
+        self.out_features, self.in_features = weight.shape
+        self.fmt, self.tensor_scale = weight.fmt, weight.tensor_scale
+        self.register_buffer("codes", weight.codes)
+        self.register_buffer("scales", weight.scales)
+        self.bias = None if bias is None else torch.nn.Parameter(bias.detach().clone())
+
+    @classmethod
+    def from_linear(cls, linear, fmt="MXFP4", qw=None, tensor_scale=None):
+        """Encodes a torch.nn.Linear on a CUDA device (NVFP4's tensor scale from its weights unless given)."""
+        w = linear.weight.detach()
+        if tensor_scale is None:
+            tensor_scale = tensor_scale_for(w) if fmt == "NVFP4" else 1.0
+        return cls(quantize(w, fmt, qw, tensor_scale), linear.bias)
+
+    @property
+    def weight4(self):
+        return Mx4Tensor(self.codes, self.scales, self.fmt, self.out_features, self.in_features, self.tensor_scale)
+
+    def forward(self, x):
+        y = linear(x, self.weight4)
+        return y if self.bias is None else y + self.bias.to(y.dtype)
+
+    def extra_repr(self):
+        return f"in_features={self.in_features}, out_features={self.out_features}, fmt={self.fmt}, bias={self.bias is not None}"

@@ -1,0 +1,114 @@
+"""Microscaled 4-bit operands without a GPU: the oracle against the GGUF container's own decoder,
+operand checks, and the refusals of the C entry points (perm_b200/mx4.py)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import mx4_oracle as mo
+from perm_b200 import _native as nat
+from perm_b200 import mx4
+
+
+def test_oracle_container_decodes_as_gguf_does():
+    import gguf
+    rng = np.random.default_rng(0)
+    x = (rng.standard_normal((5, 256)) * np.exp(rng.standard_normal((5, 1)))).astype(np.float32)
+    codes, byte = mo.quantize(x, "MXFP4")
+    got = gguf.dequantize(mo.container(codes, byte), gguf.GGMLQuantizationType.MXFP4)
+    assert np.array_equal(got.astype(np.float64), mo.values(codes, byte, "MXFP4"))
+
+
+def test_oracle_pack_round_trips():
+    rng = np.random.default_rng(1)
+    for fmt in mo.BLOCK:
+        for rows, n in ((1, 5), (130, 300), (257, 512)):
+            codes, byte = mo.quantize(rng.standard_normal((rows, n)), fmt)
+            c, s = mo.pack(codes, byte, fmt, n)
+            c2, b2 = mo.unpack(c, s, fmt, rows, n)
+            assert np.array_equal(c2[:, :codes.shape[1]], codes) and np.array_equal(b2[:, :byte.shape[1]], byte)
+            assert c.size == nat.lib().cp_mx4_codes_bytes(rows, n)
+            assert s.size == nat.lib().cp_mx4_scales_bytes(nat.MX4_ID[fmt], rows, n)
+
+
+def test_operand_checks():
+    def make(rows=3, n=300, fmt="MXFP4", g=1.0, codes=None, scales=None):
+        c = torch.zeros((3, 256), dtype=torch.uint8) if codes is None else codes
+        s = torch.zeros((1, 4, 32, 4, 4), dtype=torch.uint8) if scales is None else scales
+        return mx4.Mx4Tensor(c, s, fmt, rows, n, g)
+    q = make()
+    assert q.shape == (3, 300) and "MXFP4" in repr(q)
+    for kw in (dict(fmt="MXFP8"), dict(rows=4), dict(n=0), dict(n=600), dict(fmt="NVFP4"), dict(g=0.0), dict(g=-1.0),
+               dict(g=float("nan")), dict(g=float("inf")), dict(codes=torch.zeros((3, 256))),
+               dict(codes=torch.zeros((3, 512), dtype=torch.uint8)[:, ::2]),
+               dict(scales=torch.zeros((2, 4, 32, 4, 4), dtype=torch.uint8))):
+        with pytest.raises(ValueError):
+            make(**kw)
+
+
+def test_host_tensors_are_refused():
+    q = mx4.Mx4Tensor(torch.zeros((3, 128), dtype=torch.uint8), torch.zeros((1, 2, 32, 4, 4), dtype=torch.uint8), "MXFP4", 3, 64)
+    x = torch.zeros(2, 64)
+    for call in (lambda: mx4.quantize(x, "MXFP4"), lambda: mx4.dequantize(q), lambda: mx4.matmul(q, q),
+                 lambda: mx4.linear(x, q), lambda: mx4.linear_grad(torch.zeros(2, 3), q),
+                 lambda: mx4.from_gguf(torch.zeros((1, 34), dtype=torch.uint8), 64)):
+        with pytest.raises(nat.CudaPathError):
+            call()
+
+
+def test_argument_checks_need_no_gpu():
+    q = mx4.Mx4Tensor(torch.zeros((3, 128), dtype=torch.uint8), torch.zeros((1, 2, 32, 4, 4), dtype=torch.uint8), "MXFP4", 3, 64)
+    r = mx4.Mx4Tensor(torch.zeros((3, 128), dtype=torch.uint8), torch.zeros((1, 2, 32, 4, 4), dtype=torch.uint8), "MXFP4", 3, 65)
+    with pytest.raises(ValueError):
+        mx4.matmul(q, r)
+    with pytest.raises(ValueError):
+        mx4.matmul(q, q, torch.float64)
+    with pytest.raises(ValueError):
+        mx4.dequantize(q, torch.int8)
+    with pytest.raises(ValueError):
+        mx4.linear(torch.zeros(2, 65), q)
+    with pytest.raises(ValueError):
+        mx4.linear(torch.zeros(2, 64, dtype=torch.float64), q)
+    with pytest.raises(ValueError):
+        mx4.linear_grad(torch.zeros(2, 64), q)
+    with pytest.raises(ValueError):
+        mx4.quantize(torch.zeros(2, 64), "FP4")
+
+
+def test_c_entry_points_refuse():
+    L = nat.lib()
+    buf = ctypes.create_string_buffer(4096 + 64)
+    p = (ctypes.addressof(buf) + 63) // 64 * 64        # never dereferenced: every call below is refused first
+    MX, NV, BF = nat.MX4_ID["MXFP4"], nat.MX4_ID["NVFP4"], nat.CP_MX4_BF16
+    quant = lambda f=MX, d=BF, x=p, rows=2, n=64, ld=64, g=1.0, c=p, s=p: L.cp_mx4_quantize(f, d, x, rows, n, ld, None, g, c, s, None)  # noqa: E731
+    assert quant(f=41) == nat.CP_ERR_TYPE and quant(d=7) == nat.CP_ERR_TYPE
+    assert quant(rows=-1) == nat.CP_ERR_SHAPE and quant(n=0) == nat.CP_ERR_SHAPE and quant(ld=63) == nat.CP_ERR_SHAPE
+    assert quant(rows=1 << 40) == nat.CP_ERR_SHAPE
+    assert quant(g=2.0) == nat.CP_ERR_ARG                       # MXFP4 has no tensor scale
+    for g in (3.0, 0.0, -1.0, float("nan"), float("inf"), 2.0 ** 110):
+        assert quant(f=NV, g=g) == nat.CP_ERR_ARG
+    assert quant(x=None) == nat.CP_ERR_ARG and quant(c=p + 8) == nat.CP_ERR_ARG and quant(x=p + 1) == nat.CP_ERR_ARG
+    assert quant(rows=0) == nat.CP_OK
+    deq = lambda f=MX, d=BF, c=p, n=64, o=p: L.cp_mx4_dequantize(f, c, p, 2, n, 1.0, d, o, None)  # noqa: E731
+    assert deq(f=8) == nat.CP_ERR_TYPE and deq(d=-1) == nat.CP_ERR_TYPE and deq(n=-4) == nat.CP_ERR_SHAPE
+    assert deq(c=None) == nat.CP_ERR_ARG and deq(o=p + 1) == nat.CP_ERR_ARG
+    assert L.cp_mx4_from_gguf(p, 2, 48, p, p, None) == nat.CP_ERR_SHAPE
+    assert L.cp_mx4_from_gguf(None, 2, 64, p, p, None) == nat.CP_ERR_ARG
+    mm = lambda f=MX, a=p, n=64, d=BF, y=p, t=2: L.cp_mx4_matmul(f, a, p, t, p, p, 3, n, 1.0, d, y, None)  # noqa: E731
+    assert mm(f=2) == nat.CP_ERR_TYPE and mm(d=3) == nat.CP_ERR_TYPE and mm(n=0) == nat.CP_ERR_SHAPE
+    assert mm(a=p + 4) == nat.CP_ERR_ARG and mm(y=None) == nat.CP_ERR_ARG and mm(t=0) == nat.CP_OK
+    lin = lambda f=MX, d=BF, x=p, T=2, ld=64, tr=0, y=p, ws=None, wsb=0: L.cp_mx4_linear(  # noqa: E731
+        f, d, x, T, ld, p, p, 64, 64, 1.0, tr, y, ws, wsb, None)
+    assert lin(f=0) == nat.CP_ERR_TYPE and lin(d=9) == nat.CP_ERR_TYPE and lin(T=-1) == nat.CP_ERR_SHAPE
+    assert lin(ld=60) == nat.CP_ERR_SHAPE and lin(x=None) == nat.CP_ERR_ARG and lin(y=p + 1) == nat.CP_ERR_ARG
+    assert lin(T=0) == nat.CP_OK
+    big = L.cp_mx4_linear_workspace_bytes(nat.CP_MX4_F32, p, 4096, 64, 64, 64, 0)
+    if big:
+        assert lin(d=nat.CP_MX4_F32, T=4096) == nat.CP_ERR_WORKSPACE
+    # the container's entry points
+    assert L.cp_kquant_encode(MX, p, 2, 48, None, p, None) == nat.CP_ERR_SHAPE
+    assert L.cp_kquant_decode(MX, p + 1, 2, 64, p, None) == nat.CP_ERR_ARG
+    assert L.cp_kquant_encode(NV, p, 2, 64, None, p, None) == nat.CP_ERR_TYPE
+    assert L.cp_grid_params(MX, p, 2, 256, p, p, None) == nat.CP_ERR_TYPE
+    assert L.cp_block_bytes(MX) == 17

@@ -662,6 +662,15 @@ static int check_mx4_dtype(int dtype) {
   return CP_OK;
 }
 
+// Launcher codes of the tensor-core products.
+static int mx4_rc(int rc, const char* what) {
+  const char* why = rc == 4 ? "the kernel's shared memory was refused" : rc == 5 ? "a tensor map was refused" : nullptr;
+  if (!why) return check_launch(what);
+  cudaGetLastError();
+  std::snprintf(g_err, sizeof(g_err), "%s: %s", what, why);
+  return CP_ERR_CUDA;
+}
+
 static size_t mx4_elem(int dtype) { return dtype == CP_MX4_F32 ? 4 : 2; }
 
 int64_t cp_mx4_codes_bytes(int64_t rows, int64_t n) { return rows > 0 && n > 0 ? rows * cpk::mx4_pitch(n) : 0; }
@@ -715,6 +724,7 @@ int cp_mx4_matmul(int fmt, const uint8_t* a_codes, const uint8_t* a_scales, int6
   if (int rc = check_mx4(fmt, a_rows, n)) return rc;
   if (int rc = check_mx4(fmt, w_rows, n)) return rc;
   if (int rc = check_mx4_dtype(dtype)) return rc;
+  if (a_rows > ((int64_t)1 << 38) / (w_rows + 1)) return set_err(CP_ERR_SHAPE, "cp_mx4_matmul: result too large");
   if (a_rows == 0 || w_rows == 0) return CP_OK;
   if (!a_codes || !a_scales || !w_codes || !w_scales || !y) return set_err(CP_ERR_ARG, "null pointer");
   if (((uintptr_t)a_codes | (uintptr_t)a_scales | (uintptr_t)w_codes | (uintptr_t)w_scales) & 15)
@@ -722,7 +732,7 @@ int cp_mx4_matmul(int fmt, const uint8_t* a_codes, const uint8_t* a_scales, int6
   if ((uintptr_t)y % mx4_elem(dtype)) return set_err(CP_ERR_ARG, "y is misaligned");
   ProfScope ps(kProfOther, (cudaStream_t)stream);
   const cpk::Mx4View a{a_codes, a_scales, a_rows, n, fmt}, w{w_codes, w_scales, w_rows, n, fmt};
-  return check_rc(cpk::launch_mx4_matmul(a, w, alpha, dtype, y, (cudaStream_t)stream), "cp_mx4_matmul");
+  return mx4_rc(cpk::launch_mx4_matmul(a, w, alpha, dtype, y, (cudaStream_t)stream), "cp_mx4_matmul");
 }
 
 static int mx4_x_aligned(int dtype, const void* x, int64_t ld) {
@@ -741,6 +751,7 @@ int cp_mx4_linear(int fmt, int dtype, const void* x, int64_t T, int64_t ld, cons
   if (int rc = check_mx4(fmt, rows, n)) return rc;
   if (int rc = check_mx4(fmt, T, transpose ? rows + 1 : n)) return rc;
   if (int rc = check_mx4_dtype(dtype)) return rc;
+  if (T > ((int64_t)1 << 38) / ((transpose ? n : rows) + 1)) return set_err(CP_ERR_SHAPE, "cp_mx4_linear: result too large");
   if (T > 1 && ld < (transpose ? rows : n)) return set_err(CP_ERR_SHAPE, "cp_mx4_linear: ld smaller than a row of x");
   if (T == 0 || (rows == 0 && !transpose)) return CP_OK;
   if (rows == 0) {   // a sum over no rows
@@ -758,13 +769,13 @@ int cp_mx4_linear(int fmt, int dtype, const void* x, int64_t T, int64_t ld, cons
     return set_err(CP_ERR_WORKSPACE, "workspace smaller than cp_mx4_linear_workspace_bytes()");
   ProfScope ps(kProfOther, (cudaStream_t)stream);
   const cpk::Mx4View w{codes, scales, rows, n, fmt};
-  return check_rc(cpk::launch_mx4_linear(dtype, x, T, ld, w, alpha, transpose, y, workspace, (cudaStream_t)stream),
-                  "cp_mx4_linear");
+  return mx4_rc(cpk::launch_mx4_linear(dtype, x, T, ld, w, alpha, transpose, y, workspace, (cudaStream_t)stream),
+                "cp_mx4_linear");
 }
 
 int cp_mx4_status(void* stream) {
   int st = 0;
-  if (cpk::mx4_read_status((cudaStream_t)stream, &st) != 0) return check_launch("cp_mx4_status");
+  if (cpk::mx4_matmul_status((cudaStream_t)stream, &st) != 0) return check_launch("cp_mx4_status");
   if (st == 0) return CP_OK;
   return set_err(CP_ERR_TIMEOUT, "a bounded wait in a 4-bit product ran out; its result is incomplete");
 }

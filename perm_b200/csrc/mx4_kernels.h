@@ -43,6 +43,7 @@ size_t mx4_linear_workspace_bytes(int dtype, int64_t T, int64_t rows, int64_t n,
 int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, const Mx4View& w, float alpha, int transpose,
                       void* y, void* ws, cudaStream_t stream);
 
-int mx4_read_status(cudaStream_t stream, int* status);
+// Status words of the products' bounded waits (read and cleared; synchronises the stream).
+int mx4_matmul_status(cudaStream_t stream, int* status);
 
 }  // namespace cpk

@@ -74,18 +74,9 @@ int launch_product(const Packed& a, const void* x, int dtype_x, int64_t T, int64
 
 size_t mx4_linear_workspace_bytes(int, int64_t, int64_t, int64_t, int64_t, int, int) { return 0; }
 
-int launch_mx4_matmul(const Mx4View& a, const Mx4View& w, float alpha, int dtype, void* y, cudaStream_t stream) {
-  return launch_product({a.codes, a.scales, a.rows, a.n}, nullptr, 0, a.rows, 0, w, 0, alpha, dtype, y, stream);
-}
-
 int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, const Mx4View& w, float alpha, int transpose,
                       void* y, void*, cudaStream_t stream) {
   return launch_product({}, x, dtype, T, ld, w, transpose, alpha, dtype, y, stream);
-}
-
-int mx4_read_status(cudaStream_t, int* status) {
-  *status = 0;
-  return 0;
 }
 
 }  // namespace cpk

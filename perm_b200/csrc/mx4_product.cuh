@@ -1,0 +1,96 @@
+// What the tensor-core products with 4-bit operands share: results, split sums, launches.
+#pragma once
+#include <algorithm>
+#include <atomic>
+#include "ef_kernels.h"
+#include "kquant_kernels.h"
+#include "mx4_format.cuh"
+#include "umma.cuh"
+
+namespace cpk {
+
+__device__ __forceinline__ void put_out(void* y, int dtype, int64_t i, float v) {
+  if (dtype == kMxBF16) static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
+  else if (dtype == kMxF16) static_cast<__half*>(y)[i] = __float2half_rn(v);
+  else static_cast<float*>(y)[i] = v;
+}
+
+// A role that gives up stops the others of its CTA and records the failure.
+__device__ __forceinline__ void fail_cta(volatile int* abort, int* status) {
+  *abort = 1;
+  atomicOr(status, 1);
+}
+
+// Sums the cluster's partial tiles ([token][128 rows] float32 at the same place of every CTA's
+// shared memory) in rank order; this CTA takes its share of the tokens.
+__device__ __forceinline__ void join_partials(const void* part, int rank, int split, int cols, int64_t row0, int64_t t0,
+                                              int64_t rows, float alpha, int dtype, void* y) {
+  const int c0 = cols * rank / split, c1 = cols * (rank + 1) / split;
+  const uint32_t at = smem_u32(part);
+  for (int i = threadIdx.x + c0 * 128; i < c1 * 128; i += blockDim.x) {
+    const int64_t row = row0 + (i & 127);
+    if (row >= rows) continue;
+    float v = 0.0f;
+    for (int p = 0; p < split; p++) v += ld_cluster_f32(peer_addr(at + 4 * i, p));
+    put_out(y, dtype, (t0 + (i >> 7)) * rows + row, alpha * v);
+  }
+}
+
+// Opts a kernel into its shared memory, once per device.
+template <auto K> inline bool opt_in_smem(size_t bytes) {
+  static std::atomic<unsigned long long> opted{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (opted.load() & (1ull << dev)) return true;
+  if (cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
+  opted.fetch_or(1ull << dev);
+  return true;
+}
+
+// Tensor map of byte rows (128-byte swizzle for 128-byte boxes, none for narrower ones).
+inline bool codes_map(CUtensorMap* m, const uint8_t* p, int64_t pitch, int64_t rows, int box_bytes, int box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)pitch, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)pitch};
+  const cuuint32_t box[2] = {(cuuint32_t)box_bytes, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(p), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Launches kernel K in clusters; 0, 4 (its shared memory was refused) or 6 (the launch was).
+template <auto K, typename... A>
+inline int launch_cluster(int grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {
+  if (!opt_in_smem<K>(smem)) return 4;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, 1, 1);
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, K, args...) != cudaSuccess) return 6;
+  note_launch();
+  return 0;
+}
+
+// Reads and clears a translation unit's status word.
+template <typename S> inline int read_status_word(S& word, cudaStream_t stream, int* status) {
+  int zero = 0;
+  if (cudaMemcpyFromSymbolAsync(status, word, sizeof(int), 0, cudaMemcpyDeviceToHost, stream) != cudaSuccess ||
+      cudaStreamSynchronize(stream) != cudaSuccess)
+    return 1;
+  if (*status && (cudaMemcpyToSymbolAsync(word, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream) != cudaSuccess ||
+                  cudaStreamSynchronize(stream) != cudaSuccess))
+    return 1;
+  return 0;
+}
+
+}  // namespace cpk

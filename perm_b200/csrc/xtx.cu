@@ -54,9 +54,9 @@
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <atomic>
-#include <mutex>
 #include "xtx_kernels.h"
 #include "kquant_kernels.h"
+#include "umma.cuh"
 
 namespace cpk {
 namespace {
@@ -99,84 +99,12 @@ struct XtxParams {
                      // any pair tile, so the waits on its stage run out; -1 = none
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ unsigned long long gtime() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_id() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
-  return r;
-}
-// Address in the shared::cluster window of the same variable in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t peer_addr(uint32_t a, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void mbar_init(uint32_t a, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(a), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t a, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(a), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t a) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(a) : "memory");
-}
-// Arrive on a barrier of the other CTA of the pair (a = shared::cluster address).
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t a) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint32_t a, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(a), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Bounded wait for the phase with the given parity.  False when it ran out (limit_ns of
-// global time) or a role of this CTA pair gave up (abort word nonzero).
-__device__ __forceinline__ bool mbar_wait(uint32_t a, uint32_t parity, volatile int* abort,
-                                          unsigned long long limit_ns) {
-  if (mbar_try(a, parity)) return true;
-  const unsigned long long t0 = gtime();
-  for (uint32_t n = 1; n < (1u << 30); n++) {
-    if (mbar_try(a, parity)) return true;
-    if ((n & 255) == 0 && (*abort || gtime() - t0 > limit_ns)) return false;
-  }
-  return false;
-}
 // Load into this CTA's shared memory, completing on a barrier of either CTA of the pair.
 __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t mbar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(mbar)
       : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// Shared-memory matrix descriptor, 128-byte swizzle, MN-major: rows of 64 bf16 (128 B) at a
-// 128 B pitch, 8-row groups SBO bytes apart, 64-column atoms LBO bytes apart.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) |
-         ((uint64_t)((sbo >> 4) & 0x3FFF) << 32) | (1ull << 46) | (2ull << 61);
 }
 // One M = 256 MMA over the CTA pair: the descriptors' shared-memory offsets address the same
 // layout in both CTAs (A rows 0-127 and B columns 0-127 in the even CTA, the rest in the odd).
@@ -192,19 +120,6 @@ __device__ __forceinline__ void umma_pair_bf16(uint32_t d_tmem, uint64_t adesc, 
 __device__ __forceinline__ void umma_commit_pair(uint32_t mbar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar) : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
-  uint32_t r[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int e = 0; e < 16; e++) v[e] = __uint_as_float(r[e]);
-}
-
 // Pair index p -> (TI, TJ), TJ <= TI: row block TI holds pairs TJ = 0 .. TI.
 __device__ __forceinline__ void pair_coords(int p, int& ti2, int& tj2) {
   int r = 0;
@@ -566,19 +481,6 @@ __global__ void __launch_bounds__(256) xtx_split_kernel(const float4* __restrict
     hi[k] = make_uint2(*reinterpret_cast<const uint32_t*>(&h01), *reinterpret_cast<const uint32_t*>(&h23));
     lo[k] = make_uint2(*reinterpret_cast<const uint32_t*>(&l01), *reinterpret_cast<const uint32_t*>(&l23));
   }
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
-  return fn;
 }
 
 int make_map(CUtensorMap* m, const void* x, int64_t T, int64_t d) {

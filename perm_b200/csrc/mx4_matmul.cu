@@ -163,48 +163,50 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int it = 0, n = 0;
-      bool ok = true;
-      for (int tile = first; ok && tile < prm.tiles; tile += stride, n++) {
-        if (n > 0 && !mbar_wait(acce, (n - 1) & 1, abort, kWaitNs)) {
+    const bool elected = elect_one();
+    int it = 0, n = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < prm.tiles; tile += stride, n++) {
+      if (n > 0 && !mbar_wait_warp(acce, (n - 1) & 1, abort, kWaitNs)) {
+        ok = false;
+        break;
+      }
+      for (int s = s_begin; s < s_end; s++, it++) {
+        const int st = it % C::kStages;
+        if (!mbar_wait_warp(full0 + 8 * st, (it / C::kStages) & 1, abort, kWaitNs)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        for (int s = s_begin; s < s_end; s++, it++) {
-          const int st = it % C::kStages;
-          if (!mbar_wait(full0 + 8 * st, (it / C::kStages) & 1, abort, kWaitNs)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t sw = ring + st * C::kStage, sx = sw + C::kWBytes, ss = sx + C::kXBytes;
-          const uint32_t ta = tmem + NT + (it & 1) * C::kScaleCols, tb = ta + C::kAtoms * 4;
+        const uint32_t sw = ring + st * C::kStage, sx = sw + C::kWBytes;
+        const uint64_t ad = sw128_desc(sw, 16, 1024), bd = sw128_desc(sx, 16, 1024), sd = scale_desc(sx + C::kXBytes);
+        const uint32_t ta = tmem + NT + (it & 1) * C::kScaleCols, tb = ta + C::kAtoms * 4;
+        const uint32_t more = s > s_begin;
+        if (elected) {   // descriptors count in 16 bytes
 #pragma unroll
           for (int a = 0; a < C::kAtoms; a++) {
-            scale_cp(ta + 4 * a, scale_desc(ss + a * 512));
+            scale_cp(ta + 4 * a, sd + a * 32);
 #pragma unroll
-            for (int k = 0; k < C::kXT; k++)
-              scale_cp(tb + (a * C::kXT + k) * 4, scale_desc(ss + (1 + k) * C::kSBytes + a * 512));
+            for (int k = 0; k < C::kXT; k++) scale_cp(tb + (a * C::kXT + k) * 4, sd + (1 + k) * (C::kSBytes / 16) + a * 32);
           }
 #pragma unroll
           for (int kk = 0; kk < 4; kk++) {
-            const uint64_t ad = sw128_desc(sw + kk * 32, 16, 1024), bd = sw128_desc(sx + kk * 32, 16, 1024);
             const int atom = FMT == kMXFP4 ? kk / 2 : kk;
             const uint32_t id = FMT == kMXFP4 ? (kk & 1) * 2u : 0u;   // which half of the scale word
-            umma_mx4<FMT>(tmem, ad, bd, C::kIdesc | (id << 4) | (id << 29), ta + 4 * atom, tb + 4 * C::kXT * atom,
-                          s > s_begin || kk > 0);
+            umma_mx4<FMT>(tmem, ad + 2 * kk, bd + 2 * kk, C::kIdesc | (id << 4) | (id << 29), ta + 4 * atom,
+                          tb + 4 * C::kXT * atom, kk > 0 ? 1u : more);
           }
           umma_commit(empty0 + 8 * st);
         }
-        if (ok) umma_commit(accf);
+        __syncwarp();
       }
-      if (!ok) fail_cta(abort, &g_status);
-      umma_commit(done);   // all MMAs complete before tensor memory is freed
-      int zero = 0;
-      mbar_wait(done, 0, &zero, kWaitNs);
+      if (ok && elected) umma_commit(accf);
+      __syncwarp();
     }
+    if (!ok) fail_cta(abort, &g_status);
+    if (elected) umma_commit(done);   // all MMAs complete before tensor memory is freed
+    int zero = 0;
+    mbar_wait(done, 0, &zero, kWaitNs);
   } else {
     const int q = warp & 3, hh = (warp - 2) >> 2;
     const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16) + hh * (NT / 2);
@@ -228,13 +230,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < NT / 2; c++) part[(hh * (NT / 2) + c) * 128 + r] = v[c];
       } else {
-        const int64_t row = (int64_t)(tile % prm.mtiles) * 128 + r;
-        const int64_t t0 = (int64_t)(tile / prm.mtiles) * NT + hh * (NT / 2);
-        if (row < prm.rows) {
-#pragma unroll
-          for (int c = 0; c < NT / 2; c++)
-            if (t0 + c < prm.T) put_out(prm.y, prm.dtype, (t0 + c) * prm.rows + row, prm.alpha * v[c]);
-        }
+        store_tile<NT / 2>(v, prm.alpha, prm.y, prm.dtype, (int64_t)(tile % prm.mtiles) * 128 + 32 * q, prm.rows,
+                           (int64_t)(tile / prm.mtiles) * NT + hh * (NT / 2), prm.T);
       }
     }
   }

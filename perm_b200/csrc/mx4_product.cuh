@@ -15,6 +15,48 @@ __device__ __forceinline__ void put_out(void* y, int dtype, int64_t i, float v) 
   else static_cast<float*>(y)[i] = v;
 }
 
+// Stores N accumulator columns of a warp: lane = output row (row0 + lane of rows), register = token
+// (t0 + c of T); y is [T, rows].  Two-byte types: neighbouring lanes swap halves of a packed pair of
+// columns, so that a lane holds two rows of one token and stores four bytes; a store instruction
+// then covers two tokens x 64 bytes.  (One row and one token at a time, with the type looked up for
+// each, took longer than the product.)
+template <int N>
+__device__ __forceinline__ void store_tile(const float (&v)[N], float alpha, void* y, int dtype, int64_t row0, int64_t rows,
+                                           int64_t t0, int64_t T) {
+  const int lane = threadIdx.x % 32;
+  const int64_t row = row0 + lane;
+  const int live = (int)min((int64_t)N, max((int64_t)0, T - t0));
+  if (dtype == kMxF32) {
+    float* p = static_cast<float*>(y) + t0 * rows + row;
+    if (row < rows) {
+#pragma unroll
+      for (int c = 0; c < N; c++, p += rows)
+        if (c < live) *p = alpha * v[c];
+    }
+    return;
+  }
+  const bool bf = dtype == kMxBF16;
+  const int odd = lane & 1;
+  const bool pairs = rows % 2 == 0 && (reinterpret_cast<uintptr_t>(y) & 3) == 0;
+  const uint32_t sel = odd ? 0x3276u : 0x5410u;
+  uint16_t* p = static_cast<uint16_t*>(y) + (t0 + odd) * rows + (row - odd);
+#pragma unroll
+  for (int c = 0; c < N; c += 2, p += 2 * rows) {
+    const float a = alpha * v[c], b = alpha * v[c + 1];
+    uint32_t w;
+    if (bf) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, w, 1);
+    const uint32_t two = __byte_perm(w, other, sel);   // rows row - odd, row - odd + 1 of token c + odd
+    if (pairs) {
+      if (row < rows && c + odd < live) *reinterpret_cast<uint32_t*>(p) = two;
+    } else if (c + odd < live) {
+      if (row - odd < rows) p[0] = (uint16_t)two;
+      if (row - odd + 1 < rows) p[1] = (uint16_t)(two >> 16);
+    }
+  }
+}
+
 // A role that gives up stops the others of its CTA and records the failure.
 __device__ __forceinline__ void fail_cta(volatile int* abort, int* status) {
   *abort = 1;

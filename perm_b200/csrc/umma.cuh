@@ -100,6 +100,21 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(mbar)
       : "memory");
 }
+// One lane of a converged warp.  Code around it that all lanes run keeps its loop counters and
+// descriptors in uniform registers, where the tensor-core instructions want them; under a
+// per-lane branch each instruction first moves its operands over (measured: about 75 clocks for a
+// tcgen05.cp and 150 for a block-scaled MMA, more than the instructions themselves take).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// mbar_wait by a converged warp, with one answer.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t a, uint32_t parity, volatile int* abort,
+                                               unsigned long long limit_ns) {
+  const bool got = mbar_wait(a, parity, abort, limit_ns);
+  return __all_sync(0xffffffffu, got);
+}
 // Contiguous copy (16-byte aligned, a multiple of 16 bytes).
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t mbar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),

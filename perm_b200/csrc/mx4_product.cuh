@@ -102,6 +102,19 @@ inline bool codes_map(CUtensorMap* m, const uint8_t* p, int64_t pitch, int64_t r
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Tensor map of scale tiles (512 bytes each, one after another), boxes of `box` tiles.
+inline bool scales_map(CUtensorMap* m, const uint8_t* p, int64_t tiles, int box) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {128, (cuuint64_t)tiles};
+  const cuuint64_t strides[1] = {512};
+  const cuuint32_t boxes[2] = {128, (cuuint32_t)box};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<uint8_t*>(p), dims, strides, boxes, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Launches kernel K in clusters; 0, 4 (its shared memory was refused) or 6 (the launch was).
 template <auto K, typename... A>
 inline int launch_cluster(int grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {

@@ -115,12 +115,24 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t a, uint32_t parity, vola
   const bool got = mbar_wait(a, parity, abort, limit_ns);
   return __all_sync(0xffffffffu, got);
 }
-// Contiguous copy (16-byte aligned, a multiple of 16 bytes).
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t mbar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(mbar)
-               : "memory");
+// Load into this CTA's shared memory, completing on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(mbar)
+      : "memory");
 }
+// Arrive on the barrier at shared::cluster address `mbar` once the MMAs issued so far complete.
+__device__ __forceinline__ void umma_commit_pair(uint32_t mbar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar) : "memory");
+}
+// A role that gives up stops both CTAs of the pair and records the failure.
+__device__ __forceinline__ void fail_pair(volatile int* abort, uint32_t peer_abort, int* status) {
+  *abort = 1;
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_abort), "r"(1) : "memory");
+  atomicOr(status, 1);
+}
+
 // Arrive on this CTA's barrier once the MMAs issued so far complete.
 __device__ __forceinline__ void umma_commit(uint32_t mbar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar) : "memory");
@@ -129,6 +141,50 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t a) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
   return v;
+}
+
+// N accumulator columns of this warp's lanes into registers, one wait for all of them.
+template <int N> __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float (&v)[N]) {
+  static_assert(N % 16 == 0, "loaded 16 columns at a time");
+#pragma unroll
+  for (int c = 0; c < N; c += 16) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v + c);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr + c));
+  }
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  // the registers are valid only from here on: keep their uses below the wait
+#pragma unroll
+  for (int c = 0; c < N; c++) asm volatile("" : "+f"(v[c]));
+}
+
+// The one-SM or the pair form of the same step.
+template <bool PAIR>
+__device__ __forceinline__ void tma_load_group(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t mbar) {
+  if (PAIR) tma_load_pair(dst, map, x, y, mbar);
+  else tma_load(dst, map, x, y, mbar);
+}
+template <bool PAIR> __device__ __forceinline__ void umma_commit_group(uint32_t mbar) {
+  if (PAIR) umma_commit_pair(mbar);
+  else umma_commit(mbar);
+}
+// By one converged warp (of each CTA of a pair); the address lands in shared memory at `dst`.
+template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
+  if (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+template <bool PAIR> __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
+  if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {

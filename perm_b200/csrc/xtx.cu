@@ -99,13 +99,6 @@ struct XtxParams {
                      // any pair tile, so the waits on its stage run out; -1 = none
 };
 
-// Load into this CTA's shared memory, completing on a barrier of either CTA of the pair.
-__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t mbar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(mbar)
-      : "memory");
-}
 // One M = 256 MMA over the CTA pair: the descriptors' shared-memory offsets address the same
 // layout in both CTAs (A rows 0-127 and B columns 0-127 in the even CTA, the rest in the odd).
 __device__ __forceinline__ void umma_pair_bf16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t accum) {
@@ -115,10 +108,6 @@ __device__ __forceinline__ void umma_pair_bf16(uint32_t d_tmem, uint64_t adesc, 
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(adesc), "l"(bdesc), "r"(kIdesc), "r"(accum)
       : "memory");
-}
-// Arrive on the barrier at shared::cluster address `mbar` once the MMAs issued so far complete.
-__device__ __forceinline__ void umma_commit_pair(uint32_t mbar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar) : "memory");
 }
 // Pair index p -> (TI, TJ), TJ <= TI: row block TI holds pairs TJ = 0 .. TI.
 __device__ __forceinline__ void pair_coords(int p, int& ti2, int& tj2) {
@@ -149,13 +138,6 @@ __device__ __forceinline__ void item_coords(int i, const XtxParams& prm, Seg& sg
     sg.ge = min(sg.ge, gb + prm.sub_per);
     sg.gb = gb;
   }
-}
-
-// A role that gives up stops both CTAs of the pair and records the failure.
-__device__ __forceinline__ void fail_pair(volatile int* abort, uint32_t peer_abort, int* status) {
-  *abort = 1;
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_abort), "r"(1) : "memory");
-  atomicOr(status, 1);
 }
 
 __global__ void __launch_bounds__(kThreads, 1)

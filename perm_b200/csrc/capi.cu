@@ -735,14 +735,14 @@ int cp_mx4_matmul(int fmt, const uint8_t* a_codes, const uint8_t* a_scales, int6
   return mx4_rc(cpk::launch_mx4_matmul(a, w, alpha, dtype, y, (cudaStream_t)stream), "cp_mx4_matmul");
 }
 
-static int mx4_x_aligned(int dtype, const void* x, int64_t ld) {
-  return ((uintptr_t)x & 15) == 0 && (ld * (int64_t)mx4_elem(dtype)) % 16 == 0;
+static int mx4_x_aligned(int dtype, const void* x, int64_t T, int64_t ld) {
+  return ((uintptr_t)x & 15) == 0 && (T == 1 || (ld * (int64_t)mx4_elem(dtype)) % 16 == 0);
 }
 
 size_t cp_mx4_linear_workspace_bytes(int dtype, const void* x, int64_t T, int64_t ld, int64_t rows, int64_t n,
                                      int transpose) {
   if (T <= 0 || rows <= 0 || n <= 0) return 0;
-  return cpk::mx4_linear_workspace_bytes(dtype, T, rows, n, ld, mx4_x_aligned(dtype, x, ld), transpose);
+  return cpk::mx4_linear_workspace_bytes(dtype, T, rows, n, mx4_x_aligned(dtype, x, T, ld), transpose);
 }
 
 int cp_mx4_linear(int fmt, int dtype, const void* x, int64_t T, int64_t ld, const uint8_t* codes,
@@ -751,7 +751,7 @@ int cp_mx4_linear(int fmt, int dtype, const void* x, int64_t T, int64_t ld, cons
   if (int rc = check_mx4(fmt, rows, n)) return rc;
   if (int rc = check_mx4(fmt, T, transpose ? rows + 1 : n)) return rc;
   if (int rc = check_mx4_dtype(dtype)) return rc;
-  if (T > ((int64_t)1 << 38) / ((transpose ? n : rows) + 1)) return set_err(CP_ERR_SHAPE, "cp_mx4_linear: result too large");
+  if (T >= (int64_t)1 << 29 || T > ((int64_t)1 << 38) / ((transpose ? n : rows) + 1)) return set_err(CP_ERR_SHAPE, "cp_mx4_linear: result too large");
   if (T > 1 && ld < (transpose ? rows : n)) return set_err(CP_ERR_SHAPE, "cp_mx4_linear: ld smaller than a row of x");
   if (T == 0 || (rows == 0 && !transpose)) return CP_OK;
   if (rows == 0) {   // a sum over no rows
@@ -769,14 +769,16 @@ int cp_mx4_linear(int fmt, int dtype, const void* x, int64_t T, int64_t ld, cons
     return set_err(CP_ERR_WORKSPACE, "workspace smaller than cp_mx4_linear_workspace_bytes()");
   ProfScope ps(kProfOther, (cudaStream_t)stream);
   const cpk::Mx4View w{codes, scales, rows, n, fmt};
-  return mx4_rc(cpk::launch_mx4_linear(dtype, x, T, ld, w, alpha, transpose, y, workspace, (cudaStream_t)stream),
+  return mx4_rc(cpk::launch_mx4_linear(dtype, x, T, ld, mx4_x_aligned(dtype, x, T, ld), w, alpha, transpose, y, workspace,
+                                       (cudaStream_t)stream),
                 "cp_mx4_linear");
 }
 
 int cp_mx4_status(void* stream) {
-  int st = 0;
-  if (cpk::mx4_matmul_status((cudaStream_t)stream, &st) != 0) return check_launch("cp_mx4_status");
-  if (st == 0) return CP_OK;
+  int st = 0, st2 = 0;
+  if (cpk::mx4_matmul_status((cudaStream_t)stream, &st) != 0 || cpk::mx4_linear_status((cudaStream_t)stream, &st2) != 0)
+    return check_launch("cp_mx4_status");
+  if (st == 0 && st2 == 0) return CP_OK;
   return set_err(CP_ERR_TIMEOUT, "a bounded wait in a 4-bit product ran out; its result is incomplete");
 }
 

@@ -38,12 +38,13 @@ int launch_mx4_matmul(const Mx4View& a, const Mx4View& w, float alpha, int dtype
 
 // transpose == 0: y[t][r] = alpha * sum_k x[t][k] w[r][k]   (x [T, w.n],    y [T, w.rows])
 // transpose == 1: y[t][k] = alpha * sum_r x[t][r] w[r][k]   (x [T, w.rows], y [T, w.n])
-size_t mx4_linear_workspace_bytes(int dtype, int64_t T, int64_t rows, int64_t n, int64_t ld, int aligned,
-                                  int transpose);
-int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, const Mx4View& w, float alpha, int transpose,
-                      void* y, void* ws, cudaStream_t stream);
+// aligned: x's rows start on 16-byte boundaries.
+size_t mx4_linear_workspace_bytes(int dtype, int64_t T, int64_t rows, int64_t n, int aligned, int transpose);
+int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, int aligned, const Mx4View& w, float alpha,
+                      int transpose, void* y, void* ws, cudaStream_t stream);
 
 // Status words of the products' bounded waits (read and cleared; synchronises the stream).
 int mx4_matmul_status(cudaStream_t stream, int* status);
+int mx4_linear_status(cudaStream_t stream, int* status);
 
 }  // namespace cpk

@@ -1,82 +1,580 @@
-// Products with 4-bit operands: a 64 x 64 output tile per CTA, operands decoded to float32 in shared
-// memory 32 deep, 4 x 4 outputs per thread.
-#include <cuda_runtime.h>
-#include "kquant_kernels.h"
-#include "mx4_format.cuh"
+// Products of activations in their own type with frozen 4-bit weights w [rows, n]:
+//   y = alpha * x w^T   (x [T, n], TR = false)
+//   y = alpha * x w     (x [T, rows], TR = true: the first form's gradient with respect to x)
+//
+// Tensor-core kernel (tcgen05 kind::f16, bf16 x bf16 -> f32).  An e2m1 value times its block scale
+// has at most six significant bits, so it is exact in bf16, and so is every product in the float32
+// accumulator.  The 4-bit weights go from global to shared memory as they are (TMA) and eight warps
+// decode them there, 64 columns of the reduction at a time, into the swizzled bf16 tile that the
+// MMA reads: the K-major one for x w^T, the MN-major one for x w, where the packed axis is the
+// output's.  Weights are the M side (128 rows of the output per CTA), tokens the N side.
+//
+// Decoding.  cvt turns two codes into two f16 values; f16 holds an e2m1 value in the sign and the
+// top six bits, and the same bits three places lower are the bf16 of the value times 2^-112.  One
+// bf16 product with 2^112 times the block scale makes it whole: five instructions for two
+// weights.  MXFP4 scales above 2^15, where that factor would overflow, take a second product.
+//
+// float16 and float32 activations are cut into bf16 parts (8 significant bits each: two for float16,
+// three for float32, no remainder) by a first kernel, and every decoded weight tile is multiplied
+// by all the parts, so the result is that of the activations as they are.  Rows of x that TMA
+// cannot address (not 16-byte aligned) go through the same kernel.
+//
+// Work split, joins and bounded waits are those of the 4-bit products: SM pairs on 256 x 256 tiles
+// for many tokens, clusters over the reduction where there are few tiles (mx4_matmul.cu).  Two
+// accumulators alternate, so storing one tile overlaps the MMAs of the next.  float32 results restart the
+// accumulation every few steps and sum the chunks in round-to-nearest registers, because the tensor core's own
+// accumulation truncates.
+#include "mx4_product.cuh"
 
 namespace cpk {
 namespace {
 
-struct Packed {
-  const uint8_t* codes;
-  const uint8_t* scales;
-  int64_t rows, n;
+__device__ int g_status;
+
+constexpr unsigned long long kWaitNs = 1000000000ull;
+constexpr int kThreads = 512;   // warps: 0 x loads, 1 MMA, 2 code loads, 3 allocation, 4-7 epilogue, 8-15 decoding
+constexpr int kChunkSteps = 3;  // 64-deep steps of one float32 accumulation chain (36 MMAs with three parts)
+
+template <int FMT, int NT, bool PAIR, bool TR> struct Cfg {
+  static constexpr int kXRows = PAIR ? NT / 2 : NT;
+  static constexpr int kA = 128 * 128;                     // decoded tile: 128 rows x 64, bf16
+  static constexpr int kB = kXRows * 128;                  // tokens x 64, bf16
+  static constexpr int kSub = TR ? 2 : 4;                  // 64-deep steps per code stage
+  static constexpr int kCodes = TR ? 128 * 64 : 128 * 128; // 128 w rows x 128 columns, or x 256
+  static constexpr int kAtoms = (FMT == kMXFP4 ? 1 : 2) * (TR ? 1 : 2);   // its scale tiles
+  static constexpr int kC = (kCodes + kAtoms * 512 + 1023) / 1024 * 1024;
+  static constexpr int kAS = 4, kCS = 3;
+  static constexpr int kFit = (224 * 1024 - kAS * kA - kCS * kC) / kB;
+  static constexpr int kBS = kFit < 8 ? kFit : 8;
+  static constexpr int kRing = kAS * kA + kBS * kB + kCS * kC;
+  static constexpr size_t kSmem = 1024 + (size_t)kRing + 512;
+  static constexpr uint32_t kTmem = 2 * NT < 64 ? 64 : 2 * NT;
+  static_assert(kB % 1024 == 0 && kBS >= 3, "stages keep the swizzle's alignment");
+  // f32 accumulator, A and B bf16, A MN-major in the transposed form, N >> 3, M >> 4
+  static constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((TR ? 1u : 0u) << 15) |
+                                     ((uint32_t)(NT >> 3) << 17) | ((PAIR ? 16u : 8u) << 24);
 };
-template <int FMT> __device__ __forceinline__ float packed_at(const Packed& p, int64_t r, int64_t k) {
-  if (r >= p.rows || k >= p.n) return 0.0f;
-  const int64_t chunks = (p.n + 255) / 256;
-  const uint32_t b = p.codes[r * chunks * 128 + (k >> 1)];
-  const float q = e2m1x2_value((b >> (4 * (k & 1))) & 15).x;
-  constexpr int B = mx_block<FMT>();
-  return q * mx_scale_value<FMT>(p.scales[mx_scale_offset(r, k / B, chunks * (64 / B))]);
-}
-__device__ __forceinline__ float dense_at(const void* x, int dtype, int64_t i) {
-  return dtype == kMxBF16  ? __bfloat162float(static_cast<const __nv_bfloat16*>(x)[i])
-         : dtype == kMxF16 ? __half2float(static_cast<const __half*>(x)[i])
-                           : static_cast<const float*>(x)[i];
-}
-__device__ __forceinline__ void put(void* y, int dtype, int64_t i, float v) {
-  if (dtype == kMxBF16) static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
-  else if (dtype == kMxF16) static_cast<__half*>(y)[i] = __float2half_rn(v);
-  else static_cast<float*>(y)[i] = v;
+
+struct LinParams {
+  void* y;
+  int64_t T, out;       // y is [T, out]
+  int64_t wrows;        // rows of w
+  float alpha;
+  int dtype;
+  int parts;
+  int steps;            // 64-deep steps of the reduction
+  int groups;           // scale tiles per 128 rows of w
+  int mtiles, tiles;
+};
+
+template <bool PAIR>
+__device__ __forceinline__ void umma_bf16(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accum) {
+  if (PAIR)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(ad), "l"(bd), "r"(idesc), "r"(accum)
+                 : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(ad), "l"(bd), "r"(idesc), "r"(accum)
+                 : "memory");
 }
 
-template <int FMT>
-__global__ void __launch_bounds__(256) product_kernel(Packed a, const void* x, int dtype_x, int64_t T, int64_t ld,
-                                                      Packed w, int transpose, float alpha, int dtype, void* y) {
-  __shared__ float sx[32][65], sw[32][65];
-  const int64_t out = transpose ? w.n : w.rows, K = transpose ? w.rows : w.n;
-  const int64_t o0 = (int64_t)blockIdx.x * 64, t0 = (int64_t)blockIdx.y * 64;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < K; k0 += 32) {
-    for (int i = threadIdx.x; i < 2048; i += 256) {
-      const int k = i % 32, j = i / 32;
-      const int64_t t = t0 + j, o = o0 + j, kk = k0 + k;
-      sx[k][j] = t >= T || kk >= K ? 0.0f : x ? dense_at(x, dtype_x, t * ld + kk) : packed_at<FMT>(a, t, kk);
-      sw[k][j] = transpose ? packed_at<FMT>(w, kk, o) : packed_at<FMT>(w, o, kk);
-    }
-    __syncthreads();
-    for (int k = 0; k < 32; k++)
-      for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) acc[i][j] += sx[k][ty + 16 * i] * sw[k][tx + 16 * j];
-    __syncthreads();
+// bf16 (twice) of 2^112 times a block scale; `more` is a further factor, 1 unless the first would
+// overflow.
+__device__ __forceinline__ uint32_t twice(uint32_t b) { return b | (b << 16); }
+__device__ __forceinline__ uint32_t factor_e8m0(uint32_t byte, uint32_t& more) {
+  more = 0;
+  if (byte > 142) {
+    more = byte == 255 ? twice(0x7FC0) : twice((byte - 142 + 127) << 7);   // byte 254: 2^112, the field's 239
+    byte = 142;
   }
-  for (int i = 0; i < 4; i++)
-    for (int j = 0; j < 4; j++) {
-      const int64_t t = t0 + ty + 16 * i, o = o0 + tx + 16 * j;
-      if (t < T && o < out) put(y, dtype, t * out + o, alpha * acc[i][j]);
-    }
+  return twice((byte + 112) << 7);
+}
+__device__ __forceinline__ uint32_t factor_e4m3(uint32_t byte) {
+  return twice(__float_as_uint(e4m3_value(byte) * 5.192296858534827628530496329220096e33f) >> 16);   // 2^112; 0x7F stays NaN
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Eight codes -> eight bf16 values times 2^-112, in pairs.
+__device__ __forceinline__ void decode8(uint32_t w, uint32_t (&v)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+      : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = ((v[i] >> 3) & 0x0FC00FC0u) | (v[i] & 0x80008000u);
 }
 
-int launch_product(const Packed& a, const void* x, int dtype_x, int64_t T, int64_t ld, const Mx4View& w, int transpose,
-                   float alpha, int dtype, void* y, cudaStream_t stream) {
-  const int64_t out = transpose ? w.n : w.rows;
-  const dim3 grid((unsigned)((out + 63) / 64), (unsigned)((T + 63) / 64));
-  const Packed pw{w.codes, w.scales, w.rows, w.n};
-  if (w.fmt == kMXFP4) product_kernel<kMXFP4><<<grid, 256, 0, stream>>>(a, x, dtype_x, T, ld, pw, transpose, alpha, dtype, y);
-  else product_kernel<kNVFP4><<<grid, 256, 0, stream>>>(a, x, dtype_x, T, ld, pw, transpose, alpha, dtype, y);
-  note_launch();
-  return 0;
+template <int FMT, int NT, bool PAIR, bool TR, bool CHUNK>
+__global__ void __launch_bounds__(kThreads, 1)
+    mx4_linear_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
+                      const __grid_constant__ CUtensorMap map_x, const LinParams prm, int split) {
+  using C = Cfg<FMT, NT, PAIR, TR>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::kRing);
+  constexpr int kBars = 2 * (C::kAS + C::kBS + C::kCS) + 5;
+  volatile int* misc = reinterpret_cast<volatile int*>(bars + kBars);   // [0] tmem, [1] abort
+  const uint32_t ring_a = smem_u32(base), ring_b = ring_a + C::kAS * C::kA, ring_c = ring_b + C::kBS * C::kB;
+  const uint32_t afull = smem_u32(bars), aempty = afull + 8 * C::kAS;
+  const uint32_t bfull = aempty + 8 * C::kAS, bempty = bfull + 8 * C::kBS;
+  const uint32_t cfull = bempty + 8 * C::kBS, cempty = cfull + 8 * C::kCS;
+  const uint32_t accf = cempty + 8 * C::kCS, acce = accf + 16, done = acce + 16;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = PAIR || split > 1 ? (int)cluster_rank() : 0;
+  const bool leader = !PAIR || rank == 0;
+  const int group = PAIR ? 2 : split;
+  const int first = (int)blockIdx.x / group, stride = (int)gridDim.x / group;
+  // this CTA's code stages, and its 64-deep steps
+  const int stages = (prm.steps + C::kSub - 1) / C::kSub;
+  const int c_begin = PAIR ? 0 : (int)((int64_t)stages * rank / split);
+  const int c_end = PAIR ? stages : (int)((int64_t)stages * (rank + 1) / split);
+  const int s_begin = c_begin * C::kSub, s_end = min(prm.steps, c_end * C::kSub);
+  auto tile_row = [&](int tile) { return (int64_t)(tile % prm.mtiles) * (PAIR ? 256 : 128) + (PAIR ? rank * 128 : 0); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kAS; s++) {
+      mbar_init(afull + 8 * s, PAIR ? 16 : 8);
+      mbar_init(aempty + 8 * s, 1);
+    }
+    for (int s = 0; s < C::kBS; s++) {
+      mbar_init(bfull + 8 * s, 1);
+      mbar_init(bempty + 8 * s, 1);
+    }
+    for (int s = 0; s < C::kCS; s++) {
+      mbar_init(cfull + 8 * s, 1);
+      mbar_init(cempty + 8 * s, 8);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(accf + 8 * b, 1);
+      mbar_init(acce + 8 * b, PAIR ? 8 : 4);
+    }
+    mbar_init(done, 1);
+    misc[1] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_s)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_x)) : "memory");
+  }
+  if (warp == 3) tmem_alloc<PAIR>(smem_u32((const void*)&misc[0]), C::kTmem);
+  tc_fence_before();
+  __syncthreads();
+  if (PAIR) cluster_sync();   // both CTAs' barriers are initialised and their tensor memory allocated
+  tc_fence_after();
+  const uint32_t tmem = (uint32_t)misc[0];
+  volatile int* abort = &misc[1];
+  const uint32_t peer_abort = PAIR ? peer_addr(smem_u32((const void*)&misc[1]), rank ^ 1) : 0;
+  auto fail = [&] {
+    if (PAIR) fail_pair(abort, peer_abort, &g_status);
+    else fail_cta(abort, &g_status);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {   // ---- x tiles, part by part
+      const uint32_t lead_bfull = PAIR ? peer_addr(bfull, 0) : bfull;
+      int it = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < prm.tiles; tile += stride) {
+        const int t0 = tile / prm.mtiles * NT + (PAIR ? rank * C::kXRows : 0);
+        for (int s = s_begin; ok && s < s_end; s++)
+          for (int p = 0; p < prm.parts; p++, it++) {
+            const int st = it % C::kBS, round = it / C::kBS;
+            if (round > 0 && !mbar_wait(bempty + 8 * st, (round - 1) & 1, abort, kWaitNs)) {
+              ok = false;
+              break;
+            }
+            if (leader) mbar_expect_tx(bfull + 8 * st, (PAIR ? 2 : 1) * C::kB);
+            tma_load_group<PAIR>(ring_b + st * C::kB, &map_x, s * 64, (int)(p * prm.T) + t0, lead_bfull + 8 * st);
+          }
+      }
+      if (!ok) fail();
+      for (int k = max(0, it - C::kBS); k < it; k++) {   // every load issued lands before the CTA goes on
+        int zero = 0;
+        mbar_wait((leader ? bfull : bempty) + 8 * (k % C::kBS), (k / C::kBS) & 1, &zero, kWaitNs);
+      }
+    }
+  } else if (warp == 2) {
+    if (lane == 0) {   // ---- codes and scales of this CTA's rows
+      int it = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < prm.tiles; tile += stride) {
+        const int m0 = (int)tile_row(tile);
+        for (int c = c_begin; c < c_end; c++, it++) {
+          const int st = it % C::kCS, round = it / C::kCS;
+          if (round > 0 && !mbar_wait(cempty + 8 * st, (round - 1) & 1, abort, kWaitNs)) {
+            ok = false;
+            break;
+          }
+          const uint32_t fb = cfull + 8 * st, sc = ring_c + st * C::kC;
+          mbar_expect_tx(fb, C::kCodes + C::kAtoms * 512);
+          if (TR) {
+            tma_load(sc, &map_w, m0 / 2, c * 128, fb);
+            tma_load(sc + C::kCodes, &map_s, 0, c * prm.groups + m0 / 128 * C::kAtoms, fb);
+          } else {
+            tma_load(sc, &map_w, c * 128, m0, fb);
+            tma_load(sc + C::kCodes, &map_s, 0, m0 / 128 * prm.groups + c * C::kAtoms, fb);
+          }
+        }
+      }
+      if (!ok) fail();
+      for (int k = max(0, it - C::kCS); k < it; k++) {
+        int zero = 0;
+        mbar_wait(cfull + 8 * (k % C::kCS), (k / C::kCS) & 1, &zero, kWaitNs);
+      }
+    }
+  } else if (warp == 1) {
+    if (leader) {   // ---- MMAs
+      const bool elected = elect_one();
+      const uint32_t peer_aempty = PAIR ? peer_addr(aempty, 1) : 0, peer_bempty = PAIR ? peer_addr(bempty, 1) : 0;
+      const uint32_t peer_accf = PAIR ? peer_addr(accf, 1) : 0;
+      int ia = 0, ib = 0, cg = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < prm.tiles; tile += stride) {
+        for (int g0 = s_begin; ok && g0 < s_end; cg++) {
+          const int b = cg & 1, g1 = CHUNK ? min(s_end, g0 + kChunkSteps) : s_end;
+          const uint32_t acc = tmem + b * NT;
+          if (cg >= 2 && !mbar_wait_warp(acce + 8 * b, ((cg >> 1) - 1) & 1, abort, kWaitNs)) {
+            ok = false;
+            break;
+          }
+          for (int s = g0; s < g1 && ok; s++, ia++) {
+            const int as = ia % C::kAS;
+            if (!(PAIR ? mbar_wait_cluster(afull + 8 * as, (ia / C::kAS) & 1, abort, kWaitNs)
+                       : mbar_wait_warp(afull + 8 * as, (ia / C::kAS) & 1, abort, kWaitNs))) {
+              ok = false;
+              break;
+            }
+            const uint32_t sa = ring_a + as * C::kA;
+            const uint64_t ad = TR ? sw128_desc(sa, 8192, 1024) : sw128_desc(sa, 16, 1024);
+            for (int p = 0; p < prm.parts; p++, ib++) {
+              const int bs = ib % C::kBS;
+              if (!mbar_wait_warp(bfull + 8 * bs, (ib / C::kBS) & 1, abort, kWaitNs)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const uint64_t bd = sw128_desc(ring_b + bs * C::kB, 16, 1024);
+              const uint32_t more = s > g0 || p > 0;
+              if (elected) {
+#pragma unroll
+                for (int kk = 0; kk < 4; kk++)   // 16 deep: 32 bytes of a K-major row, or 16 rows of 128
+                  umma_bf16<PAIR>(acc, ad + (TR ? 128 : 2) * kk, bd + 2 * kk, C::kIdesc, kk > 0 ? 1u : more);
+                umma_commit_group<PAIR>(bempty + 8 * bs);
+                if (PAIR) umma_commit_pair(peer_bempty + 8 * bs);
+              }
+              __syncwarp();
+            }
+            if (ok && elected) {
+              umma_commit_group<PAIR>(aempty + 8 * as);
+              if (PAIR) umma_commit_pair(peer_aempty + 8 * as);
+            }
+            __syncwarp();
+          }
+          if (ok && elected) {
+            umma_commit_group<PAIR>(accf + 8 * b);
+            if (PAIR) umma_commit_pair(peer_accf + 8 * b);
+          }
+          __syncwarp();
+          g0 = g1;
+        }
+      }
+      if (!ok) fail();
+      if (elected) umma_commit_group<PAIR>(done);   // all MMAs complete before tensor memory is freed
+      int zero = 0;
+      mbar_wait(done, 0, &zero, kWaitNs);
+    }
+  } else if (warp >= 8) {
+    // ---- decoding: a thread takes 32 codes (16 bytes) of a 64-deep step: half of a row's, or (TR) a
+    // quarter of a w row's 128 columns
+    const int d = threadIdx.x - 256;
+    const int r = TR ? d & 63 : d & 127, h = TR ? d >> 6 : d >> 7;
+    const uint32_t dst0 = TR ? (h >> 1) * 8192 + r * 128 : r * 128;
+    const int chunk0 = TR ? (h & 1) * 4 : h * 4, x7 = r & 7;
+    const uint32_t lead_afull = PAIR ? peer_addr(afull, 0) : afull;
+    int ia = 0, ic = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < prm.tiles; tile += stride)
+      for (int c = c_begin; c < c_end && ok; c++, ic++) {
+        const int cs = ic % C::kCS;
+        if (!mbar_wait_warp(cfull + 8 * cs, (ic / C::kCS) & 1, abort, kWaitNs)) {
+          ok = false;
+          break;
+        }
+        const uint8_t* codes = base + C::kAS * C::kA + C::kBS * C::kB + cs * C::kC;
+        const uint8_t* scales = codes + C::kCodes;
+        const int subs = min(C::kSub, prm.steps - c * C::kSub);
+        for (int sub = 0; sub < subs; sub++, ia++) {
+          const int R = TR ? sub * 64 + r : r;   // row of the code stage
+          const uint32_t at = TR ? R * 64 + ((h ^ ((R >> 1) & 3)) << 4) : R * 128 + (((sub * 2 + h) ^ x7) << 4);
+          const uint4 q = *reinterpret_cast<const uint4*>(codes + at);
+          const int srow = (R & 31) * 16 + (R >> 5) * 4;
+          uint32_t f0, f1, more = 0;
+          if (FMT == kMXFP4) {
+            const uint32_t byte = TR ? scales[srow + h] : scales[(sub >> 1) * 512 + srow + (sub & 1) * 2 + h];
+            f0 = f1 = factor_e8m0(byte, more);
+          } else {
+            const uint8_t* s2 = TR ? scales + (h >> 1) * 512 + srow + (h & 1) * 2 : scales + sub * 512 + srow + h * 2;
+            const uint32_t two = *reinterpret_cast<const uint16_t*>(s2);
+            f0 = factor_e4m3(two & 0xFF);
+            f1 = factor_e4m3(two >> 8);
+          }
+          // rows past the last (their scale bytes are not defined) are part of the reduction: zero
+          if (TR && (int64_t)c * 128 + R >= prm.wrows) f0 = f1 = more = 0;
+          const int as = ia % C::kAS;
+          if (ia >= C::kAS && !mbar_wait_warp(aempty + 8 * as, (ia / C::kAS - 1) & 1, abort, kWaitNs)) {
+            ok = false;
+            break;
+          }
+          const uint32_t dst = ring_a + as * C::kA + dst0;
+          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            uint32_t v[4];
+            decode8(w[i], v);
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = mul_bf16x2(v[k], i < 2 ? f0 : f1);
+            if (FMT == kMXFP4 && more) {
+#pragma unroll
+              for (int k = 0; k < 4; k++) v[k] = mul_bf16x2(v[k], more);
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (((chunk0 + i) ^ x7) << 4)), "r"(v[0]),
+                         "r"(v[1]), "r"(v[2]), "r"(v[3])
+                         : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read through the async proxy
+          __syncwarp();
+          if (lane == 0) {
+            if (leader) mbar_arrive(afull + 8 * as);
+            else mbar_arrive_remote_release(lead_afull + 8 * as);
+          }
+        }
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(cempty + 8 * cs);
+      }
+    if (!ok) fail();
+  } else if (warp >= 4) {
+    // ---- epilogue: warp 4 + q holds TMEM lanes 32 q .. + 31
+    const int q = warp & 3;
+    const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16);
+    const uint32_t lead_acce = PAIR ? peer_addr(acce, 0) : acce;
+    float* part = reinterpret_cast<float*>(base);
+    int cg = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < prm.tiles; tile += stride) {
+      const int64_t row0 = tile_row(tile) + 32 * q, t0 = (int64_t)(tile / prm.mtiles) * NT;
+      auto emit = [&](const float(&v)[32], int c) {   // columns c .. c + 31 of the tile
+        if (split > 1) {   // the loads and MMAs of this CTA's only tile are complete: the rings are free
+#pragma unroll
+          for (int e = 0; e < 32; e++) part[(c + e) * 128 + 32 * q + lane] = v[e];
+        } else {
+          store_tile<32>(v, prm.alpha, prm.y, prm.dtype, row0, prm.out, t0 + c, prm.T);
+        }
+      };
+      if constexpr (CHUNK) {
+        float m[NT / 32][32];
+#pragma unroll
+        for (int c = 0; c < NT / 32; c++)
+#pragma unroll
+          for (int e = 0; e < 32; e++) m[c][e] = 0.0f;
+        for (int g0 = s_begin; g0 < s_end; g0 += kChunkSteps, cg++) {
+          const int b = cg & 1;
+          if (!mbar_wait_warp(accf + 8 * b, (cg >> 1) & 1, abort, kWaitNs)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < NT / 32; c++) {
+            float v[32];
+            tmem_ld_cols(trow + b * NT + 32 * c, v);
+#pragma unroll
+            for (int e = 0; e < 32; e++) m[c][e] += v[e];
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (leader) mbar_arrive(acce + 8 * b);
+            else mbar_arrive_remote(lead_acce + 8 * b);
+          }
+        }
+        if (ok) {
+#pragma unroll
+          for (int c = 0; c < NT / 32; c++) emit(m[c], 32 * c);
+        }
+      } else {
+        const int b = cg & 1;
+        if (!mbar_wait_warp(accf + 8 * b, (cg >> 1) & 1, abort, kWaitNs)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < NT; c += 32) {
+          float v[32];
+          tmem_ld_cols(trow + b * NT + c, v);
+          if (c + 32 == NT) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (leader) mbar_arrive(acce + 8 * b);
+              else mbar_arrive_remote(lead_acce + 8 * b);
+            }
+          }
+          emit(v, c);
+        }
+        cg++;
+      }
+    }
+    if (!ok) fail();
+  }
+  __syncwarp();
+  __syncthreads();
+  if (PAIR) {
+    cluster_sync();   // neither CTA touches the other's memory from here on
+  } else if (split > 1) {
+    cluster_sync();
+    const int64_t t0 = (int64_t)(first / prm.mtiles) * NT;
+    join_partials(base, rank, split, (int)min((int64_t)NT, prm.T - t0), tile_row(first), t0, prm.out, prm.alpha, prm.dtype,
+                  prm.y);
+    cluster_sync();
+  }
+  if (warp == 3) {
+    tc_fence_after();
+    tmem_free<PAIR>(tmem, C::kTmem);
+  }
 }
+
+// x [T, K] -> bf16 parts [parts][T][Kp] that sum to x exactly: each part takes the next 8 significant
+// bits (truncated, so no part overflows); of a NaN or infinity the first part holds it all.
+template <typename S>
+__global__ void __launch_bounds__(256) parts_kernel(const S* __restrict__ x, int64_t T, int64_t K, int64_t ld, int64_t Kp,
+                                                    int parts, __nv_bfloat16* __restrict__ out) {
+  const int64_t per = Kp / 8, total = T * per;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t t = i / per, k = (i - t * per) * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = k + e < K ? float(x[t * ld + k + e]) : 0.0f;
+    for (int p = 0; p < parts; p++) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        uint32_t b = __float_as_uint(v[e]);
+        const bool odd = (b & 0x7F800000u) == 0x7F800000u;
+        if (odd && (b & 0x007FFFFFu)) b |= 0x00400000u;
+        b >>= 16;
+        v[e] = odd ? 0.0f : __fsub_rn(v[e], __uint_as_float(b << 16));
+        w[e / 2] = e & 1 ? w[e / 2] | b << 16 : b;
+      }
+      *reinterpret_cast<uint4*>(out + (p * T + t) * Kp + k) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+int parts_of(int dtype) { return dtype == kMxBF16 ? 1 : dtype == kMxF16 ? 2 : 3; }
+
+struct XView {
+  const void* p;   // bf16
+  int64_t rows, K, ld;
+};
+
+bool x_map(CUtensorMap* m, const XView& x, int box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)x.K, (cuuint64_t)x.rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)x.ld * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x.p), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int FMT, int NT, bool PAIR, bool TR, bool CHUNK>
+int launch_tiles(const XView& x, int parts, int64_t T, const Mx4View& w, float alpha, int dtype, void* y, int split,
+                 cudaStream_t stream) {
+  using C = Cfg<FMT, NT, PAIR, TR>;
+  const int64_t pitch = mx4_pitch(w.n), groups = pitch / (FMT == kMXFP4 ? 64 : 32), wt = (w.rows + 127) / 128;
+  CUtensorMap mw, ms, mx;
+  if (!codes_map(&mw, w.codes, pitch, w.rows, TR ? 64 : 128, 128) || !scales_map(&ms, w.scales, wt * groups, C::kAtoms) ||
+      !x_map(&mx, x, C::kXRows))
+    return 5;
+  LinParams p;
+  p.y = y;
+  p.T = T;
+  p.out = TR ? w.n : w.rows;
+  p.wrows = w.rows;
+  p.alpha = alpha;
+  p.dtype = dtype;
+  p.parts = parts;
+  p.steps = (int)((x.K + 63) / 64);
+  p.groups = (int)groups;
+  const int64_t mt = (p.out + 127) / 128;
+  p.mtiles = (int)(PAIR ? (mt + 1) / 2 : mt);
+  p.tiles = p.mtiles * (int)((T + NT - 1) / NT);
+  const int sms = device_sm_count();
+  const int grid = PAIR ? 2 * std::min(p.tiles, sms / 2) : split > 1 ? p.tiles * split : std::min(p.tiles, sms);
+  return launch_cluster<mx4_linear_kernel<FMT, NT, PAIR, TR, CHUNK>>(grid, kThreads, C::kSmem, PAIR ? 2 : split, stream, mw,
+                                                                    ms, mx, p, split);
+}
+
+template <int FMT, bool TR>
+int launch_form(const XView& x, int parts, int64_t T, const Mx4View& w, float alpha, int dtype, void* y,
+                cudaStream_t stream) {
+  const int sms = device_sm_count();
+  const int64_t mt = ((TR ? w.n : w.rows) + 127) / 128;
+  const int stages = (int)((x.K + (TR ? 127 : 255)) / (TR ? 128 : 256));
+  const bool chunk = dtype == kMxF32;
+  const int nt = chunk ? 64 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+  const int64_t tiles = mt * ((T + nt - 1) / nt), pairs = (mt + 1) / 2 * ((T + 255) / 256);
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= sms && split * 2 <= stages) split *= 2;
+  if (chunk) return launch_tiles<FMT, 64, false, TR, true>(x, parts, T, w, alpha, dtype, y, split, stream);
+  const double one = (double)((tiles + sms - 1) / sms) / split, pair = 1.6 * (double)((pairs + sms / 2 - 1) / (sms / 2));
+  if (T > 128 && pair <= one) return launch_tiles<FMT, 256, true, TR, false>(x, parts, T, w, alpha, dtype, y, 1, stream);
+  switch (nt) {
+    case 32: return launch_tiles<FMT, 32, false, TR, false>(x, parts, T, w, alpha, dtype, y, split, stream);
+    case 64: return launch_tiles<FMT, 64, false, TR, false>(x, parts, T, w, alpha, dtype, y, split, stream);
+    default: return launch_tiles<FMT, 128, false, TR, false>(x, parts, T, w, alpha, dtype, y, split, stream);
+  }
+}
+
+int64_t parts_pitch(int64_t K) { return (K + 7) / 8 * 8; }
 
 }  // namespace
 
-size_t mx4_linear_workspace_bytes(int, int64_t, int64_t, int64_t, int64_t, int, int) { return 0; }
-
-int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, const Mx4View& w, float alpha, int transpose,
-                      void* y, void*, cudaStream_t stream) {
-  return launch_product({}, x, dtype, T, ld, w, transpose, alpha, dtype, y, stream);
+size_t mx4_linear_workspace_bytes(int dtype, int64_t T, int64_t rows, int64_t n, int aligned, int transpose) {
+  if (dtype == kMxBF16 && aligned) return 0;
+  return (size_t)parts_of(dtype) * T * parts_pitch(transpose ? rows : n) * 2;
 }
+
+int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, int aligned, const Mx4View& w, float alpha,
+                      int transpose, void* y, void* ws, cudaStream_t stream) {
+  if (!bind_context()) return 6;
+  const int64_t K = transpose ? w.rows : w.n;
+  const int parts = parts_of(dtype);
+  XView xv{x, T, K, T == 1 ? parts_pitch(K) : ld};   // one row has no pitch of its own
+  if (mx4_linear_workspace_bytes(dtype, T, w.rows, w.n, aligned, transpose) > 0) {
+    const int64_t Kp = parts_pitch(K);
+    const unsigned grid = (unsigned)std::min<int64_t>((T * (Kp / 8) + 255) / 256, (int64_t)device_sm_count() * 8);
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(ws);
+    if (dtype == kMxBF16) parts_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), T, K, ld, Kp, parts, out);
+    else if (dtype == kMxF16) parts_kernel<<<grid, 256, 0, stream>>>(static_cast<const __half*>(x), T, K, ld, Kp, parts, out);
+    else parts_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(x), T, K, ld, Kp, parts, out);
+    note_launch();
+    xv = XView{ws, parts * T, K, Kp};
+  }
+  if (w.fmt == kMXFP4)
+    return transpose ? launch_form<kMXFP4, true>(xv, parts, T, w, alpha, dtype, y, stream)
+                     : launch_form<kMXFP4, false>(xv, parts, T, w, alpha, dtype, y, stream);
+  return transpose ? launch_form<kNVFP4, true>(xv, parts, T, w, alpha, dtype, y, stream)
+                   : launch_form<kNVFP4, false>(xv, parts, T, w, alpha, dtype, y, stream);
+}
+
+int mx4_linear_status(cudaStream_t stream, int* status) { return read_status_word(g_status, stream, status); }
 
 }  // namespace cpk

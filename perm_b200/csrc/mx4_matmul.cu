@@ -331,6 +331,7 @@ int launch_format(const Mx4View& a, const Mx4View& w, float alpha, int dtype, vo
 }  // namespace
 
 int launch_mx4_matmul(const Mx4View& a, const Mx4View& w, float alpha, int dtype, void* y, cudaStream_t stream) {
+  if (!bind_context()) return 6;
   return w.fmt == kMXFP4 ? launch_format<kMXFP4>(a, w, alpha, dtype, y, stream)
                          : launch_format<kNVFP4>(a, w, alpha, dtype, y, stream);
 }

@@ -89,7 +89,15 @@ template <auto K> inline bool opt_in_smem(size_t bytes) {
   return true;
 }
 
-// Tensor map of byte rows (128-byte swizzle for 128-byte boxes, none for narrower ones).
+// Makes the device's context current on this thread.  Tensor maps are made by the driver, which wants
+// one, and a thread that has only launched through PyTorch's deferred device selection (the
+// autograd engine's) may have none yet.
+inline bool bind_context() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+}
+
+// Tensor map of byte rows, boxes of 128 or 64 bytes swizzled over their width.
 inline bool codes_map(CUtensorMap* m, const uint8_t* p, int64_t pitch, int64_t rows, int box_bytes, int box_rows) {
   auto fn = encode_fn();
   if (!fn) return false;
@@ -98,7 +106,7 @@ inline bool codes_map(CUtensorMap* m, const uint8_t* p, int64_t pitch, int64_t r
   const cuuint32_t box[2] = {(cuuint32_t)box_bytes, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(p), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

@@ -113,6 +113,10 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
 }
+// Arrive on a barrier of the other CTA of the pair, after this thread's writes to shared memory.
+__device__ __forceinline__ void mbar_arrive_remote_release(uint32_t a) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
+}
 // mbar_wait by a converged warp, with one answer.
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t a, uint32_t parity, volatile int* abort,
                                                unsigned long long limit_ns) {
@@ -189,6 +193,14 @@ template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t dst, ui
 template <bool PAIR> __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
   if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
   else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+}
+
+// The same for a barrier that threads of the other CTA arrive on after writing shared memory.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t a, uint32_t parity, volatile int* abort,
+                                                  unsigned long long limit_ns) {
+  const bool got = mbar_wait(a, parity, abort, limit_ns);
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  return __all_sync(0xffffffffu, got);
 }
 
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {

@@ -43,13 +43,11 @@ template <int FMT, int NT, bool PAIR, bool TR> struct Cfg {
   static constexpr int kCodes = TR ? 128 * 64 : 128 * 128; // 128 w rows x 128 columns, or x 256
   static constexpr int kAtoms = (FMT == kMXFP4 ? 1 : 2) * (TR ? 1 : 2);   // its scale tiles
   static constexpr int kC = (kCodes + kAtoms * 512 + 1023) / 1024 * 1024;
-  static constexpr int kAS = 4, kCS = 3;
-  static constexpr int kFit = (224 * 1024 - kAS * kA - kCS * kC) / kB;
-  static constexpr int kBS = kFit < 8 ? kFit : 8;
-  static constexpr int kRing = kAS * kA + kBS * kB + kCS * kC;
-  static constexpr size_t kSmem = 1024 + (size_t)kRing + 512;
+  static constexpr int kCS = 3, kMaxStages = 8;
+  static constexpr int kRing = (224 * 1024 - kCS * kC) / 1024 * 1024;   // stages of one decoded tile and its x tiles
+  static constexpr size_t kSmem = 1024 + (size_t)kRing + kCS * kC + 512;
   static constexpr uint32_t kTmem = 2 * NT < 64 ? 64 : 2 * NT;
-  static_assert(kB % 1024 == 0 && kBS >= 3, "stages keep the swizzle's alignment");
+  static_assert(kB % 1024 == 0 && kRing >= NT * 512, "stages keep the swizzle's alignment, and a partial tile fits");
   // f32 accumulator, A and B bf16, A MN-major in the transposed form, N >> 3, M >> 4
   static constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((TR ? 1u : 0u) << 15) |
                                      ((uint32_t)(NT >> 3) << 17) | ((PAIR ? 16u : 8u) << 24);
@@ -62,9 +60,28 @@ struct LinParams {
   float alpha;
   int dtype;
   int parts;
+  int nst;              // stages of the ring
   int steps;            // 64-deep steps of the reduction
   int groups;           // scale tiles per 128 rows of w
   int mtiles, tiles;
+};
+
+// A place in a ring of n stages and the parity of its current use.
+struct Ring {
+  int st;
+  uint32_t ph;
+  __device__ __forceinline__ void advance(int k, int n) {   // 0 <= k <= n + 1
+    st += k;
+    while (st >= n) st -= n, ph ^= 1;
+  }
+  __device__ __forceinline__ void back(int n) {
+    if (--st < 0) st += n, ph ^= 1;
+  }
+  __device__ __forceinline__ Ring ahead(int k, int n) const {
+    Ring r = *this;
+    r.advance(k, n);
+    return r;
+  }
 };
 
 template <bool PAIR>
@@ -116,13 +133,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<FMT, NT, PAIR, TR>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::kRing);
-  constexpr int kBars = 2 * (C::kAS + C::kBS + C::kCS) + 5;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::kRing + C::kCS * C::kC);
+  constexpr int kBars = 2 * (C::kMaxStages + C::kCS) + 5;
   volatile int* misc = reinterpret_cast<volatile int*>(bars + kBars);   // [0] tmem, [1] abort
-  const uint32_t ring_a = smem_u32(base), ring_b = ring_a + C::kAS * C::kA, ring_c = ring_b + C::kBS * C::kB;
-  const uint32_t afull = smem_u32(bars), aempty = afull + 8 * C::kAS;
-  const uint32_t bfull = aempty + 8 * C::kAS, bempty = bfull + 8 * C::kBS;
-  const uint32_t cfull = bempty + 8 * C::kBS, cempty = cfull + 8 * C::kCS;
+  const int nst = prm.nst, stage_bytes = C::kA + prm.parts * C::kB;
+  const uint32_t ring = smem_u32(base), ring_c = ring + C::kRing;
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * C::kMaxStages;
+  const uint32_t cfull = empty0 + 8 * C::kMaxStages, cempty = cfull + 8 * C::kCS;
   const uint32_t accf = cempty + 8 * C::kCS, acce = accf + 16, done = acce + 16;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int rank = PAIR || split > 1 ? (int)cluster_rank() : 0;
@@ -137,13 +154,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto tile_row = [&](int tile) { return (int64_t)(tile % prm.mtiles) * (PAIR ? 256 : 128) + (PAIR ? rank * 128 : 0); };
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kAS; s++) {
-      mbar_init(afull + 8 * s, PAIR ? 16 : 8);
-      mbar_init(aempty + 8 * s, 1);
-    }
-    for (int s = 0; s < C::kBS; s++) {
-      mbar_init(bfull + 8 * s, 1);
-      mbar_init(bempty + 8 * s, 1);
+    for (int s = 0; s < C::kMaxStages; s++) {
+      mbar_init(full0 + 8 * s, 1 + (PAIR ? 8 : 4));   // the x loads, and the four warps that decode a step
+      mbar_init(empty0 + 8 * s, 1);
     }
     for (int s = 0; s < C::kCS; s++) {
       mbar_init(cfull + 8 * s, 1);
@@ -174,27 +187,36 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   if (warp == 0) {
-    if (lane == 0) {   // ---- x tiles, part by part
-      const uint32_t lead_bfull = PAIR ? peer_addr(bfull, 0) : bfull;
-      int it = 0;
+    if (lane == 0) {   // ---- x tiles, all parts of a step
+      const uint32_t lead_full = PAIR ? peer_addr(full0, 0) : full0;
+      Ring rg{0, 0};
+      int loads = 0;
       bool ok = true;
       for (int tile = first; ok && tile < prm.tiles; tile += stride) {
         const int t0 = tile / prm.mtiles * NT + (PAIR ? rank * C::kXRows : 0);
-        for (int s = s_begin; ok && s < s_end; s++)
-          for (int p = 0; p < prm.parts; p++, it++) {
-            const int st = it % C::kBS, round = it / C::kBS;
-            if (round > 0 && !mbar_wait(bempty + 8 * st, (round - 1) & 1, abort, kWaitNs)) {
-              ok = false;
-              break;
-            }
-            if (leader) mbar_expect_tx(bfull + 8 * st, (PAIR ? 2 : 1) * C::kB);
-            tma_load_group<PAIR>(ring_b + st * C::kB, &map_x, s * 64, (int)(p * prm.T) + t0, lead_bfull + 8 * st);
+        for (int s = s_begin; s < s_end; s++, loads++) {
+          if (loads >= nst && !mbar_wait(empty0 + 8 * rg.st, rg.ph ^ 1, abort, kWaitNs)) {
+            ok = false;
+            break;
           }
+          if (leader) mbar_expect_tx(full0 + 8 * rg.st, (PAIR ? 2 : 1) * prm.parts * C::kB);
+          const uint32_t sx = ring + rg.st * stage_bytes + C::kA;
+          for (int p = 0; p < prm.parts; p++)
+            tma_load_group<PAIR>(sx + p * C::kB, &map_x, s * 64, (int)(p * prm.T) + t0, lead_full + 8 * rg.st);
+          rg.advance(1, nst);
+        }
       }
       if (!ok) fail();
-      for (int k = max(0, it - C::kBS); k < it; k++) {   // every load issued lands before the CTA goes on
-        int zero = 0;
-        mbar_wait((leader ? bfull : bempty) + 8 * (k % C::kBS), (k / C::kBS) & 1, &zero, kWaitNs);
+      // Every load issued lands before the CTA goes on.  With all roles well, the last stages' MMAs,
+      // which waited for them, show that; after a failure the decoders may be missing from the
+      // full barriers, so wait as long as a load could take.
+      for (int k = min(loads, nst); ok && k > 0; k--) {
+        rg.back(nst);
+        ok = mbar_wait(empty0 + 8 * rg.st, rg.ph, abort, kWaitNs);
+      }
+      if (!ok) {
+        const unsigned long long t0 = gtime();
+        while (gtime() - t0 < 2000000ull) __nanosleep(10000);
       }
     }
   } else if (warp == 2) {
@@ -229,9 +251,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     if (leader) {   // ---- MMAs
       const bool elected = elect_one();
-      const uint32_t peer_aempty = PAIR ? peer_addr(aempty, 1) : 0, peer_bempty = PAIR ? peer_addr(bempty, 1) : 0;
-      const uint32_t peer_accf = PAIR ? peer_addr(accf, 1) : 0;
-      int ia = 0, ib = 0, cg = 0;
+      Ring rg{0, 0};
+      int cg = 0;
       bool ok = true;
       for (int tile = first; ok && tile < prm.tiles; tile += stride) {
         for (int g0 = s_begin; ok && g0 < s_end; cg++) {
@@ -241,43 +262,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
-          for (int s = g0; s < g1 && ok; s++, ia++) {
-            const int as = ia % C::kAS;
-            if (!(PAIR ? mbar_wait_cluster(afull + 8 * as, (ia / C::kAS) & 1, abort, kWaitNs)
-                       : mbar_wait_warp(afull + 8 * as, (ia / C::kAS) & 1, abort, kWaitNs))) {
+          for (int s = g0; s < g1; s++) {
+            if (!mbar_wait_warp<PAIR>(full0 + 8 * rg.st, rg.ph, abort, kWaitNs)) {
               ok = false;
               break;
             }
-            const uint32_t sa = ring_a + as * C::kA;
+            tc_fence_after();
+            const uint32_t sa = ring + rg.st * stage_bytes;
             const uint64_t ad = TR ? sw128_desc(sa, 8192, 1024) : sw128_desc(sa, 16, 1024);
-            for (int p = 0; p < prm.parts; p++, ib++) {
-              const int bs = ib % C::kBS;
-              if (!mbar_wait_warp(bfull + 8 * bs, (ib / C::kBS) & 1, abort, kWaitNs)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              const uint64_t bd = sw128_desc(ring_b + bs * C::kB, 16, 1024);
-              const uint32_t more = s > g0 || p > 0;
-              if (elected) {
+            const uint64_t bd = sw128_desc(sa + C::kA, 16, 1024);
+            if (elected) {
+              for (int p = 0; p < prm.parts; p++)
 #pragma unroll
                 for (int kk = 0; kk < 4; kk++)   // 16 deep: 32 bytes of a K-major row, or 16 rows of 128
-                  umma_bf16<PAIR>(acc, ad + (TR ? 128 : 2) * kk, bd + 2 * kk, C::kIdesc, kk > 0 ? 1u : more);
-                umma_commit_group<PAIR>(bempty + 8 * bs);
-                if (PAIR) umma_commit_pair(peer_bempty + 8 * bs);
-              }
-              __syncwarp();
-            }
-            if (ok && elected) {
-              umma_commit_group<PAIR>(aempty + 8 * as);
-              if (PAIR) umma_commit_pair(peer_aempty + 8 * as);
+                  umma_bf16<PAIR>(acc, ad + (TR ? 128 : 2) * kk, bd + p * (C::kB / 16) + 2 * kk, C::kIdesc,
+                                  (uint32_t)(s - g0) | p | kk);
+              umma_commit_group<PAIR>(empty0 + 8 * rg.st);
             }
             __syncwarp();
+            rg.advance(1, nst);
           }
-          if (ok && elected) {
-            umma_commit_group<PAIR>(accf + 8 * b);
-            if (PAIR) umma_commit_pair(peer_accf + 8 * b);
-          }
+          if (ok && elected) umma_commit_group<PAIR>(accf + 8 * b);
           __syncwarp();
           g0 = g1;
         }
@@ -288,14 +293,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait(done, 0, &zero, kWaitNs);
     }
   } else if (warp >= 8) {
-    // ---- decoding: a thread takes 32 codes (16 bytes) of a 64-deep step: half of a row's, or (TR) a
-    // quarter of a w row's 128 columns
-    const int d = threadIdx.x - 256;
-    const int r = TR ? d & 63 : d & 127, h = TR ? d >> 6 : d >> 7;
-    const uint32_t dst0 = TR ? (h >> 1) * 8192 + r * 128 : r * 128;
-    const int chunk0 = TR ? (h & 1) * 4 : h * 4, x7 = r & 7;
-    const uint32_t lead_afull = PAIR ? peer_addr(afull, 0) : afull;
-    int ia = 0, ic = 0;
+    // ---- decoding.  Two groups of four warps take alternate 64-deep steps, so one group's waits and
+    // fences overlap the other's work; a thread takes 64 codes (32 bytes) of a step: a row's, or (TR)
+    // half of a w row's 128 columns.  It decodes into registers before it waits for the stage.
+    const int d = threadIdx.x & 127, g = (threadIdx.x - 256) >> 7;
+    const int r = TR ? d & 63 : d, h = TR ? d >> 6 : 0, x7 = r & 7;
+    const uint32_t dst0 = h * 8192 + r * 128;
+    const uint32_t lead_full = PAIR ? peer_addr(full0, 0) : full0;
+    Ring rg{0, 0};
+    int ic = 0, seen = 0;
     bool ok = true;
     for (int tile = first; ok && tile < prm.tiles; tile += stride)
       for (int c = c_begin; c < c_end && ok; c++, ic++) {
@@ -304,56 +310,67 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = false;
           break;
         }
-        const uint8_t* codes = base + C::kAS * C::kA + C::kBS * C::kB + cs * C::kC;
+        const uint8_t* codes = base + C::kRing + cs * C::kC;
         const uint8_t* scales = codes + C::kCodes;
         const int subs = min(C::kSub, prm.steps - c * C::kSub);
-        for (int sub = 0; sub < subs; sub++, ia++) {
+        for (int sub = g; sub < subs; sub += 2) {
           const int R = TR ? sub * 64 + r : r;   // row of the code stage
-          const uint32_t at = TR ? R * 64 + ((h ^ ((R >> 1) & 3)) << 4) : R * 128 + (((sub * 2 + h) ^ x7) << 4);
-          const uint4 q = *reinterpret_cast<const uint4*>(codes + at);
+          uint4 q[2];
+          uint32_t f[4], more[2] = {0, 0};
           const int srow = (R & 31) * 16 + (R >> 5) * 4;
-          uint32_t f0, f1, more = 0;
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+            q[j] = *reinterpret_cast<const uint4*>(codes + (TR ? R * 64 + (((h * 2 + j) ^ ((R >> 1) & 3)) << 4)
+                                                               : R * 128 + (((sub * 2 + j) ^ x7) << 4)));
           if (FMT == kMXFP4) {
-            const uint32_t byte = TR ? scales[srow + h] : scales[(sub >> 1) * 512 + srow + (sub & 1) * 2 + h];
-            f0 = f1 = factor_e8m0(byte, more);
+            const uint32_t two = *reinterpret_cast<const uint16_t*>(TR ? scales + srow + h * 2
+                                                                       : scales + (sub >> 1) * 512 + srow + (sub & 1) * 2);
+            f[0] = f[1] = factor_e8m0(two & 0xFF, more[0]);
+            f[2] = f[3] = factor_e8m0(two >> 8, more[1]);
           } else {
-            const uint8_t* s2 = TR ? scales + (h >> 1) * 512 + srow + (h & 1) * 2 : scales + sub * 512 + srow + h * 2;
-            const uint32_t two = *reinterpret_cast<const uint16_t*>(s2);
-            f0 = factor_e4m3(two & 0xFF);
-            f1 = factor_e4m3(two >> 8);
+            const uint32_t four = *reinterpret_cast<const uint32_t*>(scales + (TR ? h : sub) * 512 + srow);
+#pragma unroll
+            for (int j = 0; j < 4; j++) f[j] = factor_e4m3((four >> (8 * j)) & 0xFF);
           }
           // rows past the last (their scale bytes are not defined) are part of the reduction: zero
-          if (TR && (int64_t)c * 128 + R >= prm.wrows) f0 = f1 = more = 0;
-          const int as = ia % C::kAS;
-          if (ia >= C::kAS && !mbar_wait_warp(aempty + 8 * as, (ia / C::kAS - 1) & 1, abort, kWaitNs)) {
+          if (TR && (int64_t)c * 128 + R >= prm.wrows) {
+            f[0] = f[1] = f[2] = f[3] = 0;
+            more[0] = more[1] = 0;
+          }
+          uint32_t v[8][4];
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const uint4& qq = q[i / 4];
+            decode8(i % 4 == 0 ? qq.x : i % 4 == 1 ? qq.y : i % 4 == 2 ? qq.z : qq.w, v[i]);
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[i][k] = mul_bf16x2(v[i][k], f[i / 2]);
+            if (FMT == kMXFP4 && more[i / 4]) {
+#pragma unroll
+              for (int k = 0; k < 4; k++) v[i][k] = mul_bf16x2(v[i][k], more[i / 4]);
+            }
+          }
+          const Ring at = rg.ahead(sub, nst);
+          if (seen + sub >= nst && !mbar_wait_warp(empty0 + 8 * at.st, at.ph ^ 1, abort, kWaitNs)) {
             ok = false;
             break;
           }
-          const uint32_t dst = ring_a + as * C::kA + dst0;
-          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+          const uint32_t dst = ring + at.st * stage_bytes + dst0;
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            uint32_t v[4];
-            decode8(w[i], v);
-#pragma unroll
-            for (int k = 0; k < 4; k++) v[k] = mul_bf16x2(v[k], i < 2 ? f0 : f1);
-            if (FMT == kMXFP4 && more) {
-#pragma unroll
-              for (int k = 0; k < 4; k++) v[k] = mul_bf16x2(v[k], more);
-            }
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (((chunk0 + i) ^ x7) << 4)), "r"(v[0]),
-                         "r"(v[1]), "r"(v[2]), "r"(v[3])
+          for (int i = 0; i < 8; i++)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + ((i ^ x7) << 4)), "r"(v[i][0]), "r"(v[i][1]),
+                         "r"(v[i][2]), "r"(v[i][3])
                          : "memory");
-          }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read through the async proxy
           __syncwarp();
           if (lane == 0) {
-            if (leader) mbar_arrive(afull + 8 * as);
-            else mbar_arrive_remote_release(lead_afull + 8 * as);
+            if (leader) mbar_arrive(full0 + 8 * at.st);
+            else mbar_arrive_remote_release(lead_full + 8 * at.st);
           }
         }
         __syncwarp();
         if (ok && lane == 0) mbar_arrive(cempty + 8 * cs);
+        rg.advance(subs, nst);
+        seen += subs;
       }
     if (!ok) fail();
   } else if (warp >= 4) {
@@ -511,6 +528,7 @@ int launch_tiles(const XView& x, int parts, int64_t T, const Mx4View& w, float a
   p.alpha = alpha;
   p.dtype = dtype;
   p.parts = parts;
+  p.nst = std::min(C::kMaxStages, C::kRing / (C::kA + parts * C::kB));
   p.steps = (int)((x.K + 63) / 64);
   p.groups = (int)groups;
   const int64_t mt = (p.out + 127) / 128;

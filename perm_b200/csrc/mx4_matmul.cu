@@ -186,7 +186,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     if (leader) {
       const bool elected = elect_one();
-      const uint32_t peer_empty0 = PAIR ? peer_addr(empty0, 1) : 0, peer_accf = PAIR ? peer_addr(accf, 1) : 0;
       int it = 0, n = 0;
       bool ok = true;
       for (int tile = first; ok && tile < prm.tiles; tile += stride, n++) {
@@ -221,14 +220,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                                   tb + 4 * C::kXT * atom, kk > 0 ? 1u : more);
             }
             umma_commit_group<PAIR>(empty0 + 8 * st);
-            if (PAIR) umma_commit_pair(peer_empty0 + 8 * st);
           }
           __syncwarp();
         }
-        if (ok && elected) {
-          umma_commit_group<PAIR>(accf);
-          if (PAIR) umma_commit_pair(peer_accf);
-        }
+        if (ok && elected) umma_commit_group<PAIR>(accf);
         __syncwarp();
       }
       if (!ok) fail();

@@ -52,25 +52,36 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t a) {
 // loops of waiting warps slow the warp that issues the MMAs (a 4-bit product in one-SM tiles: 322 us
 // against 260).
 constexpr uint32_t kTryNs = 50000;
-__device__ __forceinline__ bool mbar_try(uint32_t a, uint32_t parity) {
+// CLUSTER: with the writes of threads of the other CTA of the pair that arrived with release.
+template <bool CLUSTER = false> __device__ __forceinline__ bool mbar_try(uint32_t a, uint32_t parity) {
   uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(a), "r"(parity), "r"(kTryNs)
-      : "memory");
+  if (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(a), "r"(parity), "r"(kTryNs)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(a), "r"(parity), "r"(kTryNs)
+        : "memory");
   return ok != 0;
 }
 // Bounded wait for the phase with the given parity.  False when it ran out (limit_ns of
 // global time) or a role of this CTA pair gave up (abort word nonzero).
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(uint32_t a, uint32_t parity, volatile int* abort,
                                           unsigned long long limit_ns) {
-  if (mbar_try(a, parity)) return true;
+  if (mbar_try<CLUSTER>(a, parity)) return true;
   const unsigned long long t0 = gtime();
   for (uint32_t n = 1; n < (1u << 30); n++) {
-    if (mbar_try(a, parity)) return true;
+    if (mbar_try<CLUSTER>(a, parity)) return true;
     if (*abort || gtime() - t0 > limit_ns) return false;
   }
   return false;
@@ -118,9 +129,10 @@ __device__ __forceinline__ void mbar_arrive_remote_release(uint32_t a) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
 }
 // mbar_wait by a converged warp, with one answer.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t a, uint32_t parity, volatile int* abort,
                                                unsigned long long limit_ns) {
-  const bool got = mbar_wait(a, parity, abort, limit_ns);
+  const bool got = mbar_wait<CLUSTER>(a, parity, abort, limit_ns);
   return __all_sync(0xffffffffu, got);
 }
 // Load into this CTA's shared memory, completing on a barrier of either CTA of the pair.
@@ -176,9 +188,16 @@ __device__ __forceinline__ void tma_load_group(uint32_t dst, const CUtensorMap* 
   if (PAIR) tma_load_pair(dst, map, x, y, mbar);
   else tma_load(dst, map, x, y, mbar);
 }
+// Arrive on the barrier at this shared-memory offset, in both CTAs of a pair, once the MMAs issued so
+// far complete.
 template <bool PAIR> __device__ __forceinline__ void umma_commit_group(uint32_t mbar) {
-  if (PAIR) umma_commit_pair(mbar);
-  else umma_commit(mbar);
+  if (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(mbar),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    umma_commit(mbar);
 }
 // By one converged warp (of each CTA of a pair); the address lands in shared memory at `dst`.
 template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
@@ -193,14 +212,6 @@ template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t dst, ui
 template <bool PAIR> __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
   if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
   else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
-}
-
-// The same for a barrier that threads of the other CTA arrive on after writing shared memory.
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t a, uint32_t parity, volatile int* abort,
-                                                  unsigned long long limit_ns) {
-  const bool got = mbar_wait(a, parity, abort, limit_ns);
-  asm volatile("fence.acq_rel.cluster;" ::: "memory");
-  return __all_sync(0xffffffffu, got);
 }
 
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {

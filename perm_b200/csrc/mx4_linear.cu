@@ -4,10 +4,10 @@
 //
 // Tensor-core kernel (tcgen05 kind::f16, bf16 x bf16 -> f32).  An e2m1 value times its block scale
 // has at most six significant bits, so it is exact in bf16, and so is every product in the float32
-// accumulator.  The 4-bit weights go from global to shared memory as they are (TMA) and eight warps
-// decode them there, 64 columns of the reduction at a time, into the swizzled bf16 tile that the
-// MMA reads: the K-major one for x w^T, the MN-major one for x w, where the packed axis is the
-// output's.  Weights are the M side (128 rows of the output per CTA), tokens the N side.
+// accumulator.  The 4-bit weights go from global to shared memory as they are (TMA), 128 x 128 at a
+// time, and decoding warps write them as the swizzled bf16 tile that the MMA reads: K-major for
+// x w^T, MN-major for x w, where the packed axis is the output's.  Both are the same bytes: two
+// halves of 64 columns, 128 bytes a row.  Weights are the M side (128 rows of the output per CTA), tokens the N side.
 //
 // Decoding.  cvt turns two codes into two f16 values; f16 holds an e2m1 value in the sign and the
 // top six bits, and the same bits three places lower are the bf16 of the value times 2^-112.  One
@@ -32,19 +32,21 @@ namespace {
 __device__ int g_status;
 
 constexpr unsigned long long kWaitNs = 1000000000ull;
-constexpr int kThreads = 512;   // warps: 0 x loads, 1 MMA, 2 code loads, 3 allocation, 4-7 epilogue, 8-15 decoding
-constexpr int kChunkSteps = 3;  // 64-deep steps of one float32 accumulation chain (36 MMAs with three parts)
+constexpr int kChunkSteps = 1;  // 128-deep steps of one float32 accumulation chain (24 MMAs with three parts)
 
-template <int FMT, int NT, bool PAIR, bool TR> struct Cfg {
+template <int FMT, int NT, bool PAIR, bool TR, bool CHUNK> struct Cfg {
+  // warps: 0 x loads, 1 MMA, 2 code loads, 3 allocation, 4-7 epilogue, then groups of eight that decode
+  // alternate steps.  float32 results keep NT sums per epilogue thread, which leaves registers for one group.
+  static constexpr int kGroups = CHUNK ? 1 : 2;
+  static constexpr int kThreads = 256 + 256 * kGroups;
   static constexpr int kXRows = PAIR ? NT / 2 : NT;
-  static constexpr int kA = 128 * 128;                     // decoded tile: 128 rows x 64, bf16
-  static constexpr int kB = kXRows * 128;                  // tokens x 64, bf16
-  static constexpr int kSub = TR ? 2 : 4;                  // 64-deep steps per code stage
-  static constexpr int kCodes = TR ? 128 * 64 : 128 * 128; // 128 w rows x 128 columns, or x 256
-  static constexpr int kAtoms = (FMT == kMXFP4 ? 1 : 2) * (TR ? 1 : 2);   // its scale tiles
+  static constexpr int kA = 128 * 256;                     // decoded tile: 128 rows x 128, bf16
+  static constexpr int kB = kXRows * 256;                  // tokens x 128, bf16
+  static constexpr int kAtoms = FMT == kMXFP4 ? 1 : 2;     // scale tiles of 128 x 128 codes
+  static constexpr int kCodes = 128 * 64;
   static constexpr int kC = (kCodes + kAtoms * 512 + 1023) / 1024 * 1024;
-  static constexpr int kCS = 3, kMaxStages = 8;
-  static constexpr int kRing = (224 * 1024 - kCS * kC) / 1024 * 1024;   // stages of one decoded tile and its x tiles
+  static constexpr int kCS = 3, kMaxStages = 6;
+  static constexpr int kRing = (225 * 1024 - kCS * kC) / 1024 * 1024;   // stages of one decoded tile and its x tiles
   static constexpr size_t kSmem = 1024 + (size_t)kRing + kCS * kC + 512;
   static constexpr uint32_t kTmem = 2 * NT < 64 ? 64 : 2 * NT;
   static_assert(kB % 1024 == 0 && kRing >= NT * 512, "stages keep the swizzle's alignment, and a partial tile fits");
@@ -61,7 +63,7 @@ struct LinParams {
   int dtype;
   int parts;
   int nst;              // stages of the ring
-  int steps;            // 64-deep steps of the reduction
+  int steps;            // 128-deep steps of the reduction
   int groups;           // scale tiles per 128 rows of w
   int mtiles, tiles;
 };
@@ -70,17 +72,11 @@ struct LinParams {
 struct Ring {
   int st;
   uint32_t ph;
-  __device__ __forceinline__ void advance(int k, int n) {   // 0 <= k <= n + 1
-    st += k;
-    while (st >= n) st -= n, ph ^= 1;
+  __device__ __forceinline__ void advance(int n) {
+    if (++st == n) st = 0, ph ^= 1;
   }
   __device__ __forceinline__ void back(int n) {
     if (--st < 0) st += n, ph ^= 1;
-  }
-  __device__ __forceinline__ Ring ahead(int k, int n) const {
-    Ring r = *this;
-    r.advance(k, n);
-    return r;
   }
 };
 
@@ -127,10 +123,10 @@ __device__ __forceinline__ void decode8(uint32_t w, uint32_t (&v)[4]) {
 }
 
 template <int FMT, int NT, bool PAIR, bool TR, bool CHUNK>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
     mx4_linear_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
                       const __grid_constant__ CUtensorMap map_x, const LinParams prm, int split) {
-  using C = Cfg<FMT, NT, PAIR, TR>;
+  using C = Cfg<FMT, NT, PAIR, TR, CHUNK>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::kRing + C::kCS * C::kC);
@@ -146,16 +142,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool leader = !PAIR || rank == 0;
   const int group = PAIR ? 2 : split;
   const int first = (int)blockIdx.x / group, stride = (int)gridDim.x / group;
-  // this CTA's code stages, and its 64-deep steps
-  const int stages = (prm.steps + C::kSub - 1) / C::kSub;
-  const int c_begin = PAIR ? 0 : (int)((int64_t)stages * rank / split);
-  const int c_end = PAIR ? stages : (int)((int64_t)stages * (rank + 1) / split);
-  const int s_begin = c_begin * C::kSub, s_end = min(prm.steps, c_end * C::kSub);
+  const int s_begin = PAIR ? 0 : (int)((int64_t)prm.steps * rank / split);   // this CTA's steps
+  const int s_end = PAIR ? prm.steps : (int)((int64_t)prm.steps * (rank + 1) / split);
   auto tile_row = [&](int tile) { return (int64_t)(tile % prm.mtiles) * (PAIR ? 256 : 128) + (PAIR ? rank * 128 : 0); };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kMaxStages; s++) {
-      mbar_init(full0 + 8 * s, 1 + (PAIR ? 8 : 4));   // the x loads, and the four warps that decode a step
+      mbar_init(full0 + 8 * s, 1 + (PAIR ? 16 : 8));   // the x loads, and the warps that decode the step
       mbar_init(empty0 + 8 * s, 1);
     }
     for (int s = 0; s < C::kCS; s++) {
@@ -202,8 +195,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (leader) mbar_expect_tx(full0 + 8 * rg.st, (PAIR ? 2 : 1) * prm.parts * C::kB);
           const uint32_t sx = ring + rg.st * stage_bytes + C::kA;
           for (int p = 0; p < prm.parts; p++)
-            tma_load_group<PAIR>(sx + p * C::kB, &map_x, s * 64, (int)(p * prm.T) + t0, lead_full + 8 * rg.st);
-          rg.advance(1, nst);
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+              tma_load_group<PAIR>(sx + p * C::kB + k * (C::kB / 2), &map_x, s * 128 + k * 64, (int)(p * prm.T) + t0,
+                                   lead_full + 8 * rg.st);
+          rg.advance(nst);
         }
       }
       if (!ok) fail();
@@ -225,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int tile = first; ok && tile < prm.tiles; tile += stride) {
         const int m0 = (int)tile_row(tile);
-        for (int c = c_begin; c < c_end; c++, it++) {
+        for (int s = s_begin; s < s_end; s++, it++) {
           const int st = it % C::kCS, round = it / C::kCS;
           if (round > 0 && !mbar_wait(cempty + 8 * st, (round - 1) & 1, abort, kWaitNs)) {
             ok = false;
@@ -234,11 +230,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t fb = cfull + 8 * st, sc = ring_c + st * C::kC;
           mbar_expect_tx(fb, C::kCodes + C::kAtoms * 512);
           if (TR) {
-            tma_load(sc, &map_w, m0 / 2, c * 128, fb);
-            tma_load(sc + C::kCodes, &map_s, 0, c * prm.groups + m0 / 128 * C::kAtoms, fb);
+            tma_load(sc, &map_w, m0 / 2, s * 128, fb);
+            tma_load(sc + C::kCodes, &map_s, 0, s * prm.groups + m0 / 128 * C::kAtoms, fb);
           } else {
-            tma_load(sc, &map_w, c * 128, m0, fb);
-            tma_load(sc + C::kCodes, &map_s, 0, m0 / 128 * prm.groups + c * C::kAtoms, fb);
+            tma_load(sc, &map_w, s * 64, m0, fb);
+            tma_load(sc + C::kCodes, &map_s, 0, m0 / 128 * prm.groups + s * C::kAtoms, fb);
           }
         }
       }
@@ -269,18 +265,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc_fence_after();
             const uint32_t sa = ring + rg.st * stage_bytes;
-            const uint64_t ad = TR ? sw128_desc(sa, 8192, 1024) : sw128_desc(sa, 16, 1024);
+            const uint64_t ad = TR ? sw128_desc(sa, 16384, 1024) : sw128_desc(sa, 16, 1024);
             const uint64_t bd = sw128_desc(sa + C::kA, 16, 1024);
             if (elected) {
               for (int p = 0; p < prm.parts; p++)
 #pragma unroll
-                for (int kk = 0; kk < 4; kk++)   // 16 deep: 32 bytes of a K-major row, or 16 rows of 128
-                  umma_bf16<PAIR>(acc, ad + (TR ? 128 : 2) * kk, bd + p * (C::kB / 16) + 2 * kk, C::kIdesc,
+                for (int kk = 0; kk < 8; kk++)   // 16 deep: 32 bytes of a K-major row (four to a half), or 16 rows
+                  umma_bf16<PAIR>(acc, ad + (TR ? 128 * kk : kk / 4 * 1024 + kk % 4 * 2),
+                                  bd + p * (C::kB / 16) + kk / 4 * (C::kB / 32) + kk % 4 * 2, C::kIdesc,
                                   (uint32_t)(s - g0) | p | kk);
               umma_commit_group<PAIR>(empty0 + 8 * rg.st);
             }
             __syncwarp();
-            rg.advance(1, nst);
+            rg.advance(nst);
           }
           if (ok && elected) umma_commit_group<PAIR>(accf + 8 * b);
           __syncwarp();
@@ -293,47 +290,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait(done, 0, &zero, kWaitNs);
     }
   } else if (warp >= 8) {
-    // ---- decoding.  Two groups of four warps take alternate 64-deep steps, so one group's waits and
-    // fences overlap the other's work; a thread takes 64 codes (32 bytes) of a step: a row's, or (TR)
-    // half of a w row's 128 columns.  It decodes into registers before it waits for the stage.
-    const int d = threadIdx.x & 127, g = (threadIdx.x - 256) >> 7;
-    const int r = TR ? d & 63 : d, h = TR ? d >> 6 : 0, x7 = r & 7;
-    const uint32_t dst0 = h * 8192 + r * 128;
+    // ---- decoding.  Groups take alternate steps, so one group's waits and fences overlap the other's
+    // work; a thread takes 64 codes (32 bytes): half of a row's 128.  It decodes into registers before it
+    // waits for the stage.
+    const int d = threadIdx.x & 255, g = (threadIdx.x - 256) >> 8;
+    const int r = d & 127, h = d >> 7, x7 = r & 7;
+    const uint32_t dst0 = h * 16384 + r * 128;
+    const uint32_t at0 = r * 64 + (((h * 2) ^ ((r >> 1) & 3)) << 4), at1 = r * 64 + (((h * 2 + 1) ^ ((r >> 1) & 3)) << 4);
+    const int srow = (r & 31) * 16 + (r >> 5) * 4;
     const uint32_t lead_full = PAIR ? peer_addr(full0, 0) : full0;
     Ring rg{0, 0};
-    int ic = 0, seen = 0;
+    int seen = 0;
     bool ok = true;
     for (int tile = first; ok && tile < prm.tiles; tile += stride)
-      for (int c = c_begin; c < c_end && ok; c++, ic++) {
-        const int cs = ic % C::kCS;
-        if (!mbar_wait_warp(cfull + 8 * cs, (ic / C::kCS) & 1, abort, kWaitNs)) {
+      for (int s = s_begin; s < s_end; s++, seen++, rg.advance(nst)) {
+        if (C::kGroups > 1 && (seen & 1) != g) continue;
+        const int cs = seen % C::kCS;
+        if (!mbar_wait_warp(cfull + 8 * cs, (seen / C::kCS) & 1, abort, kWaitNs)) {
           ok = false;
           break;
         }
         const uint8_t* codes = base + C::kRing + cs * C::kC;
-        const uint8_t* scales = codes + C::kCodes;
-        const int subs = min(C::kSub, prm.steps - c * C::kSub);
-        for (int sub = g; sub < subs; sub += 2) {
-          const int R = TR ? sub * 64 + r : r;   // row of the code stage
-          uint4 q[2];
+        const uint8_t* scales = codes + C::kCodes + srow;
+        {
+          const uint4 q[2] = {*reinterpret_cast<const uint4*>(codes + at0), *reinterpret_cast<const uint4*>(codes + at1)};
           uint32_t f[4], more[2] = {0, 0};
-          const int srow = (R & 31) * 16 + (R >> 5) * 4;
-#pragma unroll
-          for (int j = 0; j < 2; j++)
-            q[j] = *reinterpret_cast<const uint4*>(codes + (TR ? R * 64 + (((h * 2 + j) ^ ((R >> 1) & 3)) << 4)
-                                                               : R * 128 + (((sub * 2 + j) ^ x7) << 4)));
           if (FMT == kMXFP4) {
-            const uint32_t two = *reinterpret_cast<const uint16_t*>(TR ? scales + srow + h * 2
-                                                                       : scales + (sub >> 1) * 512 + srow + (sub & 1) * 2);
+            const uint32_t two = *reinterpret_cast<const uint16_t*>(scales + h * 2);
             f[0] = f[1] = factor_e8m0(two & 0xFF, more[0]);
             f[2] = f[3] = factor_e8m0(two >> 8, more[1]);
           } else {
-            const uint32_t four = *reinterpret_cast<const uint32_t*>(scales + (TR ? h : sub) * 512 + srow);
+            const uint32_t four = *reinterpret_cast<const uint32_t*>(scales + h * 512);
 #pragma unroll
             for (int j = 0; j < 4; j++) f[j] = factor_e4m3((four >> (8 * j)) & 0xFF);
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(cempty + 8 * cs);   // the stage's bytes are in registers
           // rows past the last (their scale bytes are not defined) are part of the reduction: zero
-          if (TR && (int64_t)c * 128 + R >= prm.wrows) {
+          if (TR && (int64_t)s * 128 + r >= prm.wrows) {
             f[0] = f[1] = f[2] = f[3] = 0;
             more[0] = more[1] = 0;
           }
@@ -349,28 +343,23 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int k = 0; k < 4; k++) v[i][k] = mul_bf16x2(v[i][k], more[i / 4]);
             }
           }
-          const Ring at = rg.ahead(sub, nst);
-          if (seen + sub >= nst && !mbar_wait_warp(empty0 + 8 * at.st, at.ph ^ 1, abort, kWaitNs)) {
+          if (seen >= nst && !mbar_wait_warp(empty0 + 8 * rg.st, rg.ph ^ 1, abort, kWaitNs)) {
             ok = false;
             break;
           }
-          const uint32_t dst = ring + at.st * stage_bytes + dst0;
+          const uint32_t dst = ring + rg.st * stage_bytes + dst0;
 #pragma unroll
           for (int i = 0; i < 8; i++)
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + ((i ^ x7) << 4)), "r"(v[i][0]), "r"(v[i][1]),
                          "r"(v[i][2]), "r"(v[i][3])
                          : "memory");
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read through the async proxy
-          __syncwarp();
-          if (lane == 0) {
-            if (leader) mbar_arrive(full0 + 8 * at.st);
-            else mbar_arrive_remote_release(lead_full + 8 * at.st);
-          }
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read through the async proxy
         __syncwarp();
-        if (ok && lane == 0) mbar_arrive(cempty + 8 * cs);
-        rg.advance(subs, nst);
-        seen += subs;
+        if (lane == 0) {
+          if (leader) mbar_arrive(full0 + 8 * rg.st);
+          else mbar_arrive_remote_release(lead_full + 8 * rg.st);
+        }
       }
     if (!ok) fail();
   } else if (warp >= 4) {
@@ -383,20 +372,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int tile = first; ok && tile < prm.tiles; tile += stride) {
       const int64_t row0 = tile_row(tile) + 32 * q, t0 = (int64_t)(tile / prm.mtiles) * NT;
-      auto emit = [&](const float(&v)[32], int c) {   // columns c .. c + 31 of the tile
+      auto emit = [&](const float(&v)[16], int c) {   // columns c .. c + 15 of the tile
         if (split > 1) {   // the loads and MMAs of this CTA's only tile are complete: the rings are free
 #pragma unroll
-          for (int e = 0; e < 32; e++) part[(c + e) * 128 + 32 * q + lane] = v[e];
+          for (int e = 0; e < 16; e++) part[(c + e) * 128 + 32 * q + lane] = v[e];
         } else {
-          store_tile<32>(v, prm.alpha, prm.y, prm.dtype, row0, prm.out, t0 + c, prm.T);
+          store_tile<16>(v, prm.alpha, prm.y, prm.dtype, row0, prm.out, t0 + c, prm.T);
         }
       };
       if constexpr (CHUNK) {
-        float m[NT / 32][32];
+        float m[NT / 16][16];
 #pragma unroll
-        for (int c = 0; c < NT / 32; c++)
+        for (int c = 0; c < NT / 16; c++)
 #pragma unroll
-          for (int e = 0; e < 32; e++) m[c][e] = 0.0f;
+          for (int e = 0; e < 16; e++) m[c][e] = 0.0f;
         for (int g0 = s_begin; g0 < s_end; g0 += kChunkSteps, cg++) {
           const int b = cg & 1;
           if (!mbar_wait_warp(accf + 8 * b, (cg >> 1) & 1, abort, kWaitNs)) {
@@ -405,11 +394,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < NT / 32; c++) {
-            float v[32];
-            tmem_ld_cols(trow + b * NT + 32 * c, v);
+          for (int c = 0; c < NT / 16; c++) {
+            float v[16];
+            tmem_ld_cols(trow + b * NT + 16 * c, v);
 #pragma unroll
-            for (int e = 0; e < 32; e++) m[c][e] += v[e];
+            for (int e = 0; e < 16; e++) m[c][e] += v[e];
           }
           tc_fence_before();
           __syncwarp();
@@ -420,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (ok) {
 #pragma unroll
-          for (int c = 0; c < NT / 32; c++) emit(m[c], 32 * c);
+          for (int c = 0; c < NT / 16; c++) emit(m[c], 16 * c);
         }
       } else {
         const int b = cg & 1;
@@ -430,10 +419,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
 #pragma unroll 1
-        for (int c = 0; c < NT; c += 32) {
-          float v[32];
+        for (int c = 0; c < NT; c += 16) {
+          float v[16];
           tmem_ld_cols(trow + b * NT + c, v);
-          if (c + 32 == NT) {
+          if (c + 16 == NT) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -514,10 +503,10 @@ bool x_map(CUtensorMap* m, const XView& x, int box_rows) {
 template <int FMT, int NT, bool PAIR, bool TR, bool CHUNK>
 int launch_tiles(const XView& x, int parts, int64_t T, const Mx4View& w, float alpha, int dtype, void* y, int split,
                  cudaStream_t stream) {
-  using C = Cfg<FMT, NT, PAIR, TR>;
+  using C = Cfg<FMT, NT, PAIR, TR, CHUNK>;
   const int64_t pitch = mx4_pitch(w.n), groups = pitch / (FMT == kMXFP4 ? 64 : 32), wt = (w.rows + 127) / 128;
   CUtensorMap mw, ms, mx;
-  if (!codes_map(&mw, w.codes, pitch, w.rows, TR ? 64 : 128, 128) || !scales_map(&ms, w.scales, wt * groups, C::kAtoms) ||
+  if (!codes_map(&mw, w.codes, pitch, w.rows, 64, 128) || !scales_map(&ms, w.scales, wt * groups, C::kAtoms) ||
       !x_map(&mx, x, C::kXRows))
     return 5;
   LinParams p;
@@ -529,14 +518,14 @@ int launch_tiles(const XView& x, int parts, int64_t T, const Mx4View& w, float a
   p.dtype = dtype;
   p.parts = parts;
   p.nst = std::min(C::kMaxStages, C::kRing / (C::kA + parts * C::kB));
-  p.steps = (int)((x.K + 63) / 64);
+  p.steps = (int)((x.K + 127) / 128);
   p.groups = (int)groups;
   const int64_t mt = (p.out + 127) / 128;
   p.mtiles = (int)(PAIR ? (mt + 1) / 2 : mt);
   p.tiles = p.mtiles * (int)((T + NT - 1) / NT);
   const int sms = device_sm_count();
   const int grid = PAIR ? 2 * std::min(p.tiles, sms / 2) : split > 1 ? p.tiles * split : std::min(p.tiles, sms);
-  return launch_cluster<mx4_linear_kernel<FMT, NT, PAIR, TR, CHUNK>>(grid, kThreads, C::kSmem, PAIR ? 2 : split, stream, mw,
+  return launch_cluster<mx4_linear_kernel<FMT, NT, PAIR, TR, CHUNK>>(grid, C::kThreads, C::kSmem, PAIR ? 2 : split, stream, mw,
                                                                     ms, mx, p, split);
 }
 
@@ -545,12 +534,12 @@ int launch_form(const XView& x, int parts, int64_t T, const Mx4View& w, float al
                 cudaStream_t stream) {
   const int sms = device_sm_count();
   const int64_t mt = ((TR ? w.n : w.rows) + 127) / 128;
-  const int stages = (int)((x.K + (TR ? 127 : 255)) / (TR ? 128 : 256));
+  const int steps = (int)((x.K + 127) / 128);
   const bool chunk = dtype == kMxF32;
   const int nt = chunk ? 64 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
   const int64_t tiles = mt * ((T + nt - 1) / nt), pairs = (mt + 1) / 2 * ((T + 255) / 256);
   int split = 1;
-  while (split < 8 && tiles * split * 2 <= sms && split * 2 <= stages) split *= 2;
+  while (split < 8 && tiles * split * 2 <= sms && split * 2 <= steps) split *= 2;
   if (chunk) return launch_tiles<FMT, 64, false, TR, true>(x, parts, T, w, alpha, dtype, y, split, stream);
   const double one = (double)((tiles + sms - 1) / sms) / split, pair = 1.6 * (double)((pairs + sms / 2 - 1) / (sms / 2));
   if (T > 128 && pair <= one) return launch_tiles<FMT, 256, true, TR, false>(x, parts, T, w, alpha, dtype, y, 1, stream);

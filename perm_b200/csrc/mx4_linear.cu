@@ -45,10 +45,13 @@ template <int FMT, int NT, bool PAIR, bool TR, bool CHUNK> struct Cfg {
   static constexpr int kAtoms = FMT == kMXFP4 ? 1 : 2;     // scale tiles of 128 x 128 codes
   static constexpr int kCodes = 128 * 64;
   static constexpr int kC = (kCodes + kAtoms * 512 + 1023) / 1024 * 1024;
-  static constexpr int kCS = 3, kMaxStages = 6;
+  // code stages: as many as the largest number of groups, so that one group sees every use of a stage
+  // (a group that saw every other use could take one phase of its barrier for another)
+  static constexpr int kCS = 2, kMaxStages = 6;
   static constexpr int kRing = (225 * 1024 - kCS * kC) / 1024 * 1024;   // stages of one decoded tile and its x tiles
   static constexpr size_t kSmem = 1024 + (size_t)kRing + kCS * kC + 512;
   static constexpr uint32_t kTmem = 2 * NT < 64 ? 64 : 2 * NT;
+  static_assert(kCS % kGroups == 0, "one group per code stage");
   static_assert(kB % 1024 == 0 && kRing >= NT * 512, "stages keep the swizzle's alignment, and a partial tile fits");
   // f32 accumulator, A and B bf16, A MN-major in the transposed form, N >> 3, M >> 4
   static constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((TR ? 1u : 0u) << 15) |

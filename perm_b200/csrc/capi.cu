@@ -707,7 +707,7 @@ int cp_mx4_dequantize(int fmt, const uint8_t* codes, const uint8_t* scales, int6
   if (((uintptr_t)codes | (uintptr_t)scales) & 15) return set_err(CP_ERR_ARG, "codes and scales must be 16-byte aligned");
   if ((uintptr_t)out % mx4_elem(dtype)) return set_err(CP_ERR_ARG, "out is misaligned");
   const cpk::Mx4View v{codes, scales, rows, n, fmt};
-  return check_rc(cpk::launch_mx4_dequantize(v, tensor_scale, dtype, out, (cudaStream_t)stream), "cp_mx4_dequantize");
+  return check_rc(cpk::launch_mx4_dequantize(v, tensor_scale, dtype, out, n, (cudaStream_t)stream), "cp_mx4_dequantize");
 }
 
 int cp_mx4_from_gguf(const uint8_t* raw, int64_t nrow, int64_t n, uint8_t* codes, uint8_t* scales, void* stream) {

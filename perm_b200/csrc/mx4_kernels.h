@@ -24,7 +24,8 @@ inline int64_t mx4_scale_bytes(int fmt, int64_t rows, int64_t n) {
 
 int launch_mx4_quantize(int fmt, int dtype, const void* x, int64_t rows, int64_t n, int64_t ld, const float* qw,
                         float inv_scale, uint8_t* codes, uint8_t* scales, cudaStream_t stream);
-int launch_mx4_dequantize(const Mx4View& v, float scale, int dtype, void* out, cudaStream_t stream);
+// out: rows ld elements apart.
+int launch_mx4_dequantize(const Mx4View& v, float scale, int dtype, void* out, int64_t ld, cudaStream_t stream);
 // GGUF MXFP4 container (17-byte blocks of 32): encode, decode, weighted error, and to the operand.
 int launch_mx4_encode(const float* x, int64_t nrow, int64_t n, const float* qw, uint8_t* out, cudaStream_t stream);
 int launch_mx4_decode(const uint8_t* raw, int64_t nrow, int64_t n, float* out, cudaStream_t stream);

@@ -24,6 +24,7 @@
 // accumulators alternate, so storing one tile overlaps the MMAs of the next.  float32 results restart the
 // accumulation every few steps and sum the chunks in round-to-nearest registers, because the tensor core's own
 // accumulation truncates.
+#include "mx4_dense.cuh"
 #include "mx4_product.cuh"
 
 namespace cpk {
@@ -70,30 +71,6 @@ struct LinParams {
   int groups;           // scale tiles per 128 rows of w
   int mtiles, tiles;
 };
-
-// A place in a ring of n stages and the parity of its current use.
-struct Ring {
-  int st;
-  uint32_t ph;
-  __device__ __forceinline__ void advance(int n) {
-    if (++st == n) st = 0, ph ^= 1;
-  }
-  __device__ __forceinline__ void back(int n) {
-    if (--st < 0) st += n, ph ^= 1;
-  }
-};
-
-template <bool PAIR>
-__device__ __forceinline__ void umma_bf16(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accum) {
-  if (PAIR)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-                 "l"(ad), "l"(bd), "r"(idesc), "r"(accum)
-                 : "memory");
-  else
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-                 "l"(ad), "l"(bd), "r"(idesc), "r"(accum)
-                 : "memory");
-}
 
 // bf16 (twice) of 2^112 times a block scale; `more` is a further factor, 1 unless the first would
 // overflow.
@@ -491,18 +468,6 @@ struct XView {
   int64_t rows, K, ld;
 };
 
-bool x_map(CUtensorMap* m, const XView& x, int box_rows) {
-  auto fn = encode_fn();
-  if (!fn) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)x.K, (cuuint64_t)x.rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)x.ld * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
-  const cuuint32_t estr[2] = {1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x.p), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int FMT, int NT, bool PAIR, bool TR, bool CHUNK>
 int launch_tiles(const XView& x, int parts, int64_t T, const Mx4View& w, float alpha, int dtype, void* y, int split,
                  cudaStream_t stream) {
@@ -510,7 +475,7 @@ int launch_tiles(const XView& x, int parts, int64_t T, const Mx4View& w, float a
   const int64_t pitch = mx4_pitch(w.n), groups = pitch / (FMT == kMXFP4 ? 64 : 32), wt = (w.rows + 127) / 128;
   CUtensorMap mw, ms, mx;
   if (!codes_map(&mw, w.codes, pitch, w.rows, 64, 128) || !scales_map(&ms, w.scales, wt * groups, C::kAtoms) ||
-      !x_map(&mx, x, C::kXRows))
+      !bf16_map(&mx, x.p, x.rows, x.K, x.ld, C::kXRows))
     return 5;
   LinParams p;
   p.y = y;
@@ -553,13 +518,48 @@ int launch_form(const XView& x, int parts, int64_t T, const Mx4View& w, float al
   }
 }
 
+// Whether the weights are decoded to the workspace first.  Measured, MXFP4, bf16, decoded first / in the
+// product: 4096 -> 4096 with 512 tokens 32 / 27 us, 1024 tokens 33 / 43, 4096 tokens 96 / 148;
+// 4096 -> 14336 with 256 tokens 57 / 43, 512 tokens 78 / 77, 4096 tokens 420 / 476.
+bool use_dense(int64_t T) { return T > 640; }
+
+int launch_dense(const XView& x, int parts, int64_t T, const Mx4View& w, float alpha, int dtype, int transpose, void* y,
+                 void* wbuf, cudaStream_t stream) {
+  const int64_t ld = (w.n + 7) / 8 * 8;
+  if (int rc = launch_mx4_dequantize(w, 1.0f, kMxBF16, wbuf, ld, stream)) return rc;
+  CUtensorMap mw, mx;
+  if (!bf16_map(&mw, wbuf, w.rows, w.n, ld, transpose ? 64 : 128) || !bf16_map(&mx, x.p, x.rows, x.K, x.ld, 128)) return 5;
+  dense::Params p;
+  p.y = y;
+  if (cudaGetSymbolAddress((void**)&p.status, g_status) != cudaSuccess) return 6;
+  p.T = T;
+  p.out = transpose ? w.n : w.rows;
+  p.alpha = alpha;
+  p.dtype = dtype;
+  p.parts = parts;
+  p.nst = dense::kRing / ((1 + parts) * dense::kBox);
+  p.steps = (int)((x.K + 63) / 64);
+  p.chunk = dtype == kMxF32 ? 3 : p.steps;
+  p.mtiles = (int)((p.out + 255) / 256);
+  p.tiles = p.mtiles * (int)((T + 255) / 256);
+  const int grid = 2 * std::min(p.tiles, device_sm_count() / 2);
+  return transpose ? launch_cluster<dense::dense_kernel<true>>(grid, dense::kThreads, dense::kSmem, 2, stream, mw, mx, p)
+                   : launch_cluster<dense::dense_kernel<false>>(grid, dense::kThreads, dense::kSmem, 2, stream, mw, mx, p);
+}
+
 int64_t parts_pitch(int64_t K) { return (K + 7) / 8 * 8; }
 
 }  // namespace
 
+namespace {
+size_t parts_bytes(int dtype, int64_t T, int64_t K, int aligned) {
+  return dtype == kMxBF16 && aligned ? 0 : ((size_t)parts_of(dtype) * T * parts_pitch(K) * 2 + 255) / 256 * 256;
+}
+}  // namespace
+
 size_t mx4_linear_workspace_bytes(int dtype, int64_t T, int64_t rows, int64_t n, int aligned, int transpose) {
-  if (dtype == kMxBF16 && aligned) return 0;
-  return (size_t)parts_of(dtype) * T * parts_pitch(transpose ? rows : n) * 2;
+  return parts_bytes(dtype, T, transpose ? rows : n, aligned) +
+         (use_dense(T) ? (size_t)rows * ((n + 7) / 8 * 8) * 2 : 0);
 }
 
 int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, int aligned, const Mx4View& w, float alpha,
@@ -568,7 +568,8 @@ int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, int align
   const int64_t K = transpose ? w.rows : w.n;
   const int parts = parts_of(dtype);
   XView xv{x, T, K, T == 1 ? parts_pitch(K) : ld};   // one row has no pitch of its own
-  if (mx4_linear_workspace_bytes(dtype, T, w.rows, w.n, aligned, transpose) > 0) {
+  const size_t pb = parts_bytes(dtype, T, K, aligned);
+  if (pb > 0) {
     const int64_t Kp = parts_pitch(K);
     const unsigned grid = (unsigned)std::min<int64_t>((T * (Kp / 8) + 255) / 256, (int64_t)device_sm_count() * 8);
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(ws);
@@ -578,6 +579,8 @@ int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, int align
     note_launch();
     xv = XView{ws, parts * T, K, Kp};
   }
+  if (use_dense(T))
+    return launch_dense(xv, parts, T, w, alpha, dtype, transpose, y, static_cast<uint8_t*>(ws) + pb, stream);
   if (w.fmt == kMXFP4)
     return transpose ? launch_form<kMXFP4, true>(xv, parts, T, w, alpha, dtype, y, stream)
                      : launch_form<kMXFP4, false>(xv, parts, T, w, alpha, dtype, y, stream);

@@ -63,6 +63,30 @@ __device__ __forceinline__ void fail_cta(volatile int* abort, int* status) {
   atomicOr(status, 1);
 }
 
+// A place in a ring of n stages and the parity of its current use.
+struct Ring {
+  int st;
+  uint32_t ph;
+  __device__ __forceinline__ void advance(int n) {
+    if (++st == n) st = 0, ph ^= 1;
+  }
+  __device__ __forceinline__ void back(int n) {
+    if (--st < 0) st += n, ph ^= 1;
+  }
+};
+
+template <bool PAIR>
+__device__ __forceinline__ void umma_bf16(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accum) {
+  if (PAIR)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(ad), "l"(bd), "r"(idesc), "r"(accum)
+                 : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(ad), "l"(bd), "r"(idesc), "r"(accum)
+                 : "memory");
+}
+
 // Sums the cluster's partial tiles ([token][128 rows] float32 at the same place of every CTA's
 // shared memory) in rank order; this CTA takes its share of the tokens.
 __device__ __forceinline__ void join_partials(const void* part, int rank, int split, int cols, int64_t row0, int64_t t0,
@@ -120,6 +144,19 @@ inline bool scales_map(CUtensorMap* m, const uint8_t* p, int64_t tiles, int box)
   const cuuint32_t estr[2] = {1, 1};
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<uint8_t*>(p), dims, strides, boxes, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Tensor map of bf16 rows, boxes of 64 columns (128-byte swizzle).
+inline bool bf16_map(CUtensorMap* m, const void* p, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

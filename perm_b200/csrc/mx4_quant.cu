@@ -183,7 +183,7 @@ __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v
 template <typename T, int FMT>
 __global__ void __launch_bounds__(32 * kWarps)
     dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows, int64_t n,
-                      float scale, int chunks, int64_t units, bool vec, T* __restrict__ out) {
+                      float scale, int chunks, int64_t units, bool vec, T* __restrict__ out, int64_t ld) {
   const int64_t unit = blockIdx.x * (int64_t)kWarps + threadIdx.x / 32;
   if (unit >= units) return;
   const int lane = threadIdx.x % 32;
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(32 * kWarps)
       put(o + 2 * i, __fmul_rn(__fmul_rn(q.x, s), scale));
       put(o + 2 * i + 1, __fmul_rn(__fmul_rn(q.y, s), scale));
     }
-    T* p = out + row * n + col;
+    T* p = out + row * ld + col;
     if (vec && left >= 8) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(o)[i];
@@ -394,15 +394,15 @@ int quantize_typed(int fmt, const T* x, int64_t rows, int64_t n, int64_t ld, con
   return 0;
 }
 
-template <typename T> int dequantize_typed(const Mx4View& v, float scale, T* out, cudaStream_t stream) {
+template <typename T> int dequantize_typed(const Mx4View& v, float scale, T* out, int64_t ld, cudaStream_t stream) {
   const int chunks = (int)((v.n + 255) / 256);
   const int64_t units = row_lanes(v.rows) * chunks;
   const unsigned grid = (unsigned)((units + kWarps - 1) / kWarps);
-  const bool vec = ((uintptr_t)out & 15) == 0 && (v.n * sizeof(T)) % 16 == 0;
+  const bool vec = ((uintptr_t)out & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
   if (v.fmt == kMXFP4)
-    dequantize_kernel<T, kMXFP4><<<grid, 32 * kWarps, 0, stream>>>(v.codes, v.scales, v.rows, v.n, scale, chunks, units, vec, out);
+    dequantize_kernel<T, kMXFP4><<<grid, 32 * kWarps, 0, stream>>>(v.codes, v.scales, v.rows, v.n, scale, chunks, units, vec, out, ld);
   else
-    dequantize_kernel<T, kNVFP4><<<grid, 32 * kWarps, 0, stream>>>(v.codes, v.scales, v.rows, v.n, scale, chunks, units, vec, out);
+    dequantize_kernel<T, kNVFP4><<<grid, 32 * kWarps, 0, stream>>>(v.codes, v.scales, v.rows, v.n, scale, chunks, units, vec, out, ld);
   note_launch();
   return 0;
 }
@@ -419,11 +419,11 @@ int launch_mx4_quantize(int fmt, int dtype, const void* x, int64_t rows, int64_t
   return quantize_typed(fmt, static_cast<const float*>(x), rows, n, ld, qw, inv_scale, codes, scales, stream);
 }
 
-int launch_mx4_dequantize(const Mx4View& v, float scale, int dtype, void* out, cudaStream_t stream) {
+int launch_mx4_dequantize(const Mx4View& v, float scale, int dtype, void* out, int64_t ld, cudaStream_t stream) {
   if (v.rows == 0) return 0;
-  if (dtype == kMxBF16) return dequantize_typed(v, scale, static_cast<__nv_bfloat16*>(out), stream);
-  if (dtype == kMxF16) return dequantize_typed(v, scale, static_cast<__half*>(out), stream);
-  return dequantize_typed(v, scale, static_cast<float*>(out), stream);
+  if (dtype == kMxBF16) return dequantize_typed(v, scale, static_cast<__nv_bfloat16*>(out), ld, stream);
+  if (dtype == kMxF16) return dequantize_typed(v, scale, static_cast<__half*>(out), ld, stream);
+  return dequantize_typed(v, scale, static_cast<float*>(out), ld, stream);
 }
 
 int launch_mx4_encode(const float* x, int64_t nrow, int64_t n, const float* qw, uint8_t* out, cudaStream_t stream) {

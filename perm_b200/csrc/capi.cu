@@ -775,10 +775,11 @@ int cp_mx4_linear(int fmt, int dtype, const void* x, int64_t T, int64_t ld, cons
 }
 
 int cp_mx4_status(void* stream) {
-  int st = 0, st2 = 0;
-  if (cpk::mx4_matmul_status((cudaStream_t)stream, &st) != 0 || cpk::mx4_linear_status((cudaStream_t)stream, &st2) != 0)
+  int st[3] = {0, 0, 0};
+  if (cpk::mx4_matmul_status((cudaStream_t)stream, &st[0]) != 0 || cpk::mx4_linear_status((cudaStream_t)stream, &st[1]) != 0 ||
+      cpk::mx4_stream_status((cudaStream_t)stream, &st[2]) != 0)
     return check_launch("cp_mx4_status");
-  if (st == 0 && st2 == 0) return CP_OK;
+  if (!st[0] && !st[1] && !st[2]) return CP_OK;
   return set_err(CP_ERR_TIMEOUT, "a bounded wait in a 4-bit product ran out; its result is incomplete");
 }
 

@@ -558,6 +558,7 @@ size_t parts_bytes(int dtype, int64_t T, int64_t K, int aligned) {
 }  // namespace
 
 size_t mx4_linear_workspace_bytes(int dtype, int64_t T, int64_t rows, int64_t n, int aligned, int transpose) {
+  if (!transpose && mx4_stream_applies(dtype, T, rows, n)) return 0;
   return parts_bytes(dtype, T, transpose ? rows : n, aligned) +
          (use_dense(T) ? (size_t)rows * ((n + 7) / 8 * 8) * 2 : 0);
 }
@@ -565,6 +566,8 @@ size_t mx4_linear_workspace_bytes(int dtype, int64_t T, int64_t rows, int64_t n,
 int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, int aligned, const Mx4View& w, float alpha,
                       int transpose, void* y, void* ws, cudaStream_t stream) {
   if (!bind_context()) return 6;
+  if (!transpose && mx4_stream_applies(dtype, T, w.rows, w.n))
+    return launch_mx4_stream(dtype, x, T, ld, aligned, w, alpha, y, stream);
   const int64_t K = transpose ? w.rows : w.n;
   const int parts = parts_of(dtype);
   XView xv{x, T, K, T == 1 ? parts_pitch(K) : ld};   // one row has no pitch of its own

@@ -1,0 +1,448 @@
+// y = alpha * x w^T for a few tokens: the weights stream once from HBM, 17/32 or 9/16 of a byte each,
+// and everything else has to keep up with that.
+//
+// At 6.5 TB/s an SM gets about 44 weights a clock and issues 128 lane instructions, so a weight has
+// less than three.  Decoding to bf16 (five instructions for two weights) and storing the tile for
+// tcgen05 does not fit; here the weights go straight into registers as f16, one conversion for
+// two, and through mma.sync m16n8k16 with 16 rows of weights as the A operand and up to 8 tokens as B (more
+// tokens: more B tiles).  ldmatrix hands lane (g, t) the word of eight codes 8t .. 8t + 7 of a 32-code
+// block of row g; which k of the MMA a code sits on is free as long as x is taken in the same order, and
+// with that order the eight values of x that a lane needs are 16 neighbouring bytes.
+//
+//   MXFP4  The two MMAs of a block start from zero; their sums are multiplied by the block's power of two
+//          and added in float32, exact for every scale.
+//   NVFP4  A lane's codes lie in one block of 16; code times scale has six significant bits and fits f16,
+//          so the A registers are multiplied before the MMA, which then accumulates 256 columns.
+//
+// Activations are f16 too.  float16 is taken as it is.  bf16 and float32 rows are multiplied by a power of
+// two that brings the row's largest magnitude (of this CTA's columns) to [2^14, 2^15): a bf16 value is then
+// exact unless it is below 2^-32 of the largest, and off by at most 2^-40 of the largest otherwise.
+// float32 values are the sum of two f16 parts, the second 2^11 times finer, to within 2^-23 of each value.
+//
+// A CTA holds 128 rows (16 for each of eight warps) and a slice of the columns; a cluster of up to eight
+// shares a row tile and joins the partial sums through distributed shared memory in rank order.  Codes
+// and scale tiles arrive by TMA in stages of 256 columns; x is converted into shared memory while the first
+// stages are in flight.  Two CTAs fit an SM for up to 16 tokens.
+#include "mx4_product.cuh"
+
+namespace cpk {
+namespace {
+
+__device__ int g_status;
+
+constexpr unsigned long long kWaitNs = 1000000000ull;
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * (kWarps + 1);   // the last warp loads
+constexpr int kMaxStages = 6;
+
+struct StreamParams {
+  const void* x;
+  void* y;
+  int64_t T, K, ld, rows;
+  float alpha;
+  int dtype;
+  int steps, nst;       // 256-column steps; stages of the ring
+  int slice;            // columns of the widest slice (the pitch of the converted x)
+  int groups;           // scale tiles per 128 rows
+  int vec;              // x's rows start on 16-byte boundaries
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+// Eight codes -> four f16 pairs.
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t (&v)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+      : "r"(w));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Two e8m0 scales (low half of w) -> float32.
+__device__ __forceinline__ void e8m0x2(uint32_t w, float& lo, float& hi) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 s;\n\tcvt.u16.u32 s, %1;\n\tcvt.rn.bf16x2.ue8m0x2 %0, s;\n\t}" : "=r"(r) : "r"(w));
+  lo = __uint_as_float(r << 16);
+  hi = __uint_as_float(r & 0xFFFF0000u);
+}
+// Two e4m3 scales (low half of w, signs cleared) -> f16.
+__device__ __forceinline__ uint32_t e4m3x2(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 s;\n\tcvt.u16.u32 s, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, s;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+
+__device__ __forceinline__ float as_f32(float v) { return v; }
+__device__ __forceinline__ float as_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float as_f32(__half v) { return __half2float(v); }
+
+template <typename S> struct Parts { static constexpr int k = 1; static constexpr bool scaled = true; };
+template <> struct Parts<__half> { static constexpr int k = 1; static constexpr bool scaled = false; };
+template <> struct Parts<float> { static constexpr int k = 2; static constexpr bool scaled = true; };
+
+// Eight values of a row of x from column k on (zero past K).
+template <typename S>
+__device__ __forceinline__ void load_x8(const StreamParams& p, int t, int64_t k, float (&v)[8]) {
+  const S* src = static_cast<const S*>(p.x) + t * p.ld + k;
+  if (p.vec && k + 8 <= p.K) {
+    constexpr int W = sizeof(S) / 2;
+    uint4 w[W];
+#pragma unroll
+    for (int i = 0; i < W; i++) w[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+    const S* e = reinterpret_cast<const S*>(w);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = as_f32(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = k + i < p.K ? as_f32(src[i]) : 0.0f;
+  }
+}
+
+template <int FMT, int NB, typename S>
+__global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1)
+    mx4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
+                      const StreamParams prm, int split) {
+  constexpr int NTOK = 8 * NB, P = Parts<S>::k;
+  constexpr bool kScaled = Parts<S>::scaled;
+  constexpr int kAtoms = FMT == kMXFP4 ? 2 : 4;          // scale tiles of 128 rows x 256 columns
+  constexpr int kStage = 128 * 128 + kAtoms * 512;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int nst = prm.nst;
+  const int xpitch = prm.slice * 2 + 64;                 // bytes; 64 past a multiple of 512: no bank conflicts
+  uint8_t* xs = base + nst * kStage;                     // [part][token][column] f16
+  uint32_t* top = reinterpret_cast<uint32_t*>(xs + P * NTOK * xpitch);   // largest magnitudes, as bits
+  uint64_t* bars = reinterpret_cast<uint64_t*>(top + NTOK);
+  volatile int* misc = reinterpret_cast<volatile int*>(bars + 2 * kMaxStages);   // [0] abort
+  const uint32_t ring = smem_u32(base), full0 = smem_u32(bars), empty0 = full0 + 8 * kMaxStages;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = split > 1 ? (int)cluster_rank() : 0;
+  const int tile = (int)blockIdx.x / split;
+  const int s_begin = (int)((int64_t)prm.steps * rank / split), s_end = (int)((int64_t)prm.steps * (rank + 1) / split);
+  const int T = (int)prm.T;
+  volatile int* abort = &misc[0];
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < nst; s++) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, kWarps);
+    }
+    misc[0] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x < NTOK) top[threadIdx.x] = 0;
+  __syncthreads();
+
+  float acc[NB][4];
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[b][e] = 0.0f;
+
+  if (warp == kWarps) {
+    if (lane == 0) {
+      Ring rg{0, 0};
+      bool ok = true;
+      int loads = 0;
+      for (int s = s_begin; s < s_end; s++, loads++) {
+        if (loads >= nst && !mbar_wait(empty0 + 8 * rg.st, rg.ph ^ 1, abort, kWaitNs)) {
+          ok = false;
+          break;
+        }
+        const uint32_t fb = full0 + 8 * rg.st, sw = ring + rg.st * kStage;
+        mbar_expect_tx(fb, kStage);
+        tma_load(sw, &map_w, s * 128, tile * 128, fb);
+        tma_load(sw + 128 * 128, &map_s, 0, tile * prm.groups + s * kAtoms, fb);
+        rg.advance(nst);
+      }
+      if (!ok) fail_cta(abort, &g_status);
+      for (int k = min(loads, nst); k > 0; k--) {   // every load issued lands before the CTA goes on
+        rg.back(nst);
+        int zero = 0;
+        mbar_wait(full0 + 8 * rg.st, rg.ph, &zero, kWaitNs);
+      }
+    }
+  } else {
+    // ---- x into shared memory
+    const int per = (s_end - s_begin) * 32;   // groups of eight columns
+    const int64_t k0 = (int64_t)s_begin * 256;
+    if (kScaled) {
+      for (int i = threadIdx.x; i < T * per; i += 32 * kWarps) {
+        float v[8];
+        load_x8<S>(prm, i / per, k0 + (int64_t)(i % per) * 8, v);
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const uint32_t b = __float_as_uint(v[e]) & 0x7FFFFFFFu;
+          m = max(m, b < 0x7F800000u ? b : 0u);
+        }
+        m = __reduce_max_sync(0xffffffffu, m);   // per is a multiple of 32: a warp holds one row
+        if (lane == 0) atomicMax(&top[i / per], m);
+      }
+      asm volatile("bar.sync 1, %0;" ::"r"(32 * kWarps) : "memory");
+    }
+    for (int i = threadIdx.x; i < NTOK * per; i += 32 * kWarps) {
+      const int t = i / per, c = i % per;
+      uint32_t w[P][4];
+      if (t < T) {
+        float v[8];
+        load_x8<S>(prm, t, k0 + (int64_t)c * 8, v);
+        float up = 1.0f;
+        if (kScaled) {   // 2^(14 - e) for a largest magnitude of exponent e
+          const int e = max((int)(top[t] >> 23), 1);
+          up = __uint_as_float((uint32_t)min(268 - e, 247) << 23);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float a = kScaled ? v[e] * up : v[e], b = kScaled ? v[e + 1] * up : v[e + 1];
+          const __half2 h = __floats2half2_rn(a, b);
+          w[0][e / 2] = *reinterpret_cast<const uint32_t*>(&h);
+          if (P == 2) {
+            const float2 f = __half22float2(h);
+            const float ra = fabsf(a) < 1e30f ? (a - f.x) * 2048.0f : 0.0f, rb = fabsf(b) < 1e30f ? (b - f.y) * 2048.0f : 0.0f;
+            const __half2 l = __floats2half2_rn(ra, rb);
+            w[P - 1][e / 2] = *reinterpret_cast<const uint32_t*>(&l);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) w[p][e] = 0;
+      }
+#pragma unroll
+      for (int p = 0; p < P; p++)
+        *reinterpret_cast<uint4*>(xs + (p * NTOK + t) * xpitch + c * 16) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+    }
+    asm volatile("bar.sync 1, %0;" ::"r"(32 * kWarps) : "memory");
+
+    // ---- the weights
+    const int g = lane >> 2, t4 = lane & 3;
+    float down[NB][2];   // undoes `up` for this lane's two tokens of each tile
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+        down[b][e] = kScaled ? __uint_as_float((uint32_t)max(max((int)(top[8 * b + 2 * t4 + e] >> 23), 1) - 14, 7) << 23) : 1.0f;
+    const uint32_t row_at = (16 * warp + (lane & 7)) * 128, x7 = lane & 7;
+    const uint32_t srow = ((16 * warp + g) & 31) * 16 + ((16 * warp + g) >> 5) * 4;   // row g's scale word; row g + 8: + 128
+    const uint32_t xlane = smem_u32(xs) + g * xpitch + t4 * 16;
+    Ring rg{0, 0};
+    bool ok = true;
+    for (int s = s_begin; s < s_end; s++) {
+      if (!mbar_wait_warp(full0 + 8 * rg.st, rg.ph, abort, kWaitNs)) {
+        ok = false;
+        break;
+      }
+      const uint32_t sw = ring + rg.st * kStage;
+      const uint8_t* sc = base + rg.st * kStage + 128 * 128;
+      const uint32_t xcol = xlane + (s - s_begin) * 512;
+      float c[P][NB][4];
+      if (FMT == kNVFP4) {
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+          for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) c[p][b][e] = 0.0f;
+      }
+#pragma unroll
+      for (int half = 0; half < 2; half++) {   // 128 columns
+        uint32_t wa[4], wb[4];
+        const uint32_t at = sw + row_at + (((half * 4 + (lane >> 3)) ^ x7) << 4);
+        ldmatrix4(at, wa);               // rows g: words of four blocks of 32
+        ldmatrix4(at + 8 * 128, wb);     // rows g + 8
+        float sa[4], sb[4];
+        uint32_t ha[4], hb[4];
+        if (FMT == kMXFP4) {
+          const uint32_t va = *reinterpret_cast<const uint32_t*>(sc + half * 512 + srow);
+          const uint32_t vb = *reinterpret_cast<const uint32_t*>(sc + half * 512 + srow + 128);
+          e8m0x2(va, sa[0], sa[1]);
+          e8m0x2(va >> 16, sa[2], sa[3]);
+          e8m0x2(vb, sb[0], sb[1]);
+          e8m0x2(vb >> 16, sb[2], sb[3]);
+        } else {
+          const uint32_t sel = t4 < 2 ? 0x1010u : 0x3232u;   // this lane's block of a pair
+#pragma unroll
+          for (int j = 0; j < 4; j += 2) {
+            const uint32_t va = *reinterpret_cast<const uint32_t*>(sc + (half * 2 + j / 2) * 512 + srow) & 0x7F7F7F7Fu;
+            const uint32_t vb = *reinterpret_cast<const uint32_t*>(sc + (half * 2 + j / 2) * 512 + srow + 128) & 0x7F7F7F7Fu;
+            ha[j] = __byte_perm(e4m3x2(va), 0, sel);
+            ha[j + 1] = __byte_perm(e4m3x2(va >> 16), 0, sel);
+            hb[j] = __byte_perm(e4m3x2(vb), 0, sel);
+            hb[j + 1] = __byte_perm(e4m3x2(vb >> 16), 0, sel);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          uint32_t a[4], b[4];
+          codes_f16(wa[j], a);
+          codes_f16(wb[j], b);
+          if (FMT == kNVFP4) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) a[i] = mul_f16x2(a[i], ha[j]), b[i] = mul_f16x2(b[i], hb[j]);
+          }
+#pragma unroll
+          for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+              uint4 xv;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(xv.x), "=r"(xv.y), "=r"(xv.z), "=r"(xv.w)
+                           : "r"(xcol + (p * NTOK + nb * 8) * xpitch + half * 256 + j * 64));
+              float(&d)[4] = c[p][nb];
+              if (FMT == kMXFP4) d[0] = d[1] = d[2] = d[3] = 0.0f;
+              mma_f16(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
+              mma_f16(d, a[2], b[2], a[3], b[3], xv.z, xv.w);
+              if (FMT == kMXFP4) {
+                const float fine = p == 1 ? 1.0f / 2048.0f : 1.0f;
+                const float d0 = kScaled ? d[0] * (down[nb][0] * fine) : d[0], d1 = kScaled ? d[1] * (down[nb][1] * fine) : d[1];
+                const float d2 = kScaled ? d[2] * (down[nb][0] * fine) : d[2], d3 = kScaled ? d[3] * (down[nb][1] * fine) : d[3];
+                acc[nb][0] += d0 * sa[j];
+                acc[nb][1] += d1 * sa[j];
+                acc[nb][2] += d2 * sb[j];
+                acc[nb][3] += d3 * sb[j];
+              }
+            }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty0 + 8 * rg.st);
+      rg.advance(nst);
+      if (FMT == kNVFP4) {
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+          for (int p = 0; p < P; p++) {
+            const float fine = p == 1 ? 1.0f / 2048.0f : 1.0f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[nb][e] += c[p][nb][e] * (down[nb][e & 1] * fine);
+          }
+      }
+    }
+    if (!ok) fail_cta(abort, &g_status);
+  }
+  // ---- results: lane (g, t) has rows g, g + 8 of its warp's 16 and tokens 2t, 2t + 1 of each tile
+  const int64_t row0 = (int64_t)tile * 128;
+  if (split > 1) {
+    __syncthreads();   // all loads have landed and been read: the ring is free
+    float* part = reinterpret_cast<float*>(base);
+    if (warp < kWarps) {
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          part[(8 * nb + 2 * (lane & 3) + (e & 1)) * 128 + 16 * warp + (lane >> 2) + (e >> 1) * 8] = acc[nb][e];
+    }
+    cluster_sync();
+    join_partials(base, rank, split, T, row0, 0, prm.rows, prm.alpha, prm.dtype, prm.y);
+    cluster_sync();
+  } else if (warp < kWarps) {
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int t = 8 * nb + 2 * (lane & 3) + (e & 1);
+        const int64_t row = row0 + 16 * warp + (lane >> 2) + (e >> 1) * 8;
+        if (t < T && row < prm.rows) put_out(prm.y, prm.dtype, t * prm.rows + row, prm.alpha * acc[nb][e]);
+      }
+  }
+}
+
+template <int FMT, int NB, typename S>
+int launch_stream(StreamParams& p, const Mx4View& w, int split, cudaStream_t stream) {
+  constexpr int kAtoms = FMT == kMXFP4 ? 2 : 4, kStage = 128 * 128 + kAtoms * 512;
+  const int64_t pitch = mx4_pitch(w.n), wt = (w.rows + 127) / 128;
+  CUtensorMap mw, ms;
+  if (!codes_map(&mw, w.codes, pitch, w.rows, 128, 128) || !scales_map(&ms, w.scales, wt * p.groups, kAtoms)) return 5;
+  const size_t smem = 1024 + (size_t)p.nst * kStage + (size_t)Parts<S>::k * 8 * NB * (p.slice * 2 + 64) + 8 * NB * 4 +
+                      16 * kMaxStages + 64;
+  return launch_cluster<mx4_stream_kernel<FMT, NB, S>>((int)wt * split, kThreads, smem, split, stream, mw, ms, p, split);
+}
+
+template <int FMT, typename S>
+int launch_tokens(StreamParams& p, const Mx4View& w, int split, cudaStream_t stream) {
+  if (p.T <= 8) return launch_stream<FMT, 1, S>(p, w, split, stream);
+  if (p.T <= 16) return launch_stream<FMT, 2, S>(p, w, split, stream);
+  return launch_stream<FMT, 4, S>(p, w, split, stream);
+}
+
+}  // namespace
+
+namespace {
+struct StreamPlan {
+  int split, nst, slice;
+};
+// False where x's slices would not leave room in shared memory.
+bool stream_plan(int dtype, int64_t T, int64_t rows, int64_t n, StreamPlan* plan) {
+  if (T > 32) return false;
+  const int parts = dtype == kMxF32 ? 2 : 1, nb = T <= 8 ? 1 : T <= 16 ? 2 : 4;
+  const int64_t wt = (rows + 127) / 128, slots = (int64_t)device_sm_count() * (nb <= 2 ? 2 : 1);
+  const int steps = (int)(mx4_pitch(n) / 128), stage = 128 * 128 + 4 * 512;   // NVFP4's; MXFP4's is smaller
+  int split = 1;
+  while (split < 8 && wt * split * 2 <= slots && split * 2 <= steps) split *= 2;
+  // x's slice stays in shared memory beside at least three stages
+  auto x_bytes = [&](int sp) { return (int64_t)parts * 8 * nb * ((int64_t)(steps + sp - 1) / sp * 512 + 64); };
+  const int64_t room = 222 * 1024;
+  while (split < 8 && split * 2 <= steps && x_bytes(split) + 3 * stage > room) split *= 2;
+  if (x_bytes(split) + 3 * stage > room) return false;
+  // two CTAs to an SM where that leaves each three stages
+  const int64_t half = room / 2 - 1024 - x_bytes(split);
+  const int mine = (steps + split - 1) / split;
+  const int nst = (int)((nb <= 2 && half >= 3 * stage ? half : room - x_bytes(split)) / stage);
+  *plan = StreamPlan{split, std::min(std::min(nst, kMaxStages), mine), mine * 256};
+  return true;
+}
+}  // namespace
+
+bool mx4_stream_applies(int dtype, int64_t T, int64_t rows, int64_t n) {
+  StreamPlan plan;
+  return stream_plan(dtype, T, rows, n, &plan);
+}
+
+int launch_mx4_stream(int dtype, const void* x, int64_t T, int64_t ld, int aligned, const Mx4View& w, float alpha, void* y,
+                      cudaStream_t stream) {
+  StreamPlan plan;
+  if (!stream_plan(dtype, T, w.rows, w.n, &plan)) return 6;
+  const int steps = (int)(mx4_pitch(w.n) / 128), split = plan.split;
+  StreamParams p;
+  p.x = x;
+  p.y = y;
+  p.T = T;
+  p.K = w.n;
+  p.ld = ld;
+  p.rows = w.rows;
+  p.alpha = alpha;
+  p.dtype = dtype;
+  p.steps = steps;
+  p.nst = plan.nst;
+  p.slice = plan.slice;
+  p.groups = steps * (w.fmt == kMXFP4 ? 2 : 4);
+  p.vec = aligned;
+  if (w.fmt == kMXFP4) {
+    if (dtype == kMxBF16) return launch_tokens<kMXFP4, __nv_bfloat16>(p, w, split, stream);
+    if (dtype == kMxF16) return launch_tokens<kMXFP4, __half>(p, w, split, stream);
+    return launch_tokens<kMXFP4, float>(p, w, split, stream);
+  }
+  if (dtype == kMxBF16) return launch_tokens<kNVFP4, __nv_bfloat16>(p, w, split, stream);
+  if (dtype == kMxF16) return launch_tokens<kNVFP4, __half>(p, w, split, stream);
+  return launch_tokens<kNVFP4, float>(p, w, split, stream);
+}
+
+int mx4_stream_status(cudaStream_t stream, int* status) { return read_status_word(g_status, stream, status); }
+
+}  // namespace cpk

@@ -67,6 +67,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -94,22 +100,15 @@ template <typename S> struct Parts { static constexpr int k = 1; static constexp
 template <> struct Parts<__half> { static constexpr int k = 1; static constexpr bool scaled = false; };
 template <> struct Parts<float> { static constexpr int k = 2; static constexpr bool scaled = true; };
 
-// Eight values of a row of x from column k on (zero past K).
-template <typename S>
-__device__ __forceinline__ void load_x8(const StreamParams& p, int t, int64_t k, float (&v)[8]) {
-  const S* src = static_cast<const S*>(p.x) + t * p.ld + k;
-  if (p.vec && k + 8 <= p.K) {
-    constexpr int W = sizeof(S) / 2;
-    uint4 w[W];
+// Eight values of x in shared memory.
+template <typename S> __device__ __forceinline__ void read_x8(const uint8_t* at, float (&v)[8]) {
+  constexpr int W = sizeof(S) / 2;
+  uint4 w[W];
 #pragma unroll
-    for (int i = 0; i < W; i++) w[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
-    const S* e = reinterpret_cast<const S*>(w);
+  for (int i = 0; i < W; i++) w[i] = reinterpret_cast<const uint4*>(at)[i];
+  const S* e = reinterpret_cast<const S*>(w);
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = as_f32(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = k + i < p.K ? as_f32(src[i]) : 0.0f;
-  }
+  for (int i = 0; i < 8; i++) v[i] = as_f32(e[i]);
 }
 
 template <int FMT, int NB, typename S>
@@ -123,9 +122,11 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int nst = prm.nst;
-  const int xpitch = prm.slice * 2 + 64;                 // bytes; 64 past a multiple of 512: no bank conflicts
-  uint8_t* xs = base + nst * kStage;                     // [part][token][column] f16
-  uint32_t* top = reinterpret_cast<uint32_t*>(xs + P * NTOK * xpitch);   // largest magnitudes, as bits
+  // bytes of a token's slice; the odd end keeps eight lanes' 16-byte reads (two tokens, four groups) on
+  // different banks
+  const int xpitch = prm.slice * 2 * P + (P == 1 ? 64 : 16);
+  uint8_t* xs = base + nst * kStage;                     // [token][eight columns][part] f16
+  uint32_t* top = reinterpret_cast<uint32_t*>(xs + NTOK * xpitch);   // largest magnitudes, as bits
   uint64_t* bars = reinterpret_cast<uint64_t*>(top + NTOK);
   volatile int* misc = reinterpret_cast<volatile int*>(bars + 2 * kMaxStages);   // [0] abort
   const uint32_t ring = smem_u32(base), full0 = smem_u32(bars), empty0 = full0 + 8 * kMaxStages;
@@ -177,56 +178,71 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1)
       }
     }
   } else {
-    // ---- x into shared memory
-    const int per = (s_end - s_begin) * 32;   // groups of eight columns
+    // ---- x into shared memory: asynchronous copies of the rows as they are, then (scaled types) a pass
+    // for the largest magnitudes and one that converts each group of eight values in place
+    const int per = (s_end - s_begin) * 32;   // groups of eight columns: a multiple of 32, so a warp holds one row
     const int64_t k0 = (int64_t)s_begin * 256;
-    if (kScaled) {
-      for (int i = threadIdx.x; i < T * per; i += 32 * kWarps) {
-        float v[8];
-        load_x8<S>(prm, i / per, k0 + (int64_t)(i % per) * 8, v);
-        uint32_t m = 0;
+    const S* x = static_cast<const S*>(prm.x) + k0;
+    for (int t = 0; t < NTOK; t++)
+      for (int c = threadIdx.x; c < per; c += 32 * kWarps) {
+        uint8_t* dst = xs + t * xpitch + c * (16 * P);
+        const int64_t left = t < T ? prm.K - k0 - (int64_t)c * 8 : 0;   // values of the row from here on
+        const S* src = x + t * prm.ld + c * 8;
+        if (prm.vec || left <= 0) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const uint32_t b = __float_as_uint(v[e]) & 0x7FFFFFFFu;
-          m = max(m, b < 0x7F800000u ? b : 0u);
-        }
-        m = __reduce_max_sync(0xffffffffu, m);   // per is a multiple of 32: a warp holds one row
-        if (lane == 0) atomicMax(&top[i / per], m);
-      }
-      asm volatile("bar.sync 1, %0;" ::"r"(32 * kWarps) : "memory");
-    }
-    for (int i = threadIdx.x; i < NTOK * per; i += 32 * kWarps) {
-      const int t = i / per, c = i % per;
-      uint32_t w[P][4];
-      if (t < T) {
-        float v[8];
-        load_x8<S>(prm, t, k0 + (int64_t)c * 8, v);
-        float up = 1.0f;
-        if (kScaled) {   // 2^(14 - e) for a largest magnitude of exponent e
-          const int e = max((int)(top[t] >> 23), 1);
-          up = __uint_as_float((uint32_t)min(268 - e, 247) << 23);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float a = kScaled ? v[e] * up : v[e], b = kScaled ? v[e + 1] * up : v[e + 1];
-          const __half2 h = __floats2half2_rn(a, b);
-          w[0][e / 2] = *reinterpret_cast<const uint32_t*>(&h);
-          if (P == 2) {
-            const float2 f = __half22float2(h);
-            const float ra = fabsf(a) < 1e30f ? (a - f.x) * 2048.0f : 0.0f, rb = fabsf(b) < 1e30f ? (b - f.y) * 2048.0f : 0.0f;
-            const __half2 l = __floats2half2_rn(ra, rb);
-            w[P - 1][e / 2] = *reinterpret_cast<const uint32_t*>(&l);
+          for (int p = 0; p < P; p++) {
+            const int64_t bytes = (left - p * (8 / P)) * (int64_t)sizeof(S);
+            const uint32_t n = bytes >= 16 ? 16 : bytes > 0 ? (uint32_t)bytes : 0;   // the rest is zero
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst) + 16 * p),
+                         "l"(n ? src + p * (8 / P) : static_cast<const S*>(prm.x)), "r"(n)
+                         : "memory");
           }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++) reinterpret_cast<S*>(dst)[e] = e < left ? src[e] : S(0.0f);
         }
-      } else {
-#pragma unroll
-        for (int p = 0; p < P; p++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) w[p][e] = 0;
       }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (kScaled) {
+      __syncwarp();   // a thread reads back only what it wrote, but the maxima are a warp's
+      for (int t = 0; t < T; t++)
+        for (int c = threadIdx.x; c < per; c += 32 * kWarps) {
+          float v[8];
+          read_x8<S>(xs + t * xpitch + c * (16 * P), v);
+          uint32_t m = 0;
 #pragma unroll
-      for (int p = 0; p < P; p++)
-        *reinterpret_cast<uint4*>(xs + (p * NTOK + t) * xpitch + c * 16) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+          for (int e = 0; e < 8; e++) {
+            const uint32_t b = __float_as_uint(v[e]) & 0x7FFFFFFFu;
+            m = max(m, b < 0x7F800000u ? b : 0u);
+          }
+          m = __reduce_max_sync(0xffffffffu, m);
+          if (lane == 0) atomicMax(&top[t], m);
+        }
+      asm volatile("bar.sync 1, %0;" ::"r"(32 * kWarps) : "memory");
+      for (int t = 0; t < T; t++) {
+        // 2^(14 - e) for a largest magnitude of exponent e
+        const float up = __uint_as_float((uint32_t)min(268 - max((int)(top[t] >> 23), 1), 247) << 23);
+        for (int c = threadIdx.x; c < per; c += 32 * kWarps) {
+          uint8_t* at = xs + t * xpitch + c * (16 * P);
+          float v[8];
+          read_x8<S>(at, v);
+          uint32_t w[P][4];
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const float a = v[e] * up, b = v[e + 1] * up;
+            const __half2 h = __floats2half2_rn(a, b);
+            w[0][e / 2] = *reinterpret_cast<const uint32_t*>(&h);
+            if (P == 2) {   // of an infinity or NaN the first part holds it all
+              const float2 f = __half22float2(h);
+              const float ra = fabsf(a) < 1e30f ? (a - f.x) * 2048.0f : 0.0f, rb = fabsf(b) < 1e30f ? (b - f.y) * 2048.0f : 0.0f;
+              const __half2 l = __floats2half2_rn(ra, rb);
+              w[P - 1][e / 2] = *reinterpret_cast<const uint32_t*>(&l);
+            }
+          }
+#pragma unroll
+          for (int p = 0; p < P; p++) reinterpret_cast<uint4*>(at)[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+        }
+      }
     }
     asm volatile("bar.sync 1, %0;" ::"r"(32 * kWarps) : "memory");
 
@@ -240,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1)
         down[b][e] = kScaled ? __uint_as_float((uint32_t)max(max((int)(top[8 * b + 2 * t4 + e] >> 23), 1) - 14, 7) << 23) : 1.0f;
     const uint32_t row_at = (16 * warp + (lane & 7)) * 128, x7 = lane & 7;
     const uint32_t srow = ((16 * warp + g) & 31) * 16 + ((16 * warp + g) >> 5) * 4;   // row g's scale word; row g + 8: + 128
-    const uint32_t xlane = smem_u32(xs) + g * xpitch + t4 * 16;
+    const uint32_t xlane = smem_u32(xs) + g * xpitch + t4 * (16 * P);
     Ring rg{0, 0};
     bool ok = true;
     for (int s = s_begin; s < s_end; s++) {
@@ -250,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1)
       }
       const uint32_t sw = ring + rg.st * kStage;
       const uint8_t* sc = base + rg.st * kStage + 128 * 128;
-      const uint32_t xcol = xlane + (s - s_begin) * 512;
+      const uint32_t xcol = xlane + (s - s_begin) * (512 * P);
       float c[P][NB][4];
       if (FMT == kNVFP4) {
 #pragma unroll
@@ -303,10 +319,10 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1)
               uint4 xv;
               asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                            : "=r"(xv.x), "=r"(xv.y), "=r"(xv.z), "=r"(xv.w)
-                           : "r"(xcol + (p * NTOK + nb * 8) * xpitch + half * 256 + j * 64));
+                           : "r"(xcol + nb * 8 * xpitch + (half * 256 + j * 64) * P + p * 16));
               float(&d)[4] = c[p][nb];
-              if (FMT == kMXFP4) d[0] = d[1] = d[2] = d[3] = 0.0f;
-              mma_f16(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
+              if (FMT == kMXFP4) mma_f16_zero(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
+              else mma_f16(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
               mma_f16(d, a[2], b[2], a[3], b[3], xv.z, xv.w);
               if (FMT == kMXFP4) {
                 const float fine = p == 1 ? 1.0f / 2048.0f : 1.0f;
@@ -369,7 +385,7 @@ int launch_stream(StreamParams& p, const Mx4View& w, int split, cudaStream_t str
   const int64_t pitch = mx4_pitch(w.n), wt = (w.rows + 127) / 128;
   CUtensorMap mw, ms;
   if (!codes_map(&mw, w.codes, pitch, w.rows, 128, 128) || !scales_map(&ms, w.scales, wt * p.groups, kAtoms)) return 5;
-  const size_t smem = 1024 + (size_t)p.nst * kStage + (size_t)Parts<S>::k * 8 * NB * (p.slice * 2 + 64) + 8 * NB * 4 +
+  const size_t smem = 1024 + (size_t)p.nst * kStage + (size_t)8 * NB * (p.slice * 2 * Parts<S>::k + 64) + 8 * NB * 4 +
                       16 * kMaxStages + 64;
   return launch_cluster<mx4_stream_kernel<FMT, NB, S>>((int)wt * split, kThreads, smem, split, stream, mw, ms, p, split);
 }
@@ -396,7 +412,7 @@ bool stream_plan(int dtype, int64_t T, int64_t rows, int64_t n, StreamPlan* plan
   int split = 1;
   while (split < 8 && wt * split * 2 <= slots && split * 2 <= steps) split *= 2;
   // x's slice stays in shared memory beside at least three stages
-  auto x_bytes = [&](int sp) { return (int64_t)parts * 8 * nb * ((int64_t)(steps + sp - 1) / sp * 512 + 64); };
+  auto x_bytes = [&](int sp) { return (int64_t)8 * nb * ((int64_t)(steps + sp - 1) / sp * 512 * parts + 64); };
   const int64_t room = 222 * 1024;
   while (split < 8 && split * 2 <= steps && x_bytes(split) + 3 * stage > room) split *= 2;
   if (x_bytes(split) + 3 * stage > room) return false;

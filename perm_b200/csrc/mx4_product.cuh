@@ -102,13 +102,13 @@ __device__ __forceinline__ void join_partials(const void* part, int rank, int sp
   }
 }
 
-// Opts a kernel into its shared memory, once per device.
-template <auto K> inline bool opt_in_smem(size_t bytes) {
+// Lets a kernel use all of an SM's shared memory (launches ask for what they need), once per device.
+template <auto K> inline bool opt_in_smem() {
   static std::atomic<unsigned long long> opted{0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
   if (opted.load() & (1ull << dev)) return true;
-  if (cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
+  if (cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return false;
   opted.fetch_or(1ull << dev);
   return true;
 }
@@ -163,7 +163,7 @@ inline bool bf16_map(CUtensorMap* m, const void* p, int64_t rows, int64_t cols, 
 // Launches kernel K in clusters; 0, 4 (its shared memory was refused) or 6 (the launch was).
 template <auto K, typename... A>
 inline int launch_cluster(int grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {
-  if (!opt_in_smem<K>(smem)) return 4;
+  if (!opt_in_smem<K>()) return 4;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid, 1, 1);
   cfg.blockDim = dim3((unsigned)threads, 1, 1);

@@ -22,7 +22,7 @@
 // A CTA holds 128 rows (16 for each of eight warps) and a slice of the columns; a cluster of up to eight
 // shares a row tile and joins the partial sums through distributed shared memory in rank order.  Codes
 // and scale tiles arrive by TMA in stages of 256 columns; x is converted into shared memory while the first
-// stages are in flight.  Two CTAs fit an SM for up to 16 tokens.
+// stages are in flight.  Two CTAs fit an SM, or three for up to 8 tokens.
 #include "mx4_product.cuh"
 
 namespace cpk {
@@ -100,6 +100,18 @@ template <typename S> struct Parts { static constexpr int k = 1; static constexp
 template <> struct Parts<__half> { static constexpr int k = 1; static constexpr bool scaled = false; };
 template <> struct Parts<float> { static constexpr int k = 2; static constexpr bool scaled = true; };
 
+// Unit c of a row t, `units` to a row.
+struct Unit {
+  int t, c;
+  __device__ __forceinline__ Unit(int i, int units) : t(0), c(i) { wrap(units); }
+  __device__ __forceinline__ void next(int by, int units) {
+    c += by;
+    wrap(units);
+  }
+  __device__ __forceinline__ void wrap(int units) {
+    while (c >= units) c -= units, t++;
+  }
+};
 // Eight values of x in shared memory.
 template <typename S> __device__ __forceinline__ void read_x8(const uint8_t* at, float (&v)[8]) {
   constexpr int W = sizeof(S) / 2;
@@ -110,9 +122,27 @@ template <typename S> __device__ __forceinline__ void read_x8(const uint8_t* at,
 #pragma unroll
   for (int i = 0; i < 8; i++) v[i] = as_f32(e[i]);
 }
+// The largest finite magnitude of eight values, as float32 bits.
+template <typename S> __device__ __forceinline__ uint32_t top_x8(const uint8_t* at) {
+  if (sizeof(S) == 2) {   // bf16: two at a time; a NaN or infinity shows in the maximum and takes the long way
+    const uint4 w = *reinterpret_cast<const uint4*>(at);
+    const uint32_t two = __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu));
+    const uint32_t m = max(two >> 16, two & 0xFFFFu);
+    if (m < 0x7F80u) return m << 16;
+  }
+  float v[8];
+  read_x8<S>(at, v);
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const uint32_t b = __float_as_uint(v[e]) & 0x7FFFFFFFu;
+    m = max(m, b < 0x7F800000u ? b : 0u);
+  }
+  return m;
+}
 
 template <int FMT, int NB, typename S>
-__global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, NB == 1 ? 3 : 2)
     mx4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
                       const StreamParams prm, int split) {
   constexpr int NTOK = 8 * NB, P = Parts<S>::k;
@@ -126,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1)
   // different banks
   const int xpitch = prm.slice * 2 * P + (P == 1 ? 64 : 16);
   uint8_t* xs = base + nst * kStage;                     // [token][eight columns][part] f16
-  uint32_t* top = reinterpret_cast<uint32_t*>(xs + NTOK * xpitch);   // largest magnitudes, as bits
+  uint32_t* top = reinterpret_cast<uint32_t*>(xs + prm.T * xpitch);   // largest magnitudes, as bits
   uint64_t* bars = reinterpret_cast<uint64_t*>(top + NTOK);
   volatile int* misc = reinterpret_cast<volatile int*>(bars + 2 * kMaxStages);   // [0] abort
   const uint32_t ring = smem_u32(base), full0 = smem_u32(bars), empty0 = full0 + 8 * kMaxStages;
@@ -179,69 +209,58 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1)
     }
   } else {
     // ---- x into shared memory: asynchronous copies of the rows as they are, then (scaled types) a pass
-    // for the largest magnitudes and one that converts each group of eight values in place
-    const int per = (s_end - s_begin) * 32;   // groups of eight columns: a multiple of 32, so a warp holds one row
+    // for the largest magnitudes and one that converts each group of eight values in place.  A warp takes
+    // units of 256 columns of one row; a thread reads back only what it copied itself.
+    const int units = s_end - s_begin;   // a row's
     const int64_t k0 = (int64_t)s_begin * 256;
-    const S* x = static_cast<const S*>(prm.x) + k0;
-    for (int t = 0; t < NTOK; t++)
-      for (int c = threadIdx.x; c < per; c += 32 * kWarps) {
-        uint8_t* dst = xs + t * xpitch + c * (16 * P);
-        const int64_t left = t < T ? prm.K - k0 - (int64_t)c * 8 : 0;   // values of the row from here on
-        const S* src = x + t * prm.ld + c * 8;
-        if (prm.vec || left <= 0) {
+    Unit u(warp, units);
+    for (; u.t < T; u.next(kWarps, units)) {
+      const int c = u.c * 32 + lane;   // group of eight columns
+      const int64_t left = prm.K - k0 - (int64_t)c * 8;   // values of the row from here on
+      const S* src = static_cast<const S*>(prm.x) + u.t * prm.ld + k0 + c * 8;
+      uint8_t* dst = xs + u.t * xpitch + c * (16 * P);
+      if (prm.vec || left <= 0) {
 #pragma unroll
-          for (int p = 0; p < P; p++) {
-            const int64_t bytes = (left - p * (8 / P)) * (int64_t)sizeof(S);
-            const uint32_t n = bytes >= 16 ? 16 : bytes > 0 ? (uint32_t)bytes : 0;   // the rest is zero
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst) + 16 * p),
-                         "l"(n ? src + p * (8 / P) : static_cast<const S*>(prm.x)), "r"(n)
-                         : "memory");
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; e++) reinterpret_cast<S*>(dst)[e] = e < left ? src[e] : S(0.0f);
+        for (int p = 0; p < P; p++) {
+          const int64_t bytes = (left - p * (8 / P)) * (int64_t)sizeof(S);
+          const uint32_t n = bytes >= 16 ? 16 : bytes > 0 ? (uint32_t)bytes : 0;   // the rest is zero
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst) + 16 * p),
+                       "l"(n ? src + p * (8 / P) : static_cast<const S*>(prm.x)), "r"(n)
+                       : "memory");
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) reinterpret_cast<S*>(dst)[e] = e < left ? src[e] : S(0.0f);
       }
+    }
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (kScaled) {
-      __syncwarp();   // a thread reads back only what it wrote, but the maxima are a warp's
-      for (int t = 0; t < T; t++)
-        for (int c = threadIdx.x; c < per; c += 32 * kWarps) {
-          float v[8];
-          read_x8<S>(xs + t * xpitch + c * (16 * P), v);
-          uint32_t m = 0;
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const uint32_t b = __float_as_uint(v[e]) & 0x7FFFFFFFu;
-            m = max(m, b < 0x7F800000u ? b : 0u);
-          }
-          m = __reduce_max_sync(0xffffffffu, m);
-          if (lane == 0) atomicMax(&top[t], m);
-        }
+      for (u = Unit(warp, units); u.t < T; u.next(kWarps, units)) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, top_x8<S>(xs + u.t * xpitch + (u.c * 32 + lane) * (16 * P)));
+        if (lane == 0) atomicMax(&top[u.t], m);
+      }
       asm volatile("bar.sync 1, %0;" ::"r"(32 * kWarps) : "memory");
-      for (int t = 0; t < T; t++) {
+      for (u = Unit(warp, units); u.t < T; u.next(kWarps, units)) {
         // 2^(14 - e) for a largest magnitude of exponent e
-        const float up = __uint_as_float((uint32_t)min(268 - max((int)(top[t] >> 23), 1), 247) << 23);
-        for (int c = threadIdx.x; c < per; c += 32 * kWarps) {
-          uint8_t* at = xs + t * xpitch + c * (16 * P);
-          float v[8];
-          read_x8<S>(at, v);
-          uint32_t w[P][4];
+        const float up = __uint_as_float((uint32_t)min(268 - max((int)(top[u.t] >> 23), 1), 247) << 23);
+        uint8_t* at = xs + u.t * xpitch + (u.c * 32 + lane) * (16 * P);
+        float v[8];
+        read_x8<S>(at, v);
+        uint32_t w[P][4];
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const float a = v[e] * up, b = v[e + 1] * up;
-            const __half2 h = __floats2half2_rn(a, b);
-            w[0][e / 2] = *reinterpret_cast<const uint32_t*>(&h);
-            if (P == 2) {   // of an infinity or NaN the first part holds it all
-              const float2 f = __half22float2(h);
-              const float ra = fabsf(a) < 1e30f ? (a - f.x) * 2048.0f : 0.0f, rb = fabsf(b) < 1e30f ? (b - f.y) * 2048.0f : 0.0f;
-              const __half2 l = __floats2half2_rn(ra, rb);
-              w[P - 1][e / 2] = *reinterpret_cast<const uint32_t*>(&l);
-            }
+        for (int e = 0; e < 8; e += 2) {
+          const float a = v[e] * up, b = v[e + 1] * up;
+          const __half2 h = __floats2half2_rn(a, b);
+          w[0][e / 2] = *reinterpret_cast<const uint32_t*>(&h);
+          if (P == 2) {   // of an infinity or NaN the first part holds it all
+            const float2 f = __half22float2(h);
+            const float ra = fabsf(a) < 1e30f ? (a - f.x) * 2048.0f : 0.0f, rb = fabsf(b) < 1e30f ? (b - f.y) * 2048.0f : 0.0f;
+            const __half2 l = __floats2half2_rn(ra, rb);
+            w[P - 1][e / 2] = *reinterpret_cast<const uint32_t*>(&l);
           }
-#pragma unroll
-          for (int p = 0; p < P; p++) reinterpret_cast<uint4*>(at)[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
         }
+#pragma unroll
+        for (int p = 0; p < P; p++) reinterpret_cast<uint4*>(at)[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
       }
     }
     asm volatile("bar.sync 1, %0;" ::"r"(32 * kWarps) : "memory");
@@ -256,7 +275,10 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1)
         down[b][e] = kScaled ? __uint_as_float((uint32_t)max(max((int)(top[8 * b + 2 * t4 + e] >> 23), 1) - 14, 7) << 23) : 1.0f;
     const uint32_t row_at = (16 * warp + (lane & 7)) * 128, x7 = lane & 7;
     const uint32_t srow = ((16 * warp + g) & 31) * 16 + ((16 * warp + g) >> 5) * 4;   // row g's scale word; row g + 8: + 128
-    const uint32_t xlane = smem_u32(xs) + g * xpitch + t4 * (16 * P);
+    // tokens past the last read a row that is there; their results are not used
+    uint32_t xlane[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) xlane[b] = smem_u32(xs) + (8 * b + g < T ? 8 * b + g : 0) * xpitch + t4 * (16 * P);
     Ring rg{0, 0};
     bool ok = true;
     for (int s = s_begin; s < s_end; s++) {
@@ -266,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1)
       }
       const uint32_t sw = ring + rg.st * kStage;
       const uint8_t* sc = base + rg.st * kStage + 128 * 128;
-      const uint32_t xcol = xlane + (s - s_begin) * (512 * P);
+      const uint32_t xcol = (s - s_begin) * (512 * P);
       float c[P][NB][4];
       if (FMT == kNVFP4) {
 #pragma unroll
@@ -319,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1)
               uint4 xv;
               asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                            : "=r"(xv.x), "=r"(xv.y), "=r"(xv.z), "=r"(xv.w)
-                           : "r"(xcol + nb * 8 * xpitch + (half * 256 + j * 64) * P + p * 16));
+                           : "r"(xlane[nb] + xcol + (half * 256 + j * 64) * P + p * 16));
               float(&d)[4] = c[p][nb];
               if (FMT == kMXFP4) mma_f16_zero(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
               else mma_f16(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
@@ -385,7 +407,7 @@ int launch_stream(StreamParams& p, const Mx4View& w, int split, cudaStream_t str
   const int64_t pitch = mx4_pitch(w.n), wt = (w.rows + 127) / 128;
   CUtensorMap mw, ms;
   if (!codes_map(&mw, w.codes, pitch, w.rows, 128, 128) || !scales_map(&ms, w.scales, wt * p.groups, kAtoms)) return 5;
-  const size_t smem = 1024 + (size_t)p.nst * kStage + (size_t)8 * NB * (p.slice * 2 * Parts<S>::k + 64) + 8 * NB * 4 +
+  const size_t smem = 1024 + (size_t)p.nst * kStage + (size_t)p.T * (p.slice * 2 * Parts<S>::k + 64) + 8 * NB * 4 +
                       16 * kMaxStages + 64;
   return launch_cluster<mx4_stream_kernel<FMT, NB, S>>((int)wt * split, kThreads, smem, split, stream, mw, ms, p, split);
 }
@@ -393,8 +415,7 @@ int launch_stream(StreamParams& p, const Mx4View& w, int split, cudaStream_t str
 template <int FMT, typename S>
 int launch_tokens(StreamParams& p, const Mx4View& w, int split, cudaStream_t stream) {
   if (p.T <= 8) return launch_stream<FMT, 1, S>(p, w, split, stream);
-  if (p.T <= 16) return launch_stream<FMT, 2, S>(p, w, split, stream);
-  return launch_stream<FMT, 4, S>(p, w, split, stream);
+  return launch_stream<FMT, 2, S>(p, w, split, stream);
 }
 
 }  // namespace
@@ -405,21 +426,22 @@ struct StreamPlan {
 };
 // False where x's slices would not leave room in shared memory.
 bool stream_plan(int dtype, int64_t T, int64_t rows, int64_t n, StreamPlan* plan) {
-  if (T > 32) return false;
-  const int parts = dtype == kMxF32 ? 2 : 1, nb = T <= 8 ? 1 : T <= 16 ? 2 : 4;
-  const int64_t wt = (rows + 127) / 128, slots = (int64_t)device_sm_count() * (nb <= 2 ? 2 : 1);
+  if (T > 16) return false;
+  const int parts = dtype == kMxF32 ? 2 : 1;
+  const int64_t wt = (rows + 127) / 128, slots = (int64_t)device_sm_count() * (T <= 8 ? 3 : 2);
   const int steps = (int)(mx4_pitch(n) / 128), stage = 128 * 128 + 4 * 512;   // NVFP4's; MXFP4's is smaller
   int split = 1;
   while (split < 8 && wt * split * 2 <= slots && split * 2 <= steps) split *= 2;
   // x's slice stays in shared memory beside at least three stages
-  auto x_bytes = [&](int sp) { return (int64_t)8 * nb * ((int64_t)(steps + sp - 1) / sp * 512 * parts + 64); };
+  auto x_bytes = [&](int sp) { return T * ((int64_t)(steps + sp - 1) / sp * 512 * parts + 64); };
   const int64_t room = 222 * 1024;
   while (split < 8 && split * 2 <= steps && x_bytes(split) + 3 * stage > room) split *= 2;
   if (x_bytes(split) + 3 * stage > room) return false;
-  // two CTAs to an SM where that leaves each three stages
-  const int64_t half = room / 2 - 1024 - x_bytes(split);
+  // as many CTAs to an SM as the split counts on, where that leaves each three stages
   const int mine = (steps + split - 1) / split;
-  const int nst = (int)((nb <= 2 && half >= 3 * stage ? half : room - x_bytes(split)) / stage);
+  int nst = 0;
+  for (int ctas = T <= 8 ? 3 : 2; ctas > 0 && nst < std::min(3, mine); ctas--)
+    nst = (int)((room / ctas - 2048 - x_bytes(split)) / stage);
   *plan = StreamPlan{split, std::min(std::min(nst, kMaxStages), mine), mine * 256};
   return true;
 }

@@ -28,6 +28,11 @@ from . import _native as nat
 
 BLOCK = {"MXFP4": 32, "NVFP4": 16}
 _DTYPE = {torch.bfloat16: nat.CP_MX4_BF16, torch.float16: nat.CP_MX4_F16, torch.float32: nat.CP_MX4_F32}
+# A call on one token takes a few microseconds on the device, so the host's part is kept short: the
+# stream's address comes from torch directly (a Stream object costs more than the rest of the checks).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_workspace = {}   # sizes of a linear call -> workspace bytes
 
 
 class Mx4Tensor:
@@ -38,7 +43,7 @@ class Mx4Tensor:
     scales  uint8, tiles of 128 rows x 4 blocks, [ceil(rows/128), P/(4 block), 32, 4, 4]: entry
             [i, g, r, j, k] is the scale of row 128 i + 32 j + r, block 4 g + k; zero past n
     tensor_scale  a positive float that multiplies every value"""
-    __slots__ = ("codes", "scales", "fmt", "rows", "n", "tensor_scale")
+    __slots__ = ("codes", "scales", "fmt", "rows", "n", "tensor_scale", "dev")
 
     def __init__(self, codes, scales, fmt, rows, n, tensor_scale=1.0):
         if fmt not in BLOCK:
@@ -54,7 +59,7 @@ class Mx4Tensor:
         if not (tensor_scale > 0.0 and math.isfinite(tensor_scale)):
             raise ValueError("tensor_scale must be positive and finite")
         self.codes, self.scales, self.fmt, self.rows, self.n = codes, scales, fmt, rows, n
-        self.tensor_scale = tensor_scale
+        self.tensor_scale, self.dev = tensor_scale, codes.get_device()   # dev: CUDA device index, -1 on the host
 
     @property
     def shape(self):
@@ -68,28 +73,28 @@ class Mx4Tensor:
         return f"Mx4Tensor({self.fmt}, [{self.rows}, {self.n}], tensor_scale={self.tensor_scale}, device={self.device})"
 
 
-def _need_cuda(t, what):
-    if not t.is_cuda:
-        raise nat.CudaPathError(f"{what}: tensors must be on a CUDA device")
+def _refuse_host(what):
+    raise nat.CudaPathError(f"{what}: tensors must be on a CUDA device")
 
 
-def _call(dev, fn, what, *args):
-    """fn(*args, stream) on `dev`'s current stream, with `dev` current."""
-    idx = dev.index
-    if idx == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(idx).cuda_stream)
+def _call(idx, fn, what, *args):
+    """fn(*args, stream) on device idx's current stream, with idx the current device."""
+    if idx == _current_device():
+        rc = fn(*args, _raw_stream(idx))
     else:
         with torch.cuda.device(idx):
-            rc = fn(*args, torch.cuda.current_stream(idx).cuda_stream)
+            rc = fn(*args, _raw_stream(idx))
     if rc:
         nat.check(rc, what)
 
 
-def _empty_operand(fmt, rows, n, dev):
+def _empty_operand(like, fmt, rows, n, tensor_scale):
+    q = Mx4Tensor.__new__(Mx4Tensor)
     pitch = (n + 255) // 256 * 128
-    codes = torch.empty((rows, pitch), dtype=torch.uint8, device=dev)
-    scales = torch.empty(((rows + 127) // 128, pitch // (2 * BLOCK[fmt]), 32, 4, 4), dtype=torch.uint8, device=dev)
-    return codes, scales
+    q.codes = like.new_empty((rows, pitch), dtype=torch.uint8)
+    q.scales = like.new_empty(((rows + 127) // 128, pitch // (2 * BLOCK[fmt]), 32, 4, 4), dtype=torch.uint8)
+    q.fmt, q.rows, q.n, q.tensor_scale, q.dev = fmt, rows, n, tensor_scale, like.get_device()
+    return q
 
 
 def tensor_scale_for(x):
@@ -109,21 +114,22 @@ def quantize(x, fmt, qw=None, tensor_scale=1.0):
     weights [n], or None.  tensor_scale: a power of two (1 for MXFP4)."""
     if fmt not in BLOCK:
         raise ValueError(f"unknown 4-bit format {fmt!r}")
-    _need_cuda(x, "mx4.quantize")
+    if not x.is_cuda:
+        _refuse_host("mx4.quantize")
     dt = _DTYPE.get(x.dtype)
     if dt is None or x.dim() != 2 or x.shape[1] == 0:
         raise ValueError("mx4.quantize expects a bf16, f16 or f32 matrix [rows, n], n > 0")
     rows, n = x.shape
-    if x.stride(1) != 1 and n > 1 or rows > 1 and x.stride(0) < n:
+    if not x.is_contiguous() and (x.stride(1) != 1 or x.stride(0) < n):
         x = x.contiguous()
     if qw is not None:
         if qw.shape != (n,) or qw.device != x.device:
             raise ValueError(f"qw must hold {n} column weights on x's device")
         qw = qw.to(torch.float32).contiguous()
-    codes, scales = _empty_operand(fmt, rows, n, x.device)
-    _call(x.device, nat.lib().cp_mx4_quantize, "mx4.quantize", nat.MX4_ID[fmt], dt, x.data_ptr(), rows, n, x.stride(0),
-          None if qw is None else qw.data_ptr(), tensor_scale, codes.data_ptr(), scales.data_ptr())
-    return Mx4Tensor(codes, scales, fmt, rows, n, tensor_scale)
+    q = _empty_operand(x, fmt, rows, n, tensor_scale)
+    _call(q.dev, nat.lib().cp_mx4_quantize, "mx4.quantize", nat.MX4_ID[fmt], dt, x.data_ptr(), rows, n, x.stride(0),
+          None if qw is None else qw.data_ptr(), tensor_scale, q.codes.data_ptr(), q.scales.data_ptr())
+    return q
 
 
 def dequantize(q, dtype=torch.float32):
@@ -131,25 +137,27 @@ def dequantize(q, dtype=torch.float32):
     dt = _DTYPE.get(dtype)
     if dt is None:
         raise ValueError("mx4.dequantize: dtype must be bf16, f16 or f32")
-    _need_cuda(q.codes, "mx4.dequantize")
-    out = torch.empty((q.rows, q.n), dtype=dtype, device=q.device)
-    _call(q.device, nat.lib().cp_mx4_dequantize, "mx4.dequantize", nat.MX4_ID[q.fmt], q.codes.data_ptr(),
+    if q.dev < 0:
+        _refuse_host("mx4.dequantize")
+    out = q.codes.new_empty((q.rows, q.n), dtype=dtype)
+    _call(q.dev, nat.lib().cp_mx4_dequantize, "mx4.dequantize", nat.MX4_ID[q.fmt], q.codes.data_ptr(),
           q.scales.data_ptr(), q.rows, q.n, q.tensor_scale, dt, out.data_ptr())
     return out
 
 
 def from_gguf(raw, n):
     """GGUF MXFP4 bytes (uint8 CUDA [rows, n/32 * 17], as kquant.QUANTIZE["MXFP4"] gives) -> Mx4Tensor."""
-    _need_cuda(raw, "mx4.from_gguf")
+    if not raw.is_cuda:
+        _refuse_host("mx4.from_gguf")
     if n <= 0 or n % 32:
         raise ValueError(f"cannot reshape a row of {n} values into 32-value blocks")
     if raw.dtype != torch.uint8 or raw.dim() != 2 or raw.shape[1] != n // 32 * 17:
         raise ValueError(f"raw must be uint8 [rows, {n // 32 * 17}]")
     raw = raw.contiguous()
-    codes, scales = _empty_operand("MXFP4", raw.shape[0], n, raw.device)
-    _call(raw.device, nat.lib().cp_mx4_from_gguf, "mx4.from_gguf", raw.data_ptr(), raw.shape[0], n, codes.data_ptr(),
-          scales.data_ptr())
-    return Mx4Tensor(codes, scales, "MXFP4", raw.shape[0], n)
+    q = _empty_operand(raw, "MXFP4", raw.shape[0], n, 1.0)
+    _call(q.dev, nat.lib().cp_mx4_from_gguf, "mx4.from_gguf", raw.data_ptr(), q.rows, n, q.codes.data_ptr(),
+          q.scales.data_ptr())
+    return q
 
 
 def matmul(a, w, dtype=torch.bfloat16):
@@ -159,11 +167,12 @@ def matmul(a, w, dtype=torch.bfloat16):
         raise ValueError("mx4.matmul: dtype must be bf16, f16 or f32")
     if a.fmt != w.fmt or a.n != w.n:
         raise ValueError(f"mx4.matmul: {a!r} and {w!r} must have one format and one n")
-    if a.device != w.device:
+    if a.dev != w.dev:
         raise ValueError("mx4.matmul: operands must be on one device")
-    _need_cuda(a.codes, "mx4.matmul")
-    y = torch.empty((a.rows, w.rows), dtype=dtype, device=a.device)
-    _call(a.device, nat.lib().cp_mx4_matmul, "mx4.matmul", nat.MX4_ID[w.fmt], a.codes.data_ptr(), a.scales.data_ptr(),
+    if a.dev < 0:
+        _refuse_host("mx4.matmul")
+    y = a.codes.new_empty((a.rows, w.rows), dtype=dtype)
+    _call(a.dev, nat.lib().cp_mx4_matmul, "mx4.matmul", nat.MX4_ID[w.fmt], a.codes.data_ptr(), a.scales.data_ptr(),
           a.rows, w.codes.data_ptr(), w.scales.data_ptr(), w.rows, w.n, a.tensor_scale * w.tensor_scale, dt, y.data_ptr())
     return y
 
@@ -172,24 +181,38 @@ def _product(x, w, transpose, what):
     """x [..., K] times w^T (transpose: times w)."""
     dt = _DTYPE.get(x.dtype)
     K, out = (w.rows, w.n) if transpose else (w.n, w.rows)
+    shape = x.shape
     if dt is None:
         raise ValueError(f"{what} expects bf16, f16 or f32, not {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] != K:
-        raise ValueError(f"{what}: the last dimension must be {K}, not {tuple(x.shape)}")
-    if x.device != w.device:
+    if not shape or shape[-1] != K:
+        raise ValueError(f"{what}: the last dimension must be {K}, not {tuple(shape)}")
+    dev = w.dev
+    if x.get_device() != dev:
         raise ValueError(f"{what}: the operands must be on one device")
-    _need_cuda(x, what)
-    x2 = x if x.dim() == 2 else x.reshape(x.numel() // K if K else math.prod(x.shape[:-1]), K)
-    T = x2.shape[0]
-    if x2.stride(1) != 1 and K > 1 or T > 1 and x2.stride(0) < K:
-        x2 = x2.contiguous()
-    ld = x2.stride(0) if T > 1 else (K + 7) // 8 * 8
-    L = nat.lib()
-    y = torch.empty((*x.shape[:-1], out), dtype=x.dtype, device=x.device)
-    p = x2.data_ptr()
-    need = L.cp_mx4_linear_workspace_bytes(dt, p, T, ld, w.rows, w.n, transpose)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    _call(x.device, L.cp_mx4_linear, what, nat.MX4_ID[w.fmt], dt, p, T, ld, w.codes.data_ptr(), w.scales.data_ptr(),
+    if dev < 0:
+        _refuse_host(what)
+    if len(shape) == 2:
+        T = shape[0]
+        y = x.new_empty((T, out))
+    else:
+        T = math.prod(shape[:-1])
+        y = x.new_empty((*shape[:-1], out))
+        x = x.reshape(T, K)
+    ld = K
+    if not x.is_contiguous():
+        if x.stride(1) != 1 or T > 1 and x.stride(0) < K:
+            x = x.contiguous()
+        else:
+            ld = x.stride(0)
+    L, p = nat.lib(), x.data_ptr()
+    key = (dt, T, ld, w.rows, w.n, transpose, p & 15)
+    need = _workspace.get(key)
+    if need is None:
+        if len(_workspace) > 4096:
+            _workspace.clear()
+        need = _workspace[key] = L.cp_mx4_linear_workspace_bytes(dt, p, T, ld, w.rows, w.n, transpose)
+    ws = x.new_empty((need,), dtype=torch.uint8) if need else None
+    _call(dev, L.cp_mx4_linear, what, nat.MX4_ID[w.fmt], dt, p, T, ld, w.codes.data_ptr(), w.scales.data_ptr(),
           w.rows, w.n, w.tensor_scale, transpose, y.data_ptr(), ws.data_ptr() if need else None, need)
     return y
 
@@ -226,8 +249,8 @@ def status(device=None):
     """Raise CudaPathError if a bounded wait in an earlier product on `device` ran out (its result
     is incomplete); synchronises the current stream."""
     nat.torch_cuda()
-    dev = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index or 0)
-    _call(dev, nat.lib().cp_mx4_status, "mx4.status")
+    idx = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    _call(idx, nat.lib().cp_mx4_status, "mx4.status")
 
 
 class Linear(torch.nn.Module):

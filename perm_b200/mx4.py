@@ -227,7 +227,9 @@ class _Product(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return _Product.apply(dy, ctx.w, 1 - ctx.transpose), None, None
+        if torch.is_grad_enabled():   # create_graph: the gradient has one itself
+            return _Product.apply(dy, ctx.w, 1 - ctx.transpose), None, None
+        return _product(dy, ctx.w, 1 - ctx.transpose, "mx4.linear (backward)"), None, None
 
 
 def linear(x, w):

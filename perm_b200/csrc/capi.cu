@@ -693,7 +693,7 @@ int cp_mx4_quantize(int fmt, int dtype, const void* x, int64_t rows, int64_t n, 
   if (((uintptr_t)codes | (uintptr_t)scales) & 15) return set_err(CP_ERR_ARG, "codes and scales must be 16-byte aligned");
   if ((uintptr_t)x % mx4_elem(dtype) || ((uintptr_t)qw & 3)) return set_err(CP_ERR_ARG, "x or qw is misaligned");
   ProfScope ps(kProfFit, (cudaStream_t)stream);
-  return check_rc(cpk::launch_mx4_quantize(fmt, dtype, x, rows, n, ld, qw, 1.0f / tensor_scale, codes, scales,
+  return check_rc(cpk::launch_mx4_quantize(fmt, dtype, x, rows, n, ld, qw, tensor_scale, codes, scales,
                                            (cudaStream_t)stream),
                   "cp_mx4_quantize");
 }

@@ -48,8 +48,8 @@ __device__ __forceinline__ float2 e2m1x2_value(uint32_t byte) {
       : "r"(byte & 0xFF));
   return __half22float2(*reinterpret_cast<__half2*>(&h));
 }
-// Eight values -> eight codes, round to nearest even, saturating at 6.
-__device__ __forceinline__ uint32_t e2m1x8(const float (&q)[8]) {
+// Eight values (four pairs) -> eight codes, round to nearest even, saturating at 6.
+__device__ __forceinline__ uint32_t e2m1x8(const float2 (&q)[4]) {
   uint32_t r;
   asm("{\n\t.reg .b8 a, b, c, d;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
@@ -58,16 +58,13 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&q)[8]) {
       "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
       "mov.b32 %0, {a, b, c, d};\n\t}"
       : "=r"(r)
-      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
+      : "f"(q[0].x), "f"(q[0].y), "f"(q[1].x), "f"(q[1].y), "f"(q[2].x), "f"(q[2].y), "f"(q[3].x), "f"(q[3].y));
   return r;
 }
 
-// Largest of a block's magnitudes, as bits (a NaN or infinity is >= 0x7F800000 and wins); lanes
-// of a block hold 8 values each: 4 lanes for MXFP4, 2 for NVFP4.
-template <int FMT> __device__ __forceinline__ uint32_t mx_block_max(const float (&v)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+// Largest of a block's magnitudes, as bits (a NaN or infinity is >= 0x7F800000 and wins), from the
+// largest of this lane's; lanes of a block hold 8 values each: 4 lanes for MXFP4, 2 for NVFP4.
+template <int FMT> __device__ __forceinline__ uint32_t mx_block_max(uint32_t m) {
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
   if (FMT == kMXFP4) m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
   return m;
@@ -75,45 +72,58 @@ template <int FMT> __device__ __forceinline__ uint32_t mx_block_max(const float 
 
 // Scale byte of a block whose largest magnitude has the bits m.
 //   MXFP4: floor(log2 max) - 2, the exponent at which the maximum lies in [4, 8).
-//   NVFP4: the e4m3 nearest to max / 6.  The quotient is rounded to odd first (truncated, with a
-//   last bit that says whether anything was cut), so the second rounding is the only one that
-//   counts; max arrives already divided by the tensor scale.
-template <int FMT> __device__ __forceinline__ int mx_first_scale(uint32_t m) {
-  if (m >= 0x7F800000u) return mx_nan_scale<FMT>();
-  if (FMT == kMXFP4) return max((int)(m >> 23) - 2, 0);
-  const float a = __uint_as_float(m);
-  float q = __fdiv_rz(a, 6.0f);
-  if (__fmaf_rn(q, 6.0f, -a) != 0.0f) q = __uint_as_float(__float_as_uint(q) | 1u);
+//   NVFP4: the e4m3 nearest to max / (6 tensor_scale).  t is the approximate quotient cut to nine
+//   significant bits; the borders between e4m3 values have five.  r = a - 6 t has the right sign, and
+//   t + 1.9 r / 6, which stays short of t's neighbours, is on the side of t that a / 6 is on (t itself if
+//   they are equal), so the conversion's rounding is that of the exact quotient.
+template <int FMT> __device__ __forceinline__ int mx_first_scale(uint32_t m, float inv_tensor_scale) {
+  if (FMT == kMXFP4) return m >= 0x7F800000u ? mx_nan_scale<FMT>() : max((int)(m >> 23) - 2, 0);
+  const float a = fminf(__fmul_rn(__uint_as_float(m), inv_tensor_scale), 3e38f);
+  const float t = __uint_as_float((__float_as_uint(__fmul_rn(a, 1.0f / 6.0f)) + 0x4000u) & 0xFFFF8000u);
+  const float q = __fmaf_rn(__fmaf_rn(-6.0f, t, a), 1.9f / 6.0f, t);
   uint32_t r;
   asm("{\n\t.reg .b16 s;\n\tcvt.rn.satfinite.e4m3x2.f32 s, %1, %1;\n\tcvt.u32.u16 %0, s;\n\t}" : "=r"(r) : "f"(q));
-  return (int)(r & 0x7F);
+  return m >= 0x7F800000u ? mx_nan_scale<FMT>() : (int)(r & 0x7F);
 }
 
-// Codes of eight values against a block's scale.
-//   MXFP4: v / 2^e is exact, so the conversion's rounding is the only one.
-//   NVFP4: v / s is not.  t is the multiple of 1/4 nearest to the approximate quotient, and every
-//   border between two e2m1 values is such a multiple.  t s is exact (t has at most 5 bits where
-//   a border can lie, s has 4) and r = v - t s has the right sign, so t + 1.9 r / s, which stays
-//   within a quarter of t, is on the side of t that v is on, and is t itself on a tie.
-template <int FMT> __device__ __forceinline__ uint32_t mx_codes(const float (&v)[8], int byte) {
-  float q[8];
-  if (FMT == kMXFP4) {
-    const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);   // byte <= 253: a normal power of two
-#pragma unroll
-    for (int i = 0; i < 8; i++) q[i] = __fmul_rn(v[i], inv);
+// A block's step, the value of code 1.0: scale times a power of two (the tensor scale, or a unit in
+// which the block's values are held), and about one over it.
+struct MxStep {
+  float s, inv;
+};
+template <int FMT> __device__ __forceinline__ MxStep mx_step(int byte, float times) {
+  MxStep st;
+  st.s = __fmul_rn(mx_scale_value<FMT>(byte), times);
+  if (FMT == kMXFP4) {   // a power of two (2^-127 has the field 0): its inverse is one too
+    st.inv = __uint_as_float((uint32_t)(254 - (int)(__float_as_uint(st.s) >> 23)) << 23);
   } else {
-    const float s = e4m3_value(byte);
-    const float inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
-    const float slope = 1.9f * inv;
-    constexpr float kQuarter = 3145728.0f;   // 1.5 * 2^21: adding it rounds to a multiple of 1/4
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(st.inv) : "f"(st.s));
+    if (!(st.s > 0.0f)) st.inv = 0.0f;   // a scale of zero: every code is zero
+  }
+  return st;
+}
+
+// Codes of eight values against a block's step.
+//   MXFP4: v / 2^e is exact, so the conversion's rounding is the only one.
+//   NVFP4: v / s is not.  t is a multiple of 1/4 next to the approximate quotient, and every border
+//   between two e2m1 values is such a multiple.  t s is exact (t has at most 5 bits where a border can
+//   lie, s has 4) and r = v - t s has the right sign, so t + 1.9 r / s, which stays within a quarter of
+//   t, is on the side of t that v is on, and is t itself on a tie.  Quotients past 2^21, which only a
+//   saturated scale leaves, lose the quarter but not that they saturate.
+template <int FMT> __device__ __forceinline__ uint32_t mx_codes(const float2 (&v)[4], const MxStep& st) {
+  float2 q[4];
+  const float2 inv = make_float2(st.inv, st.inv);
+  if (FMT == kMXFP4) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      // the clamp keeps the magic addition in range; past 8 every value is 6
-      const float a = fminf(fmaxf(__fmul_rn(v[i], inv), -64.0f), 64.0f);
-      const float t = __fsub_rn(__fadd_rn(a, kQuarter), kQuarter);
-      const float r = __fmaf_rn(-t, s, v[i]);
-      // +0 for t keeps the sign of v on values that round to zero; it does not matter to any sum
-      q[i] = __fmaf_rn(r, slope, t);
+    for (int i = 0; i < 4; i++) q[i] = __fmul2_rn(v[i], inv);
+  } else {
+    constexpr float kQuarter = 3145728.0f;   // 1.5 * 2^21: adding it rounds to a multiple of 1/4
+    const float2 up = make_float2(kQuarter, kQuarter), down = make_float2(-kQuarter, -kQuarter);
+    const float2 ms = make_float2(-st.s, -st.s), slope = make_float2(1.9f * st.inv, 1.9f * st.inv);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 t = __fadd2_rn(__ffma2_rn(v[i], inv, up), down);
+      q[i] = __ffma2_rn(__ffma2_rn(t, ms, v[i]), slope, t);
     }
   }
   return e2m1x8(q);

@@ -23,7 +23,7 @@ inline int64_t mx4_scale_bytes(int fmt, int64_t rows, int64_t n) {
 }
 
 int launch_mx4_quantize(int fmt, int dtype, const void* x, int64_t rows, int64_t n, int64_t ld, const float* qw,
-                        float inv_scale, uint8_t* codes, uint8_t* scales, cudaStream_t stream);
+                        float scale, uint8_t* codes, uint8_t* scales, cudaStream_t stream);
 // out: rows ld elements apart.
 int launch_mx4_dequantize(const Mx4View& v, float scale, int dtype, void* out, int64_t ld, cudaStream_t stream);
 // GGUF MXFP4 container (17-byte blocks of 32): encode, decode, weighted error, and to the operand.

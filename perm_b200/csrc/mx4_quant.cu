@@ -14,6 +14,7 @@
 // bits; float32 sums decide it unless two candidates are within 2^-16 of each other (their
 // error is below 2^-19), and only then are the sums formed again in 64 bits.
 #include <cuda_runtime.h>
+#include <type_traits>
 #include "kquant_kernels.h"
 #include "mx4_format.cuh"
 
@@ -24,20 +25,38 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 
-// Eight consecutive values of a row; left = values of the row from here on (may be <= 0).
-template <typename T> __device__ __forceinline__ void load8(const T* p, int64_t left, bool vec, float (&v)[8]) {
+// Eight consecutive values of a row, in pairs; left = values of the row from here on (may be <= 0).
+// Returns the largest magnitude's bits.
+template <typename T>
+__device__ __forceinline__ uint32_t load8(const T* p, int64_t left, bool vec, float2 (&v)[4]) {
   if (vec && left >= 8) {
-    constexpr int W = sizeof(T) * 8 / 16;
-    uint4 w[W];
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+      v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w), v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
+    } else {
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {   // a bf16 is the upper half of its float32
 #pragma unroll
-    for (int i = 0; i < W; i++) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-    const T* e = reinterpret_cast<const T*>(w);
+        for (int i = 0; i < 4; i++) v[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xFFFF0000u));
+        const uint32_t m = __vmaxu2(__vmaxu2(u[0] & 0x7FFF7FFFu, u[1] & 0x7FFF7FFFu),
+                                    __vmaxu2(u[2] & 0x7FFF7FFFu, u[3] & 0x7FFF7FFFu));
+        return max(m & 0xFFFF0000u, m << 16);
+      } else {
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = to_f32(e[i]);
+        for (int i = 0; i < 4; i++) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      }
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = i < left ? to_f32(p[i]) : 0.0f;
+    for (int i = 0; i < 4; i++)
+      v[i] = make_float2(2 * i < left ? to_f32(p[2 * i]) : 0.0f, 2 * i + 1 < left ? to_f32(p[2 * i + 1]) : 0.0f);
   }
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    m = max(m, max(__float_as_uint(v[i].x) & 0x7FFFFFFFu, __float_as_uint(v[i].y) & 0x7FFFFFFFu));
+  return m;
 }
 
 template <int FMT> __host__ __device__ constexpr int mx_candidates() { return FMT == kMXFP4 ? 3 : 8; }
@@ -55,36 +74,39 @@ template <int FMT, typename T> __device__ __forceinline__ T block_sum(T e) {
   return e;
 }
 
-// Scale byte and codes of a block (8 values per lane; v already divided by the tensor scale).
+// Scale byte and codes of a block (8 values per lane, `top` the largest of them as bits).
 template <int FMT, bool IMAT>
-__device__ __forceinline__ uint32_t quantize_block(const float (&v)[8], const float (&w)[8], int& byte) {
-  const uint32_t m = mx_block_max<FMT>(v);
-  byte = mx_first_scale<FMT>(m);
+__device__ __forceinline__ uint32_t quantize_block(float2 (&v)[4], uint32_t top, const float2 (&w)[4], float tensor_scale,
+                                                   float inv_tensor_scale, int& byte) {
+  const uint32_t m = mx_block_max<FMT>(top);
+  byte = mx_first_scale<FMT>(m, inv_tensor_scale);
   const bool finite = m < 0x7F800000u;   // else the scale byte is NaN and the block decodes to NaN
-  uint32_t code = mx_codes<FMT>(v, byte);
-  if constexpr (IMAT) {
+  if constexpr (!IMAT) {
+    const uint32_t code = mx_codes<FMT>(v, mx_step<FMT>(byte, tensor_scale));
+    return finite ? code : 0;
+  } else {
     constexpr int C = mx_candidates<FMT>();
     const int first = byte;
-    // differences in units of the block's maximum, so that their squares neither vanish nor overflow
-    const int mexp = max((int)(m >> 23), 1);
-    const float unit = __uint_as_float((uint32_t)min(max(254 - mexp, 1), 253) << 23);
+    // values and steps in units of the block's maximum (a power of two), so that squares neither vanish
+    // nor overflow
+    const float unit = __uint_as_float((uint32_t)min(max(254 - (int)(m >> 23), 1), 253) << 23);
+    const float times = __fmul_rn(tensor_scale, unit);
     float err[C];
     uint32_t codes[C];
 #pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = __fmul2_rn(v[i], make_float2(unit, unit));
+#pragma unroll
     for (int c = 0; c < C; c++) {
-      const int b = mx_candidate<FMT>(first, c);
-      const float s = mx_scale_value<FMT>(b);
-      codes[c] = c == 0 ? code : mx_codes<FMT>(v, b);
-      float e = 0.0f;
+      const MxStep st = mx_step<FMT>(mx_candidate<FMT>(first, c), times);
+      codes[c] = mx_codes<FMT>(v, st);
+      const float2 ms = make_float2(-st.s, -st.s);
+      float2 e = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const float2 q = e2m1x2_value(codes[c] >> (8 * i));
-        const float d0 = __fmul_rn(__fmaf_rn(-q.x, s, v[2 * i]), unit);
-        const float d1 = __fmul_rn(__fmaf_rn(-q.y, s, v[2 * i + 1]), unit);
-        e = __fadd_rn(e, __fmul_rn(w[2 * i], __fmul_rn(d0, d0)));
-        e = __fadd_rn(e, __fmul_rn(w[2 * i + 1], __fmul_rn(d1, d1)));
+        const float2 d = __ffma2_rn(e2m1x2_value(codes[c] >> (8 * i)), ms, v[i]);
+        e = __ffma2_rn(__fmul2_rn(w[i], d), d, e);
       }
-      err[c] = block_sum<FMT>(e);
+      err[c] = block_sum<FMT>(e.x + e.y);
     }
     int pick = 0;
     float best = err[0];
@@ -102,30 +124,29 @@ __device__ __forceinline__ uint32_t quantize_block(const float (&v)[8], const fl
       int pd = 0;
 #pragma unroll 1
       for (int c = 0; c < C; c++) {
-        const int b = mx_candidate<FMT>(first, c);
-        const double s = (double)mx_scale_value<FMT>(b);
-        const uint32_t cw = mx_codes<FMT>(v, b);
+        const MxStep st = mx_step<FMT>(mx_candidate<FMT>(first, c), times);
+        const uint32_t cw = mx_codes<FMT>(v, st);
         double e = 0.0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const float2 q = e2m1x2_value(cw >> (8 * i));
-          const double d0 = (double)v[2 * i] - (double)q.x * s, d1 = (double)v[2 * i + 1] - (double)q.y * s;
-          e += (double)w[2 * i] * (d0 * d0);
-          e += (double)w[2 * i + 1] * (d1 * d1);
+          const double d0 = (double)v[i].x - (double)q.x * (double)st.s, d1 = (double)v[i].y - (double)q.y * (double)st.s;
+          e += (double)w[i].x * (d0 * d0);
+          e += (double)w[i].y * (d1 * d1);
         }
         e = block_sum<FMT>(e);
         if (c == 0 || e < bd) bd = e, pd = c;
       }
       if (near) pick = pd;
     }
-    if (first > 0 && finite) {   // scale byte 0 (an all but empty block) is not searched
-      byte = mx_candidate<FMT>(first, pick);
+    if (first == 0 || !finite) pick = 0;   // scale byte 0 (an all but empty block) is not searched
+    uint32_t code = codes[0];
 #pragma unroll
-      for (int c = 0; c < C; c++)
-        if (c == pick) code = codes[c];
-    }
+    for (int c = 1; c < C; c++)
+      if (c == pick) code = codes[c];
+    if (pick > 0) byte = mx_candidate<FMT>(first, pick);
+    return finite ? code : 0;
   }
-  return finite ? code : 0;
 }
 
 constexpr int kWarps = 8;
@@ -134,7 +155,7 @@ constexpr int kWarps = 8;
 template <typename T, int FMT, bool IMAT>
 __global__ void __launch_bounds__(32 * kWarps)
     quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t n, int64_t ld, const float* __restrict__ qw,
-                    float inv_scale, int chunks, int64_t units, bool vec, uint8_t* __restrict__ codes,
+                    float scale, float inv_scale, int chunks, int64_t units, bool vec, uint8_t* __restrict__ codes,
                     uint8_t* __restrict__ scales) {
   const int64_t unit = blockIdx.x * (int64_t)kWarps + threadIdx.x / 32;
   if (unit >= units) return;
@@ -143,23 +164,17 @@ __global__ void __launch_bounds__(32 * kWarps)
   const int chunk = (int)(unit - rl * chunks);
   const int64_t row0 = (rl >> 5) * 128 + (rl & 31);
   const int64_t col = (int64_t)chunk * 256 + lane * 8, left = n - col;
-  float v[4][8], w[8];
+  float2 v[4][4], w[4];
+  uint32_t top[4];
 #pragma unroll
-  for (int j = 0; j < 4; j++) load8(x + (row0 + 32 * j) * ld + col, row0 + 32 * j < rows ? left : 0, vec, v[j]);
-  if constexpr (IMAT) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) w[i] = i < left ? __ldg(qw + col + i) : 0.0f;
-  }
+  for (int j = 0; j < 4; j++) top[j] = load8(x + (row0 + 32 * j) * ld + col, row0 + 32 * j < rows ? left : 0, vec, v[j]);
+  if constexpr (IMAT) load8(qw + col, left, (reinterpret_cast<uintptr_t>(qw) & 15) == 0, w);
   constexpr int LB = mx_block<FMT>() / 8;   // lanes per block
   uint32_t sb[4];
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    if (FMT == kNVFP4) {
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[j][i] = __fmul_rn(v[j][i], inv_scale);
-    }
     int byte;
-    const uint32_t code = quantize_block<FMT, IMAT>(v[j], w, byte);
+    const uint32_t code = quantize_block<FMT, IMAT>(v[j], top[j], w, scale, inv_scale, byte);
     if (row0 + 32 * j < rows)
       *reinterpret_cast<uint32_t*>(codes + (row0 + 32 * j) * (int64_t)chunks * 128 + chunk * 128 + lane * 4) = code;
     // the four bytes of a group of four blocks, gathered into its first lane
@@ -246,20 +261,21 @@ __global__ void __launch_bounds__(256) encode_kernel(const float* __restrict__ x
   __shared__ __align__(16) uint8_t stage[kCtaBlocks * kBlkBytes];
   const int64_t b0 = (int64_t)blockIdx.x * kCtaBlocks;
   const int t = threadIdx.x, l4 = t & 3;
-  float v[4][8];
+  float2 v[4][4];
+  uint32_t top[4];
 #pragma unroll
   for (int p = 0; p < 4; p++) {
     const int64_t b = b0 + p * 64 + (t >> 2);
-    load8(x + b * 32 + l4 * 8, b < nblk ? 8 : 0, true, v[p]);
+    top[p] = load8(x + b * 32 + l4 * 8, b < nblk ? 8 : 0, true, v[p]);
   }
 #pragma unroll
   for (int p = 0; p < 4; p++) {
     const int lb = p * 64 + (t >> 2);
     const int64_t b = b0 + lb;
-    float w[8];
+    float2 w[4];
     if constexpr (IMAT) load8(qw + (b % nb_row) * 32 + l4 * 8, b < nblk ? 8 : 0, true, w);
     int byte;
-    const uint32_t c = quantize_block<kMXFP4, IMAT>(v[p], w, byte);
+    const uint32_t c = quantize_block<kMXFP4, IMAT>(v[p], top[p], w, 1.0f, 1.0f, byte);
     const uint32_t other = __shfl_xor_sync(0xffffffffu, c, 2);   // values 16 further (lanes 0, 1)
     if (l4 < 2) {
       const uint32_t lo = spread16(c & 0xFFFF) | spread16(other & 0xFFFF) << 4;
@@ -374,14 +390,15 @@ __global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* __restrict__
 int64_t row_lanes(int64_t rows) { return rows / 128 * 32 + (rows % 128 < 32 ? rows % 128 : 32); }
 
 template <typename T>
-int quantize_typed(int fmt, const T* x, int64_t rows, int64_t n, int64_t ld, const float* qw, float inv_scale,
+int quantize_typed(int fmt, const T* x, int64_t rows, int64_t n, int64_t ld, const float* qw, float scale,
                    uint8_t* codes, uint8_t* scales, cudaStream_t stream) {
   const int chunks = (int)((n + 255) / 256);
   const int64_t units = row_lanes(rows) * chunks;
   const unsigned grid = (unsigned)((units + kWarps - 1) / kWarps);
   const bool vec = ((uintptr_t)x & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
 #define CPK_Q(F, I) \
-  quantize_kernel<T, F, I><<<grid, 32 * kWarps, 0, stream>>>(x, rows, n, ld, qw, inv_scale, chunks, units, vec, codes, scales)
+  quantize_kernel<T, F, I><<<grid, 32 * kWarps, 0, stream>>>(x, rows, n, ld, qw, scale, 1.0f / scale, chunks, units, vec, codes, \
+                                                               scales)
   if (fmt == kMXFP4) {
     if (qw) CPK_Q(kMXFP4, true);
     else CPK_Q(kMXFP4, false);
@@ -410,13 +427,13 @@ template <typename T> int dequantize_typed(const Mx4View& v, float scale, T* out
 }  // namespace
 
 int launch_mx4_quantize(int fmt, int dtype, const void* x, int64_t rows, int64_t n, int64_t ld, const float* qw,
-                        float inv_scale, uint8_t* codes, uint8_t* scales, cudaStream_t stream) {
+                        float scale, uint8_t* codes, uint8_t* scales, cudaStream_t stream) {
   if (rows == 0) return 0;
   if (dtype == kMxBF16)
-    return quantize_typed(fmt, static_cast<const __nv_bfloat16*>(x), rows, n, ld, qw, inv_scale, codes, scales, stream);
+    return quantize_typed(fmt, static_cast<const __nv_bfloat16*>(x), rows, n, ld, qw, scale, codes, scales, stream);
   if (dtype == kMxF16)
-    return quantize_typed(fmt, static_cast<const __half*>(x), rows, n, ld, qw, inv_scale, codes, scales, stream);
-  return quantize_typed(fmt, static_cast<const float*>(x), rows, n, ld, qw, inv_scale, codes, scales, stream);
+    return quantize_typed(fmt, static_cast<const __half*>(x), rows, n, ld, qw, scale, codes, scales, stream);
+  return quantize_typed(fmt, static_cast<const float*>(x), rows, n, ld, qw, scale, codes, scales, stream);
 }
 
 int launch_mx4_dequantize(const Mx4View& v, float scale, int dtype, void* out, int64_t ld, cudaStream_t stream) {

@@ -49,7 +49,7 @@ __device__ __forceinline__ float2 e2m1x2_value(uint32_t byte) {
   return __half22float2(*reinterpret_cast<__half2*>(&h));
 }
 // Eight values (four pairs) -> eight codes, round to nearest even, saturating at 6.
-__device__ __forceinline__ uint32_t e2m1x8(const float2 (&q)[4]) {
+__device__ __forceinline__ uint32_t e2m1x8(const float2* q) {
   uint32_t r;
   asm("{\n\t.reg .b8 a, b, c, d;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
@@ -63,10 +63,10 @@ __device__ __forceinline__ uint32_t e2m1x8(const float2 (&q)[4]) {
 }
 
 // Largest of a block's magnitudes, as bits (a NaN or infinity is >= 0x7F800000 and wins), from the
-// largest of this lane's; lanes of a block hold 8 values each: 4 lanes for MXFP4, 2 for NVFP4.
-template <int FMT> __device__ __forceinline__ uint32_t mx_block_max(uint32_t m) {
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  if (FMT == kMXFP4) m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+// largest of each of its LANES lanes.
+template <int LANES> __device__ __forceinline__ uint32_t mx_block_max(uint32_t m) {
+#pragma unroll
+  for (int o = 1; o < LANES; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   return m;
 }
 
@@ -103,30 +103,32 @@ template <int FMT> __device__ __forceinline__ MxStep mx_step(int byte, float tim
   return st;
 }
 
-// Codes of eight values against a block's step.
+// Codes of H pairs of values against a block's step, eight to a word.
 //   MXFP4: v / 2^e is exact, so the conversion's rounding is the only one.
 //   NVFP4: v / s is not.  t is a multiple of 1/4 next to the approximate quotient, and every border
 //   between two e2m1 values is such a multiple.  t s is exact (t has at most 5 bits where a border can
 //   lie, s has 4) and r = v - t s has the right sign, so t + 1.9 r / s, which stays within a quarter of
 //   t, is on the side of t that v is on, and is t itself on a tie.  Quotients past 2^21, which only a
 //   saturated scale leaves, lose the quarter but not that they saturate.
-template <int FMT> __device__ __forceinline__ uint32_t mx_codes(const float2 (&v)[4], const MxStep& st) {
-  float2 q[4];
+template <int FMT, int H>
+__device__ __forceinline__ void mx_codes(const float2 (&v)[H], const MxStep& st, uint32_t (&code)[H / 4]) {
+  float2 q[H];
   const float2 inv = make_float2(st.inv, st.inv);
   if (FMT == kMXFP4) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) q[i] = __fmul2_rn(v[i], inv);
+    for (int i = 0; i < H; i++) q[i] = __fmul2_rn(v[i], inv);
   } else {
     constexpr float kQuarter = 3145728.0f;   // 1.5 * 2^21: adding it rounds to a multiple of 1/4
     const float2 up = make_float2(kQuarter, kQuarter), down = make_float2(-kQuarter, -kQuarter);
     const float2 ms = make_float2(-st.s, -st.s), slope = make_float2(1.9f * st.inv, 1.9f * st.inv);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < H; i++) {
       const float2 t = __fadd2_rn(__ffma2_rn(v[i], inv, up), down);
       q[i] = __ffma2_rn(__ffma2_rn(t, ms, v[i]), slope, t);
     }
   }
-  return e2m1x8(q);
+#pragma unroll
+  for (int i = 0; i < H / 4; i++) code[i] = e2m1x8(q + 4 * i);
 }
 
 }  // namespace cpk

@@ -196,7 +196,7 @@ int cp_weighted_err(int t, const uint8_t* raw, const float* x, const float* w, i
   if (int rc = check_shape(t, nrow, n, false, true)) return rc;
   if (!out || ((!raw || !x) && nrow > 0)) return set_err(CP_ERR_ARG, "null pointer");
   if (t == cpk::kMXFP4) {
-    if ((uintptr_t)raw & 15) return set_err(CP_ERR_ARG, "raw must be 16-byte aligned");
+    if (((uintptr_t)raw | (uintptr_t)x | (uintptr_t)w) & 15) return set_err(CP_ERR_ARG, "raw, x and w must be 16-byte aligned");
     if (cudaMemsetAsync(out, 0, sizeof(double), (cudaStream_t)stream) != cudaSuccess) return check_launch("cp_weighted_err");
     return check_rc(cpk::launch_mx4_weighted_err(raw, x, w, nrow, n, out, (cudaStream_t)stream), "cp_weighted_err");
   }
@@ -401,7 +401,7 @@ static int block_batch(int op, const cp_block_job* jobs, int count, void* stream
     if (int rc = check_shape(j.ggml_type, j.nrow, j.n, false, op == 2)) return rc;
     if (j.nrow == 0) continue;
     if (j.ggml_type == cpk::kMXFP4) {
-      if (!j.raw || !j.x || !j.err || ((uintptr_t)j.raw & 15))
+      if (!j.raw || !j.x || !j.err || (((uintptr_t)j.raw | (uintptr_t)j.x | (uintptr_t)j.w) & 15))
         return set_err(CP_ERR_ARG, "null or unaligned pointer in a block job");
       ProfScope ps(kProfOther, s);
       if (int rc = check_rc(cpk::launch_mx4_weighted_err(j.raw, j.x, j.w, j.nrow, j.n, j.err, s), what)) return rc;

@@ -103,32 +103,38 @@ template <int FMT> __device__ __forceinline__ MxStep mx_step(int byte, float tim
   return st;
 }
 
-// Codes of H pairs of values against a block's step, eight to a word.
+// A pair of values over a block's step, moved so that rounding to e2m1 gives what the exact quotient
+// would.
 //   MXFP4: v / 2^e is exact, so the conversion's rounding is the only one.
 //   NVFP4: v / s is not.  t is a multiple of 1/4 next to the approximate quotient, and every border
 //   between two e2m1 values is such a multiple.  t s is exact (t has at most 5 bits where a border can
 //   lie, s has 4) and r = v - t s has the right sign, so t + 1.9 r / s, which stays within a quarter of
 //   t, is on the side of t that v is on, and is t itself on a tie.  Quotients past 2^21, which only a
 //   saturated scale leaves, lose the quarter but not that they saturate.
+template <int FMT> __device__ __forceinline__ float2 mx_quotient(float2 v, const MxStep& st) {
+  const float2 inv = make_float2(st.inv, st.inv);
+  if (FMT == kMXFP4) return __fmul2_rn(v, inv);
+  constexpr float kQuarter = 3145728.0f;   // 1.5 * 2^21: adding it rounds to a multiple of 1/4
+  const float2 t = __fadd2_rn(__ffma2_rn(v, inv, make_float2(kQuarter, kQuarter)), make_float2(-kQuarter, -kQuarter));
+  const float2 r = __ffma2_rn(t, make_float2(-st.s, -st.s), v);
+  return __ffma2_rn(r, make_float2(1.9f * st.inv, 1.9f * st.inv), t);
+}
+// Codes of H pairs of values against a block's step, eight to a word.
 template <int FMT, int H>
 __device__ __forceinline__ void mx_codes(const float2 (&v)[H], const MxStep& st, uint32_t (&code)[H / 4]) {
   float2 q[H];
-  const float2 inv = make_float2(st.inv, st.inv);
-  if (FMT == kMXFP4) {
 #pragma unroll
-    for (int i = 0; i < H; i++) q[i] = __fmul2_rn(v[i], inv);
-  } else {
-    constexpr float kQuarter = 3145728.0f;   // 1.5 * 2^21: adding it rounds to a multiple of 1/4
-    const float2 up = make_float2(kQuarter, kQuarter), down = make_float2(-kQuarter, -kQuarter);
-    const float2 ms = make_float2(-st.s, -st.s), slope = make_float2(1.9f * st.inv, 1.9f * st.inv);
-#pragma unroll
-    for (int i = 0; i < H; i++) {
-      const float2 t = __fadd2_rn(__ffma2_rn(v[i], inv, up), down);
-      q[i] = __ffma2_rn(__ffma2_rn(t, ms, v[i]), slope, t);
-    }
-  }
+  for (int i = 0; i < H; i++) q[i] = mx_quotient<FMT>(v[i], st);
 #pragma unroll
   for (int i = 0; i < H / 4; i++) code[i] = e2m1x8(q + 4 * i);
+}
+// A pair of quotients rounded to e2m1.
+__device__ __forceinline__ float2 e2m1_round(float2 q) {
+  uint32_t h;
+  asm("{\n\t.reg .b8 c;\n\tcvt.rn.satfinite.e2m1x2.f32 c, %2, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, c;\n\t}"
+      : "=r"(h)
+      : "f"(q.x), "f"(q.y));
+  return __half22float2(*reinterpret_cast<__half2*>(&h));
 }
 
 }  // namespace cpk

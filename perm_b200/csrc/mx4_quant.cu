@@ -100,18 +100,16 @@ __device__ __forceinline__ void quantize_block(float2 (&v)[H], uint32_t top, con
     const float unit = __uint_as_float((uint32_t)min(max(254 - (int)(m >> 23), 1), 253) << 23);
     const float times = __fmul_rn(tensor_scale, unit);
     float err[C];
-    uint32_t codes[C][H / 4];
 #pragma unroll
     for (int i = 0; i < H; i++) v[i] = __fmul2_rn(v[i], make_float2(unit, unit));
 #pragma unroll
     for (int c = 0; c < C; c++) {
       const MxStep st = mx_step<FMT>(mx_candidate<FMT>(first, c), times);
-      mx_codes<FMT, H>(v, st, codes[c]);
       const float2 ms = make_float2(-st.s, -st.s);
       float2 e = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int i = 0; i < H; i++) {
-        const float2 d = __ffma2_rn(e2m1x2_value(codes[c][i / 4] >> (8 * (i % 4))), ms, v[i]);
+        const float2 d = __ffma2_rn(e2m1_round(mx_quotient<FMT>(v[i], st)), ms, v[i]);
         e = __ffma2_rn(__fmul2_rn(w[i], d), d, e);
       }
       err[c] = block_sum<LANES>(e.x + e.y);
@@ -133,12 +131,10 @@ __device__ __forceinline__ void quantize_block(float2 (&v)[H], uint32_t top, con
 #pragma unroll 1
       for (int c = 0; c < C; c++) {
         const MxStep st = mx_step<FMT>(mx_candidate<FMT>(first, c), times);
-        uint32_t cw[H / 4];
-        mx_codes<FMT, H>(v, st, cw);
         double e = 0.0;
 #pragma unroll
         for (int i = 0; i < H; i++) {
-          const float2 q = e2m1x2_value(cw[i / 4] >> (8 * (i % 4)));
+          const float2 q = e2m1_round(mx_quotient<FMT>(v[i], st));
           const double d0 = (double)v[i].x - (double)q.x * (double)st.s, d1 = (double)v[i].y - (double)q.y * (double)st.s;
           e += (double)w[i].x * (d0 * d0);
           e += (double)w[i].y * (d1 * d1);
@@ -149,14 +145,8 @@ __device__ __forceinline__ void quantize_block(float2 (&v)[H], uint32_t top, con
       if (near) pick = pd;
     }
     if (first == 0 || !finite) pick = 0;   // scale byte 0 (an all but empty block) is not searched
-#pragma unroll
-    for (int i = 0; i < H / 4; i++) {
-      code[i] = codes[0][i];
-#pragma unroll
-      for (int c = 1; c < C; c++)
-        if (c == pick) code[i] = codes[c][i];
-    }
     if (pick > 0) byte = mx_candidate<FMT>(first, pick);
+    mx_codes<FMT, H>(v, mx_step<FMT>(byte, times), code);
   }
 #pragma unroll
   for (int i = 0; i < H / 4; i++) code[i] = finite ? code[i] : 0;
@@ -210,50 +200,56 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 
+// A lane takes 16 bytes of results at a time (8 or 4 values), so that a warp's stores are whole lines: two
+// neighbouring stores of 16 bytes per lane took 64 us for 14336 x 4096 float32.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(32 * kWarps)
     dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows, int64_t n,
                       float scale, int chunks, int64_t units, bool vec, T* __restrict__ out, int64_t ld) {
   const int64_t unit = blockIdx.x * (int64_t)kWarps + threadIdx.x / 32;
   if (unit >= units) return;
-  const int lane = threadIdx.x % 32;
+  constexpr int G = 16 / sizeof(T), B = mx_block<FMT>();
   const int64_t rl = unit / chunks;
   const int chunk = (int)(unit - rl * chunks);
   const int64_t row0 = (rl >> 5) * 128 + (rl & 31);
-  const int64_t col = (int64_t)chunk * 256 + lane * 8, left = n - col;
-  if (left <= 0) return;
-  constexpr int LB = mx_block<FMT>() / 8;
-  const int64_t groups = (int64_t)chunks * (256 / (32 * LB));
-  const int64_t g = (int64_t)chunk * (256 / (32 * LB)) + lane / (4 * LB);
-  const uint4 sw = __ldg(reinterpret_cast<const uint4*>(scales + ((row0 >> 7) * groups + g) * 512 + (row0 & 31) * 16));
-  const uint32_t sj[4] = {sw.x, sw.y, sw.z, sw.w};
-  uint32_t c[4];
+  const int64_t pitch = (int64_t)chunks * 128, groups = (int64_t)chunks * (64 / B);
 #pragma unroll
-  for (int j = 0; j < 4; j++)
-    c[j] = row0 + 32 * j < rows ? __ldg(reinterpret_cast<const uint32_t*>(
-                                      codes + (row0 + 32 * j) * (int64_t)chunks * 128 + chunk * 128 + lane * 4))
-                                : 0;
+  for (int k = 0; k < 8 / G; k++) {
+    const int at = k * (32 * G) + (threadIdx.x % 32) * G;   // in the chunk of 256 columns
+    const int64_t col = (int64_t)chunk * 256 + at, left = n - col;
+    if (left <= 0) return;
+    const uint4 sw = __ldg(reinterpret_cast<const uint4*>(
+        scales + ((row0 >> 7) * groups + (int64_t)chunk * (64 / B) + at / (4 * B)) * 512 + (row0 & 31) * 16));
+    const uint32_t sj[4] = {sw.x, sw.y, sw.z, sw.w};
+    uint32_t c[4];
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int64_t row = row0 + 32 * j;
-    if (row >= rows) break;
-    const float s = mx_scale_value<FMT>((sj[j] >> (8 * (lane / LB % 4))) & 0xFF);
-    T o[8];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float2 q = e2m1x2_value(c[j] >> (8 * i));
-      // q s is exact, so the tensor scale's product is the only rounding before the type's own
-      put(o + 2 * i, __fmul_rn(__fmul_rn(q.x, s), scale));
-      put(o + 2 * i + 1, __fmul_rn(__fmul_rn(q.y, s), scale));
+    for (int j = 0; j < 4; j++) {
+      const uint8_t* src = codes + (row0 + 32 * j) * pitch + col / 2;
+      c[j] = row0 + 32 * j >= rows ? 0
+             : G == 8              ? __ldg(reinterpret_cast<const uint32_t*>(src))
+                                   : __ldg(reinterpret_cast<const uint16_t*>(src));
     }
-    T* p = out + row * ld + col;
-    if (vec && left >= 8) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(o)[i];
-    } else {
+    for (int j = 0; j < 4; j++) {
+      const int64_t row = row0 + 32 * j;
+      if (row >= rows) break;
+      const float s = mx_scale_value<FMT>((sj[j] >> (8 * (at / B % 4))) & 0xFF);
+      T o[G];
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (i < left) p[i] = o[i];
+      for (int i = 0; i < G / 2; i++) {
+        const float2 q = e2m1x2_value(c[j] >> (8 * i));
+        // q s is exact, so the tensor scale's product is the only rounding before the type's own
+        put(o + 2 * i, __fmul_rn(__fmul_rn(q.x, s), scale));
+        put(o + 2 * i + 1, __fmul_rn(__fmul_rn(q.y, s), scale));
+      }
+      T* p = out + row * ld + col;
+      if (vec && left >= G) {
+        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < G; i++)
+          if (i < left) p[i] = o[i];
+      }
     }
   }
 }
@@ -276,6 +272,7 @@ __global__ void __launch_bounds__(256) encode_kernel(const float* __restrict__ x
   __shared__ __align__(16) uint8_t stage[kCtaBlocks * kBlkBytes];
   const int64_t b0 = (int64_t)blockIdx.x * kCtaBlocks;
   const int t = threadIdx.x, l4 = t & 3;
+  const uint32_t in_row = IMAT ? (uint32_t)(b0 % nb_row) : 0;   // the first block's place in its row
   float2 v[4][4];
   uint32_t top[4];
 #pragma unroll
@@ -288,7 +285,7 @@ __global__ void __launch_bounds__(256) encode_kernel(const float* __restrict__ x
     const int lb = p * 64 + (t >> 2);
     const int64_t b = b0 + lb;
     float2 w[4];
-    if constexpr (IMAT) load8(qw + (b % nb_row) * 32 + l4 * 8, b < nblk ? 8 : 0, true, w);
+    if constexpr (IMAT) load8(qw + (int64_t)((in_row + lb) % (uint32_t)nb_row) * 32 + l4 * 8, b < nblk ? 8 : 0, true, w);
     int byte;
     uint32_t code[1];
     quantize_block<kMXFP4, IMAT, 4>(v[p], top[p], w, 1.0f, 1.0f, byte, code);
@@ -323,30 +320,28 @@ __device__ __forceinline__ int load_blocks(const uint8_t* __restrict__ raw, int6
   return bytes / kBlkBytes;
 }
 
-// Values 8 l4 .. 8 l4 + 7 of a staged block.
-__device__ __forceinline__ void block_values(const uint8_t* blk, int l4, float (&v)[8]) {
-  const float s = e8m0_value(blk[0]);
-  const uint8_t* q = blk + 1 + (l4 & 1) * 8;
-  const int sh = l4 >= 2 ? 4 : 0;
-#pragma unroll
-  for (int i = 0; i < 8; i++) v[i] = __fmul_rn(e2m1x2_value((q[i] >> sh) & 15).x, s);
+// Values 4 l .. 4 l + 3 of staged block lb.  Its four bytes start anywhere, so they come out of two
+// aligned words.
+__device__ __forceinline__ float4 block_values(const uint8_t* stage, int lb, int l) {
+  const uint32_t at = lb * kBlkBytes + 1 + (l & 3) * 4;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(stage) + at / 4;
+  const uint32_t c = (__funnelshift_r(w[0], w[1], 8 * (at & 3)) >> (l >= 4 ? 4 : 0)) & 0x0F0F0F0Fu;
+  const uint32_t two = c | (c >> 4);   // bytes 0 and 2: codes 0, 1 and 2, 3
+  const float s = e8m0_value(stage[lb * kBlkBytes]);
+  const float2 a = e2m1x2_value(two), b = e2m1x2_value(two >> 16);
+  return make_float4(__fmul_rn(a.x, s), __fmul_rn(a.y, s), __fmul_rn(b.x, s), __fmul_rn(b.y, s));
 }
 
 __global__ void __launch_bounds__(256) decode_kernel(const uint8_t* __restrict__ raw, int64_t nblk,
                                                      float* __restrict__ out) {
-  __shared__ __align__(16) uint8_t stage[kCtaBlocks * kBlkBytes];
+  __shared__ __align__(16) uint8_t stage[kCtaBlocks * kBlkBytes + 16];
   const int64_t b0 = (int64_t)blockIdx.x * kCtaBlocks;
   const int n = load_blocks(raw, nblk, b0, stage);
   const int t = threadIdx.x;
 #pragma unroll
-  for (int p = 0; p < 4; p++) {
-    const int lb = p * 64 + (t >> 2);
-    if (lb >= n) break;
-    float v[8];
-    block_values(stage + lb * kBlkBytes, t & 3, v);
-    float4* dst = reinterpret_cast<float4*>(out + (b0 + lb) * 32 + (t & 3) * 8);
-    dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-    dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+  for (int p = 0; p < 8; p++) {
+    const int lb = p * 32 + (t >> 3);
+    if (lb < n) reinterpret_cast<float4*>(out + b0 * 32)[p * 256 + t] = block_values(stage, lb, t & 7);
   }
 }
 
@@ -354,23 +349,22 @@ __global__ void __launch_bounds__(256) decode_kernel(const uint8_t* __restrict__
 __global__ void __launch_bounds__(256) weighted_err_kernel(const uint8_t* __restrict__ raw, const float* __restrict__ x,
                                                            const float* __restrict__ w, int64_t nblk, int nb_row,
                                                            double* __restrict__ err) {
-  __shared__ __align__(16) uint8_t stage[kCtaBlocks * kBlkBytes];
+  __shared__ __align__(16) uint8_t stage[kCtaBlocks * kBlkBytes + 16];
   __shared__ double part[8];
   const int64_t b0 = (int64_t)blockIdx.x * kCtaBlocks;
   const int n = load_blocks(raw, nblk, b0, stage);
+  const uint32_t in_row = (uint32_t)(b0 % nb_row);
   const int t = threadIdx.x;
   double e = 0.0;
-  for (int p = 0; p < 4; p++) {
-    const int lb = p * 64 + (t >> 2);
+  for (int p = 0; p < 8; p++) {
+    const int lb = p * 32 + (t >> 3);
     if (lb >= n) break;
-    float v[8];
-    block_values(stage + lb * kBlkBytes, t & 3, v);
-    const int64_t b = b0 + lb;
-    for (int i = 0; i < 8; i++) {
-      const int k = (t & 3) * 8 + i;
-      const double d = (double)v[i] - (double)x[b * 32 + k];
-      e += d * d * (w ? (double)w[(b % nb_row) * 32 + k] : 1.0);
-    }
+    const float4 v = block_values(stage, lb, t & 7);
+    const float4 y = __ldg(reinterpret_cast<const float4*>(x + b0 * 32) + p * 256 + t);
+    const float4 g = w ? __ldg(reinterpret_cast<const float4*>(w + (int64_t)((in_row + lb) % (uint32_t)nb_row) * 32) + (t & 7))
+                       : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+    const double d[4] = {(double)v.x - y.x, (double)v.y - y.y, (double)v.z - y.z, (double)v.w - y.w};
+    e += d[0] * d[0] * g.x + d[1] * d[1] * g.y + d[2] * d[2] * g.z + d[3] * d[3] * g.w;
   }
   for (int o = 16; o; o >>= 1) e += __shfl_down_sync(0xffffffffu, e, o);
   if (t % 32 == 0) part[t / 32] = e;
@@ -410,7 +404,7 @@ template <typename T, int FMT, bool IMAT>
 int quantize_typed(const T* x, int64_t rows, int64_t n, int64_t ld, const float* qw, float scale, uint8_t* codes,
                    uint8_t* scales, cudaStream_t stream) {
   // 8192 x 4096 bf16 to MXFP4: 16.5 us with H = 8, 20.8 with 4; to NVFP4, whose rounding keeps more values in
-  // registers, 22 us with either.  The weighted search keeps several candidates' codes.
+  // registers, 22 us with either.
   constexpr int H = sizeof(T) == 2 && FMT == kMXFP4 && !IMAT ? 8 : 4;
   const int64_t pitch = (n + 255) / 256 * 256;
   const int chunks = (int)((pitch + 64 * H - 1) / (64 * H));

@@ -65,6 +65,12 @@ template <int FMT> __device__ __forceinline__ int mx_candidate(int first, int c)
   const int b = first + (FMT == kMXFP4 ? kMx[c < 3 ? c : 0] : kNv[c]);
   return min(max(b, 0), FMT == kMXFP4 ? 253 : 126);
 }
+// The step of candidate c (MXFP4: the first's, its double and its half; `first` is at least 1 there).
+template <int FMT> __device__ __forceinline__ MxStep candidate_step(const MxStep& st, int first, int c, float times) {
+  if (FMT == kNVFP4) return mx_step<FMT>(mx_candidate<FMT>(first, c), times);
+  const float k = c == 0 ? 1.0f : c == 1 ? 2.0f : 0.5f;
+  return MxStep{__fmul_rn(st.s, k), __fmul_rn(st.inv, 1.0f / k)};
+}
 
 // Sum over the lanes of a block.
 template <int LANES, typename T> __device__ __forceinline__ T block_sum(T e) {
@@ -100,11 +106,12 @@ __device__ __forceinline__ void quantize_block(float2 (&v)[H], uint32_t top, con
     const float unit = __uint_as_float((uint32_t)min(max(254 - (int)(m >> 23), 1), 253) << 23);
     const float times = __fmul_rn(tensor_scale, unit);
     float err[C];
+    const MxStep step0 = mx_step<FMT>(first, times);
 #pragma unroll
     for (int i = 0; i < H; i++) v[i] = __fmul2_rn(v[i], make_float2(unit, unit));
 #pragma unroll
     for (int c = 0; c < C; c++) {
-      const MxStep st = mx_step<FMT>(mx_candidate<FMT>(first, c), times);
+      const MxStep st = candidate_step<FMT>(step0, first, c, times);
       const float2 ms = make_float2(-st.s, -st.s);
       float2 e = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -130,7 +137,7 @@ __device__ __forceinline__ void quantize_block(float2 (&v)[H], uint32_t top, con
       int pd = 0;
 #pragma unroll 1
       for (int c = 0; c < C; c++) {
-        const MxStep st = mx_step<FMT>(mx_candidate<FMT>(first, c), times);
+        const MxStep st = candidate_step<FMT>(step0, first, c, times);
         double e = 0.0;
 #pragma unroll
         for (int i = 0; i < H; i++) {

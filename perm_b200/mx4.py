@@ -27,6 +27,7 @@ import torch
 from . import _native as nat
 
 BLOCK = {"MXFP4": 32, "NVFP4": 16}
+_ID = nat.MX4_ID
 _DTYPE = {torch.bfloat16: nat.CP_MX4_BF16, torch.float16: nat.CP_MX4_F16, torch.float32: nat.CP_MX4_F32}
 # A call on one token takes a few microseconds on the device, so the host's part is kept short: the
 # stream's address comes from torch directly (a Stream object costs more than the rest of the checks).
@@ -43,7 +44,7 @@ class Mx4Tensor:
     scales  uint8, tiles of 128 rows x 4 blocks, [ceil(rows/128), P/(4 block), 32, 4, 4]: entry
             [i, g, r, j, k] is the scale of row 128 i + 32 j + r, block 4 g + k; zero past n
     tensor_scale  a positive float that multiplies every value"""
-    __slots__ = ("codes", "scales", "fmt", "rows", "n", "tensor_scale", "dev")
+    __slots__ = ("fmt", "rows", "n", "tensor_scale", "dev", "_codes", "_scales", "_buf", "_cp", "_sp")
 
     def __init__(self, codes, scales, fmt, rows, n, tensor_scale=1.0):
         if fmt not in BLOCK:
@@ -58,8 +59,38 @@ class Mx4Tensor:
             raise ValueError("codes and scales must be on one device")
         if not (tensor_scale > 0.0 and math.isfinite(tensor_scale)):
             raise ValueError("tensor_scale must be positive and finite")
-        self.codes, self.scales, self.fmt, self.rows, self.n = codes, scales, fmt, rows, n
-        self.tensor_scale, self.dev = tensor_scale, codes.get_device()   # dev: CUDA device index, -1 on the host
+        self.fmt, self.rows, self.n, self.tensor_scale = fmt, rows, n, tensor_scale
+        self.dev = codes.get_device()   # CUDA device index, -1 on the host
+        self._codes, self._scales, self._buf = codes, scales, None
+        self._cp, self._sp = codes.data_ptr(), scales.data_ptr()
+
+    @classmethod
+    def _new(cls, like, fmt, rows, n, tensor_scale):
+        """An operand on like's device, not yet filled: one allocation, of which codes and scales are
+        views made when they are asked for."""
+        q = cls.__new__(cls)
+        pitch = (n + 255) // 256 * 128
+        at = (rows * pitch + 255) // 256 * 256
+        q._buf = like.new_empty((at + (rows + 127) // 128 * (256 // BLOCK[fmt]) * pitch,), dtype=torch.uint8)
+        q.fmt, q.rows, q.n, q.tensor_scale, q.dev = fmt, rows, n, tensor_scale, like.get_device()
+        q._codes = q._scales = None
+        q._cp = q._buf.data_ptr()
+        q._sp = q._cp + at
+        return q
+
+    @property
+    def codes(self):
+        if self._codes is None:
+            pitch = (self.n + 255) // 256 * 128
+            self._codes = self._buf[:self.rows * pitch].view(self.rows, pitch)
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            pitch = (self.n + 255) // 256 * 128
+            self._scales = self._buf[(self.rows * pitch + 255) // 256 * 256:].view(-1, pitch // (2 * BLOCK[self.fmt]), 32, 4, 4)
+        return self._scales
 
     @property
     def shape(self):
@@ -67,7 +98,7 @@ class Mx4Tensor:
 
     @property
     def device(self):
-        return self.codes.device
+        return (self._codes if self._buf is None else self._buf).device
 
     def __repr__(self):
         return f"Mx4Tensor({self.fmt}, [{self.rows}, {self.n}], tensor_scale={self.tensor_scale}, device={self.device})"
@@ -86,15 +117,6 @@ def _call(idx, fn, what, *args):
             rc = fn(*args, _raw_stream(idx))
     if rc:
         nat.check(rc, what)
-
-
-def _empty_operand(like, fmt, rows, n, tensor_scale):
-    q = Mx4Tensor.__new__(Mx4Tensor)
-    pitch = (n + 255) // 256 * 128
-    q.codes = like.new_empty((rows, pitch), dtype=torch.uint8)
-    q.scales = like.new_empty(((rows + 127) // 128, pitch // (2 * BLOCK[fmt]), 32, 4, 4), dtype=torch.uint8)
-    q.fmt, q.rows, q.n, q.tensor_scale, q.dev = fmt, rows, n, tensor_scale, like.get_device()
-    return q
 
 
 def tensor_scale_for(x):
@@ -126,9 +148,9 @@ def quantize(x, fmt, qw=None, tensor_scale=1.0):
         if qw.shape != (n,) or qw.device != x.device:
             raise ValueError(f"qw must hold {n} column weights on x's device")
         qw = qw.to(torch.float32).contiguous()
-    q = _empty_operand(x, fmt, rows, n, tensor_scale)
-    _call(q.dev, nat.lib().cp_mx4_quantize, "mx4.quantize", nat.MX4_ID[fmt], dt, x.data_ptr(), rows, n, x.stride(0),
-          None if qw is None else qw.data_ptr(), tensor_scale, q.codes.data_ptr(), q.scales.data_ptr())
+    q = Mx4Tensor._new(x, fmt, rows, n, tensor_scale)
+    _call(q.dev, nat.lib().cp_mx4_quantize, "mx4.quantize", _ID[fmt], dt, x.data_ptr(), rows, n, x.stride(0),
+          None if qw is None else qw.data_ptr(), tensor_scale, q._cp, q._sp)
     return q
 
 
@@ -139,9 +161,8 @@ def dequantize(q, dtype=torch.float32):
         raise ValueError("mx4.dequantize: dtype must be bf16, f16 or f32")
     if q.dev < 0:
         _refuse_host("mx4.dequantize")
-    out = q.codes.new_empty((q.rows, q.n), dtype=dtype)
-    _call(q.dev, nat.lib().cp_mx4_dequantize, "mx4.dequantize", nat.MX4_ID[q.fmt], q.codes.data_ptr(),
-          q.scales.data_ptr(), q.rows, q.n, q.tensor_scale, dt, out.data_ptr())
+    out = (q._buf if q._codes is None else q._codes).new_empty((q.rows, q.n), dtype=dtype)
+    _call(q.dev, nat.lib().cp_mx4_dequantize, "mx4.dequantize", _ID[q.fmt], q._cp, q._sp, q.rows, q.n, q.tensor_scale, dt, out.data_ptr())
     return out
 
 
@@ -154,9 +175,8 @@ def from_gguf(raw, n):
     if raw.dtype != torch.uint8 or raw.dim() != 2 or raw.shape[1] != n // 32 * 17:
         raise ValueError(f"raw must be uint8 [rows, {n // 32 * 17}]")
     raw = raw.contiguous()
-    q = _empty_operand(raw, "MXFP4", raw.shape[0], n, 1.0)
-    _call(q.dev, nat.lib().cp_mx4_from_gguf, "mx4.from_gguf", raw.data_ptr(), q.rows, n, q.codes.data_ptr(),
-          q.scales.data_ptr())
+    q = Mx4Tensor._new(raw, "MXFP4", raw.shape[0], n, 1.0)
+    _call(q.dev, nat.lib().cp_mx4_from_gguf, "mx4.from_gguf", raw.data_ptr(), q.rows, n, q._cp, q._sp)
     return q
 
 
@@ -171,9 +191,9 @@ def matmul(a, w, dtype=torch.bfloat16):
         raise ValueError("mx4.matmul: operands must be on one device")
     if a.dev < 0:
         _refuse_host("mx4.matmul")
-    y = a.codes.new_empty((a.rows, w.rows), dtype=dtype)
-    _call(a.dev, nat.lib().cp_mx4_matmul, "mx4.matmul", nat.MX4_ID[w.fmt], a.codes.data_ptr(), a.scales.data_ptr(),
-          a.rows, w.codes.data_ptr(), w.scales.data_ptr(), w.rows, w.n, a.tensor_scale * w.tensor_scale, dt, y.data_ptr())
+    y = (w._buf if w._codes is None else w._codes).new_empty((a.rows, w.rows), dtype=dtype)
+    _call(a.dev, nat.lib().cp_mx4_matmul, "mx4.matmul", _ID[w.fmt], a._cp, a._sp, a.rows, w._cp, w._sp, w.rows, w.n,
+          a.tensor_scale * w.tensor_scale, dt, y.data_ptr())
     return y
 
 
@@ -212,8 +232,8 @@ def _product(x, w, transpose, what):
             _workspace.clear()
         need = _workspace[key] = L.cp_mx4_linear_workspace_bytes(dt, p, T, ld, w.rows, w.n, transpose)
     ws = x.new_empty((need,), dtype=torch.uint8) if need else None
-    _call(dev, L.cp_mx4_linear, what, nat.MX4_ID[w.fmt], dt, p, T, ld, w.codes.data_ptr(), w.scales.data_ptr(),
-          w.rows, w.n, w.tensor_scale, transpose, y.data_ptr(), ws.data_ptr() if need else None, need)
+    _call(dev, L.cp_mx4_linear, what, _ID[w.fmt], dt, p, T, ld, w._cp, w._sp, w.rows, w.n, w.tensor_scale, transpose,
+          y.data_ptr(), ws.data_ptr() if need else None, need)
     return y
 
 
@@ -263,8 +283,9 @@ class Linear(torch.nn.Module):
         super().__init__()
         self.out_features, self.in_features = weight.shape
         self.fmt, self.tensor_scale = weight.fmt, weight.tensor_scale
-        self.register_buffer("codes", weight.codes)
-        self.register_buffer("scales", weight.scales)
+        # buffers of their own: a view would save and move with everything it shares its storage with
+        self.register_buffer("codes", weight.codes.clone())
+        self.register_buffer("scales", weight.scales.clone())
         self.bias = None if bias is None else torch.nn.Parameter(bias.detach().clone())
 
     @classmethod

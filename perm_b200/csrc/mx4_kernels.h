@@ -46,8 +46,9 @@ int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, int align
 
 // The first form for a few tokens (mx4_stream.cu), and whether it takes these sizes.
 bool mx4_stream_applies(int dtype, int64_t T, int64_t rows, int64_t n);
+size_t mx4_stream_workspace_bytes(int dtype, int64_t T, int64_t rows, int64_t n);
 int launch_mx4_stream(int dtype, const void* x, int64_t T, int64_t ld, int aligned, const Mx4View& w, float alpha, void* y,
-                      cudaStream_t stream);
+                      void* ws, cudaStream_t stream);
 
 // Status words of the products' bounded waits (read and cleared; synchronises the stream).
 int mx4_matmul_status(cudaStream_t stream, int* status);

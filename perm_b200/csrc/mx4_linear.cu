@@ -558,7 +558,7 @@ size_t parts_bytes(int dtype, int64_t T, int64_t K, int aligned) {
 }  // namespace
 
 size_t mx4_linear_workspace_bytes(int dtype, int64_t T, int64_t rows, int64_t n, int aligned, int transpose) {
-  if (!transpose && mx4_stream_applies(dtype, T, rows, n)) return 0;
+  if (!transpose && mx4_stream_applies(dtype, T, rows, n)) return mx4_stream_workspace_bytes(dtype, T, rows, n);
   return parts_bytes(dtype, T, transpose ? rows : n, aligned) +
          (use_dense(T) ? (size_t)rows * ((n + 7) / 8 * 8) * 2 : 0);
 }
@@ -567,7 +567,7 @@ int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, int align
                       int transpose, void* y, void* ws, cudaStream_t stream) {
   if (!bind_context()) return 6;
   if (!transpose && mx4_stream_applies(dtype, T, w.rows, w.n))
-    return launch_mx4_stream(dtype, x, T, ld, aligned, w, alpha, y, stream);
+    return launch_mx4_stream(dtype, x, T, ld, aligned, w, alpha, y, ws, stream);
   const int64_t K = transpose ? w.rows : w.n;
   const int parts = parts_of(dtype);
   XView xv{x, T, K, T == 1 ? parts_pitch(K) : ld};   // one row has no pitch of its own

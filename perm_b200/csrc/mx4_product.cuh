@@ -87,7 +87,7 @@ __device__ __forceinline__ void umma_bf16(uint32_t d, uint64_t ad, uint64_t bd, 
                  : "memory");
 }
 
-// Sums the cluster's partial tiles ([token][128 rows] float32 at the same place of every CTA's
+// Sums the partial tiles of a cluster of at most eight CTAs ([token][128 rows] float32 at the same place of every CTA's
 // shared memory) in rank order; this CTA takes its share of the tokens.
 __device__ __forceinline__ void join_partials(const void* part, int rank, int split, int cols, int64_t row0, int64_t t0,
                                               int64_t rows, float alpha, int dtype, void* y) {
@@ -96,8 +96,13 @@ __device__ __forceinline__ void join_partials(const void* part, int rank, int sp
   for (int i = threadIdx.x + c0 * 128; i < c1 * 128; i += blockDim.x) {
     const int64_t row = row0 + (i & 127);
     if (row >= rows) continue;
-    float v = 0.0f;
-    for (int p = 0; p < split; p++) v += ld_cluster_f32(peer_addr(at + 4 * i, p));
+    float w[8], v = 0.0f;   // all loads ahead of the sum
+#pragma unroll
+    for (int p = 0; p < 8; p++)
+      if (p < split) w[p] = ld_cluster_f32(peer_addr(at + 4 * i, p));
+#pragma unroll
+    for (int p = 0; p < 8; p++)
+      if (p < split) v += w[p];
     put_out(y, dtype, (t0 + (i >> 7)) * rows + row, alpha * v);
   }
 }
@@ -160,25 +165,37 @@ inline bool bf16_map(CUtensorMap* m, const void* p, int64_t rows, int64_t cols, 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Launches kernel K in clusters; 0, 4 (its shared memory was refused) or 6 (the launch was).
+// Launches kernel K in clusters; 0, 4 (its shared memory was refused) or 6 (the launch was).  early: it may
+// start before the launch ahead of it in the stream has finished (and waits for that itself).
 template <auto K, typename... A>
-inline int launch_cluster(int grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {
+inline int launch_cluster_after(bool early, int grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {
   if (!opt_in_smem<K>()) return 4;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid, 1, 1);
   cfg.blockDim = dim3((unsigned)threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)cluster;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (cluster > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = (unsigned)cluster;
+    at[n].val.clusterDim.y = 1;
+    at[n++].val.clusterDim.z = 1;
+  }
+  if (early) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  cfg.numAttrs = n;
   if (cudaLaunchKernelEx(&cfg, K, args...) != cudaSuccess) return 6;
   note_launch();
   return 0;
+}
+template <auto K, typename... A>
+inline int launch_cluster(int grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {
+  return launch_cluster_after<K>(false, grid, threads, smem, cluster, stream, args...);
 }
 
 // Reads and clears a translation unit's status word.

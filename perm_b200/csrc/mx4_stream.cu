@@ -19,10 +19,15 @@
 // exact unless it is below 2^-32 of the largest, and off by at most 2^-40 of the largest otherwise.
 // float32 values are the sum of two f16 parts, the second 2^11 times finer, to within 2^-23 of each value.
 //
+// Every row tile needs x converted.  Where that is a large part of the work a first kernel converts it once,
+// into the workspace; the product is launched so that it may start beside that kernel (programmatic
+// dependent launch), brings its first weights in and waits for it only before it reads x.
+//
 // A CTA holds 128 rows (16 for each of eight warps) and a slice of the columns; a cluster of up to eight
 // shares a row tile and joins the partial sums through distributed shared memory in rank order.  Codes
 // and scale tiles arrive by TMA in stages of 256 columns; x is converted into shared memory while the first
 // stages are in flight.  Two CTAs fit an SM, or three for up to 8 tokens.
+#include <type_traits>
 #include "mx4_product.cuh"
 
 namespace cpk {
@@ -45,6 +50,8 @@ struct StreamParams {
   int slice;            // columns of the widest slice (the pitch of the converted x)
   int groups;           // scale tiles per 128 rows
   int vec;              // x's rows start on 16-byte boundaries
+  const uint32_t* top;  // converted x: the rows' largest magnitudes
+  int64_t pitch;        // and its bytes per row
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t a, uint32_t (&r)[4]) {
@@ -141,7 +148,79 @@ template <typename S> __device__ __forceinline__ uint32_t top_x8(const uint8_t* 
   return m;
 }
 
-template <int FMT, int NB, typename S>
+// 2^(14 - e) for a largest magnitude (as bits) of exponent e, and its inverse.
+__device__ __forceinline__ float scale_up(uint32_t top) {
+  return __uint_as_float((uint32_t)min(268 - max((int)(top >> 23), 1), 247) << 23);
+}
+__device__ __forceinline__ float scale_down(uint32_t top) {
+  return __uint_as_float((uint32_t)max(max((int)(top >> 23), 1) - 14, 7) << 23);
+}
+// Eight values, scaled, as f16 parts at `at` (16 bytes each).
+template <typename S> __device__ __forceinline__ void write_x8(uint8_t* at, const float (&v)[8], float up) {
+  constexpr int P = Parts<S>::k;
+  uint32_t w[P][4];
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float a = v[e] * up, b = v[e + 1] * up;
+    const __half2 h = __floats2half2_rn(a, b);
+    w[0][e / 2] = *reinterpret_cast<const uint32_t*>(&h);
+    if (P == 2) {   // of an infinity or NaN the first part holds it all
+      const float2 f = __half22float2(h);
+      const float ra = fabsf(a) < 1e30f ? (a - f.x) * 2048.0f : 0.0f, rb = fabsf(b) < 1e30f ? (b - f.y) * 2048.0f : 0.0f;
+      const __half2 l = __floats2half2_rn(ra, rb);
+      w[P - 1][e / 2] = *reinterpret_cast<const uint32_t*>(&l);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < P; p++) reinterpret_cast<uint4*>(at)[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+}
+
+// One CTA per row of x: the row's largest magnitude, and the row as scaled f16 parts, [eight
+// columns][part], zero from K to the padded end.
+template <typename S>
+__global__ void __launch_bounds__(512) convert_kernel(const S* __restrict__ x, int64_t K, int64_t ld, int vec, int groups,
+                                                      uint8_t* __restrict__ out, uint32_t* __restrict__ top) {
+  __shared__ uint32_t most;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int t = blockIdx.x;
+  const S* row = x + t * ld;
+  auto load = [&](int c, float (&v)[8]) {
+    const int64_t left = K - (int64_t)c * 8;
+    if (vec && left >= 8) {
+      read_x8<S>(reinterpret_cast<const uint8_t*>(row + c * 8), v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = e < left ? as_f32(row[c * 8 + e]) : 0.0f;
+    }
+  };
+  if (threadIdx.x == 0) most = 0;
+  __syncthreads();
+  uint32_t m = 0;
+#pragma unroll 4
+  for (int c = threadIdx.x; c < groups; c += 512) {
+    float v[8];
+    load(c, v);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const uint32_t b = __float_as_uint(v[e]) & 0x7FFFFFFFu;
+      m = max(m, b < 0x7F800000u ? b : 0u);
+    }
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (threadIdx.x % 32 == 0) atomicMax(&most, m);
+  __syncthreads();
+  if (threadIdx.x == 0) top[t] = most;
+  const float up = scale_up(most);
+#pragma unroll 4
+  for (int c = threadIdx.x; c < groups; c += 512) {
+    float v[8];
+    load(c, v);
+    write_x8<S>(out + ((int64_t)t * groups + c) * (16 * Parts<S>::k), v, up);
+  }
+}
+
+// DONE: x is what convert_kernel left.
+template <int FMT, int NB, typename S, bool DONE>
 __global__ void __launch_bounds__(kThreads, NB == 1 ? 3 : 2)
     mx4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
                       const StreamParams prm, int split) {
@@ -214,53 +293,51 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 3 : 2)
     const int units = s_end - s_begin;   // a row's
     const int64_t k0 = (int64_t)s_begin * 256;
     Unit u(warp, units);
-    for (; u.t < T; u.next(kWarps, units)) {
-      const int c = u.c * 32 + lane;   // group of eight columns
-      const int64_t left = prm.K - k0 - (int64_t)c * 8;   // values of the row from here on
-      const S* src = static_cast<const S*>(prm.x) + u.t * prm.ld + k0 + c * 8;
-      uint8_t* dst = xs + u.t * xpitch + c * (16 * P);
-      if (prm.vec || left <= 0) {
+    if (DONE) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      if (threadIdx.x < T) top[threadIdx.x] = __ldcg(prm.top + threadIdx.x);
+      for (; u.t < T; u.next(kWarps, units)) {
+        const int c = u.c * 32 + lane;
+        const uint8_t* src = static_cast<const uint8_t*>(prm.x) + u.t * prm.pitch + (k0 / 8 + c) * (16 * P);
 #pragma unroll
-        for (int p = 0; p < P; p++) {
-          const int64_t bytes = (left - p * (8 / P)) * (int64_t)sizeof(S);
-          const uint32_t n = bytes >= 16 ? 16 : bytes > 0 ? (uint32_t)bytes : 0;   // the rest is zero
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst) + 16 * p),
-                       "l"(n ? src + p * (8 / P) : static_cast<const S*>(prm.x)), "r"(n)
+        for (int p = 0; p < P; p++)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(xs) + u.t * xpitch + (c * P + p) * 16),
+                       "l"(src + 16 * p)
                        : "memory");
-        }
-      } else {
+      }
+    } else {
+      for (; u.t < T; u.next(kWarps, units)) {
+        const int c = u.c * 32 + lane;   // group of eight columns
+        const int64_t left = prm.K - k0 - (int64_t)c * 8;   // values of the row from here on
+        const S* src = static_cast<const S*>(prm.x) + u.t * prm.ld + k0 + c * 8;
+        uint8_t* dst = xs + u.t * xpitch + c * (16 * P);
+        if (prm.vec || left <= 0) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) reinterpret_cast<S*>(dst)[e] = e < left ? src[e] : S(0.0f);
+          for (int p = 0; p < P; p++) {
+            const int64_t bytes = (left - p * (8 / P)) * (int64_t)sizeof(S);
+            const uint32_t n = bytes >= 16 ? 16 : bytes > 0 ? (uint32_t)bytes : 0;   // the rest is zero
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst) + 16 * p),
+                         "l"(n ? src + p * (8 / P) : static_cast<const S*>(prm.x)), "r"(n)
+                         : "memory");
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++) reinterpret_cast<S*>(dst)[e] = e < left ? src[e] : S(0.0f);
+        }
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (kScaled) {
+    if (kScaled && !DONE) {
       for (u = Unit(warp, units); u.t < T; u.next(kWarps, units)) {
         const uint32_t m = __reduce_max_sync(0xffffffffu, top_x8<S>(xs + u.t * xpitch + (u.c * 32 + lane) * (16 * P)));
         if (lane == 0) atomicMax(&top[u.t], m);
       }
       asm volatile("bar.sync 1, %0;" ::"r"(32 * kWarps) : "memory");
       for (u = Unit(warp, units); u.t < T; u.next(kWarps, units)) {
-        // 2^(14 - e) for a largest magnitude of exponent e
-        const float up = __uint_as_float((uint32_t)min(268 - max((int)(top[u.t] >> 23), 1), 247) << 23);
         uint8_t* at = xs + u.t * xpitch + (u.c * 32 + lane) * (16 * P);
         float v[8];
         read_x8<S>(at, v);
-        uint32_t w[P][4];
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float a = v[e] * up, b = v[e + 1] * up;
-          const __half2 h = __floats2half2_rn(a, b);
-          w[0][e / 2] = *reinterpret_cast<const uint32_t*>(&h);
-          if (P == 2) {   // of an infinity or NaN the first part holds it all
-            const float2 f = __half22float2(h);
-            const float ra = fabsf(a) < 1e30f ? (a - f.x) * 2048.0f : 0.0f, rb = fabsf(b) < 1e30f ? (b - f.y) * 2048.0f : 0.0f;
-            const __half2 l = __floats2half2_rn(ra, rb);
-            w[P - 1][e / 2] = *reinterpret_cast<const uint32_t*>(&l);
-          }
-        }
-#pragma unroll
-        for (int p = 0; p < P; p++) reinterpret_cast<uint4*>(at)[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+        write_x8<S>(at, v, scale_up(top[u.t]));
       }
     }
     asm volatile("bar.sync 1, %0;" ::"r"(32 * kWarps) : "memory");
@@ -272,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 3 : 2)
     for (int b = 0; b < NB; b++)
 #pragma unroll
       for (int e = 0; e < 2; e++)
-        down[b][e] = kScaled ? __uint_as_float((uint32_t)max(max((int)(top[8 * b + 2 * t4 + e] >> 23), 1) - 14, 7) << 23) : 1.0f;
+        down[b][e] = kScaled ? scale_down(top[8 * b + 2 * t4 + e]) : 1.0f;
     const uint32_t row_at = (16 * warp + (lane & 7)) * 128, x7 = lane & 7;
     const uint32_t srow = ((16 * warp + g) & 31) * 16 + ((16 * warp + g) >> 5) * 4;   // row g's scale word; row g + 8: + 128
     // tokens past the last read a row that is there; their results are not used
@@ -401,50 +478,75 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 3 : 2)
   }
 }
 
-template <int FMT, int NB, typename S>
-int launch_stream(StreamParams& p, const Mx4View& w, int split, cudaStream_t stream) {
+template <int FMT, int NB, typename S, bool DONE>
+int launch_tiles(StreamParams& p, const Mx4View& w, int split, cudaStream_t stream) {
   constexpr int kAtoms = FMT == kMXFP4 ? 2 : 4, kStage = 128 * 128 + kAtoms * 512;
   const int64_t pitch = mx4_pitch(w.n), wt = (w.rows + 127) / 128;
   CUtensorMap mw, ms;
   if (!codes_map(&mw, w.codes, pitch, w.rows, 128, 128) || !scales_map(&ms, w.scales, wt * p.groups, kAtoms)) return 5;
   const size_t smem = 1024 + (size_t)p.nst * kStage + (size_t)p.T * (p.slice * 2 * Parts<S>::k + 64) + 8 * NB * 4 +
                       16 * kMaxStages + 64;
-  return launch_cluster<mx4_stream_kernel<FMT, NB, S>>((int)wt * split, kThreads, smem, split, stream, mw, ms, p, split);
+  return launch_cluster_after<mx4_stream_kernel<FMT, NB, S, DONE>>(DONE, (int)wt * split, kThreads, smem, split, stream, mw,
+                                                                  ms, p, split);
 }
 
-template <int FMT, typename S>
-int launch_tokens(StreamParams& p, const Mx4View& w, int split, cudaStream_t stream) {
-  if (p.T <= 8) return launch_stream<FMT, 1, S>(p, w, split, stream);
-  return launch_stream<FMT, 2, S>(p, w, split, stream);
-}
-
-}  // namespace
-
-namespace {
 struct StreamPlan {
   int split, nst, slice;
+  bool convert;         // x is converted by a kernel of its own
 };
-// False where x's slices would not leave room in shared memory.
+// False where the kernel does not take these sizes: more tokens than it is good for (MXFP4, bf16, here / decoded
+// to bf16 for tcgen05: 4096 -> 14336 with 16 tokens 18 / 23 us, with 24 tokens 33 / 23 us), or slices of x
+// that would leave no room in shared memory.
 bool stream_plan(int dtype, int64_t T, int64_t rows, int64_t n, StreamPlan* plan) {
   if (T > 16) return false;
+  const int64_t wt = (rows + 127) / 128;
+  // The converting kernel costs a launch.  4096 -> 14336, bf16, with it / without: 4 tokens 12.0 / 12.3 us, 8
+  // tokens 12.7 / 14.7, 16 tokens 18 / 24; 4096 -> 4096 with 8 tokens 7.2 / 7.0.
+  const bool convert = dtype != kMxF16 && T * n * wt > 2000000;
   const int parts = dtype == kMxF32 ? 2 : 1;
-  const int64_t wt = (rows + 127) / 128, slots = (int64_t)device_sm_count() * (T <= 8 ? 3 : 2);
+  const int most = T <= 8 ? 3 : 2;   // CTAs to an SM, by registers
+  const int64_t slots = (int64_t)device_sm_count() * most;
   const int steps = (int)(mx4_pitch(n) / 128), stage = 128 * 128 + 4 * 512;   // NVFP4's; MXFP4's is smaller
   int split = 1;
   while (split < 8 && wt * split * 2 <= slots && split * 2 <= steps) split *= 2;
-  // x's slice stays in shared memory beside at least three stages
+  // x's slice stays in shared memory beside at least two stages
   auto x_bytes = [&](int sp) { return T * ((int64_t)(steps + sp - 1) / sp * 512 * parts + 64); };
   const int64_t room = 222 * 1024;
-  while (split < 8 && split * 2 <= steps && x_bytes(split) + 3 * stage > room) split *= 2;
-  if (x_bytes(split) + 3 * stage > room) return false;
-  // as many CTAs to an SM as the split counts on, where that leaves each three stages
+  while (split < 8 && split * 2 <= steps && x_bytes(split) + 2 * stage > room / most) split *= 2;
+  if (x_bytes(split) + 2 * stage > (T <= 8 ? room : room / 2)) return false;
+  // as many CTAs to an SM as leaves each two stages
   const int mine = (steps + split - 1) / split;
   int nst = 0;
-  for (int ctas = T <= 8 ? 3 : 2; ctas > 0 && nst < std::min(3, mine); ctas--)
+  for (int ctas = most; ctas > 0 && nst < std::min(2, mine); ctas--)
     nst = (int)((room / ctas - 2048 - x_bytes(split)) / stage);
-  *plan = StreamPlan{split, std::min(std::min(nst, kMaxStages), mine), mine * 256};
+  *plan = StreamPlan{split, std::min(std::min(nst, kMaxStages), mine), mine * 256, convert};
   return true;
 }
+
+template <int FMT, typename S, bool DONE>
+int launch_tokens(StreamParams& p, const Mx4View& w, int split, cudaStream_t stream) {
+  if (p.T <= 8) return launch_tiles<FMT, 1, S, DONE>(p, w, split, stream);
+  return launch_tiles<FMT, 2, S, DONE>(p, w, split, stream);
+}
+
+template <int FMT, typename S>
+int launch_type(StreamParams& p, const Mx4View& w, int split, bool convert, void* ws, cudaStream_t stream) {
+  if constexpr (Parts<S>::scaled) {
+    if (convert) {
+      const int groups = p.steps * 32;
+      p.pitch = (int64_t)groups * 16 * Parts<S>::k;
+      uint8_t* out = static_cast<uint8_t*>(ws);
+      uint32_t* top = reinterpret_cast<uint32_t*>(out + p.T * p.pitch);
+      convert_kernel<S><<<(unsigned)p.T, 512, 0, stream>>>(static_cast<const S*>(p.x), p.K, p.ld, p.vec, groups, out, top);
+      note_launch();
+      p.x = out;
+      p.top = top;
+      return launch_tokens<FMT, S, true>(p, w, split, stream);
+    }
+  }
+  return launch_tokens<FMT, S, false>(p, w, split, stream);
+}
+
 }  // namespace
 
 bool mx4_stream_applies(int dtype, int64_t T, int64_t rows, int64_t n) {
@@ -452,12 +554,18 @@ bool mx4_stream_applies(int dtype, int64_t T, int64_t rows, int64_t n) {
   return stream_plan(dtype, T, rows, n, &plan);
 }
 
+size_t mx4_stream_workspace_bytes(int dtype, int64_t T, int64_t rows, int64_t n) {
+  StreamPlan plan;
+  if (!stream_plan(dtype, T, rows, n, &plan) || !plan.convert) return 0;
+  return (size_t)T * (mx4_pitch(n) / 128 * 32 * 16 * (dtype == kMxF32 ? 2 : 1) + 4);
+}
+
 int launch_mx4_stream(int dtype, const void* x, int64_t T, int64_t ld, int aligned, const Mx4View& w, float alpha, void* y,
-                      cudaStream_t stream) {
+                      void* ws, cudaStream_t stream) {
   StreamPlan plan;
   if (!stream_plan(dtype, T, w.rows, w.n, &plan)) return 6;
-  const int steps = (int)(mx4_pitch(w.n) / 128), split = plan.split;
-  StreamParams p;
+  const int steps = (int)(mx4_pitch(w.n) / 128);
+  StreamParams p = {};
   p.x = x;
   p.y = y;
   p.T = T;
@@ -472,13 +580,13 @@ int launch_mx4_stream(int dtype, const void* x, int64_t T, int64_t ld, int align
   p.groups = steps * (w.fmt == kMXFP4 ? 2 : 4);
   p.vec = aligned;
   if (w.fmt == kMXFP4) {
-    if (dtype == kMxBF16) return launch_tokens<kMXFP4, __nv_bfloat16>(p, w, split, stream);
-    if (dtype == kMxF16) return launch_tokens<kMXFP4, __half>(p, w, split, stream);
-    return launch_tokens<kMXFP4, float>(p, w, split, stream);
+    if (dtype == kMxBF16) return launch_type<kMXFP4, __nv_bfloat16>(p, w, plan.split, plan.convert, ws, stream);
+    if (dtype == kMxF16) return launch_type<kMXFP4, __half>(p, w, plan.split, plan.convert, ws, stream);
+    return launch_type<kMXFP4, float>(p, w, plan.split, plan.convert, ws, stream);
   }
-  if (dtype == kMxBF16) return launch_tokens<kNVFP4, __nv_bfloat16>(p, w, split, stream);
-  if (dtype == kMxF16) return launch_tokens<kNVFP4, __half>(p, w, split, stream);
-  return launch_tokens<kNVFP4, float>(p, w, split, stream);
+  if (dtype == kMxBF16) return launch_type<kNVFP4, __nv_bfloat16>(p, w, plan.split, plan.convert, ws, stream);
+  if (dtype == kMxF16) return launch_type<kNVFP4, __half>(p, w, plan.split, plan.convert, ws, stream);
+  return launch_type<kNVFP4, float>(p, w, plan.split, plan.convert, ws, stream);
 }
 
 int mx4_stream_status(cudaStream_t stream, int* status) { return read_status_word(g_status, stream, status); }

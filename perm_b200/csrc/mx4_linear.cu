@@ -503,14 +503,23 @@ int launch_form(const XView& x, int parts, int64_t T, const Mx4View& w, float al
   const int sms = device_sm_count();
   const int64_t mt = ((TR ? w.n : w.rows) + 127) / 128;
   const int steps = (int)((x.K + 127) / 128);
-  const bool chunk = dtype == kMxF32;
-  const int nt = chunk ? 64 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
-  const int64_t tiles = mt * ((T + nt - 1) / nt), pairs = (mt + 1) / 2 * ((T + 255) / 256);
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= sms && split * 2 <= steps) split *= 2;
-  if (chunk) return launch_tiles<FMT, 64, false, TR, true>(x, parts, T, w, alpha, dtype, y, split, stream);
-  const double one = (double)((tiles + sms - 1) / sms) / split, pair = 1.6 * (double)((pairs + sms / 2 - 1) / (sms / 2));
-  if (T > 128 && pair <= one) return launch_tiles<FMT, 256, true, TR, false>(x, parts, T, w, alpha, dtype, y, 1, stream);
+  // 128-deep steps take about 1350 clocks, the decoding's, for any of these tile widths, and 1750 in a pair
+  if (dtype == kMxF32) {
+    double clocks;
+    const int split = best_split(mt * ((T + 63) / 64), steps, 1350, 64, sms, &clocks);
+    return launch_tiles<FMT, 64, false, TR, true>(x, parts, T, w, alpha, dtype, y, split, stream);
+  }
+  int nt = 0, split = 1;
+  double best = 0;
+  for (int n = 32; n <= 128; n *= 2) {
+    double clocks;
+    const int s = best_split(mt * ((T + n - 1) / n), steps, 1350, n, sms, &clocks);
+    if (nt == 0 || clocks < best) nt = n, split = s, best = clocks;
+    if (n >= T) break;
+  }
+  const int64_t pairs = (mt + 1) / 2 * ((T + 255) / 256);
+  if (T > 128 && (double)((pairs + sms / 2 - 1) / (sms / 2)) * steps * 1750 + 3500 <= best)
+    return launch_tiles<FMT, 256, true, TR, false>(x, parts, T, w, alpha, dtype, y, 1, stream);
   switch (nt) {
     case 32: return launch_tiles<FMT, 32, false, TR, false>(x, parts, T, w, alpha, dtype, y, split, stream);
     case 64: return launch_tiles<FMT, 64, false, TR, false>(x, parts, T, w, alpha, dtype, y, split, stream);

@@ -311,11 +311,11 @@ int launch_format(const Mx4View& a, const Mx4View& w, float alpha, int dtype, vo
   const int nt = T <= 32 ? 32 : T <= 64 ? 64 : 128;
   const int64_t tiles = mt * ((T + nt - 1) / nt);
   const int64_t pairs = (mt + 1) / 2 * ((T + 255) / 256);
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= sms && split * 2 <= steps) split *= 2;
-  // In rounds of one-SM 128 x 128 tiles: a pair's tile takes as long as 1.6 of them.
-  const double one = (double)((tiles + sms - 1) / sms) / split, pair = 1.6 * (double)((pairs + sms / 2 - 1) / (sms / 2));
-  if (T > 128 && pair <= one) return launch_tiles<FMT, 256, true>(a, w, alpha, dtype, y, 1, stream);
+  // 256-column steps take about 600 clocks in a one-SM tile, and in a pair's, of four times the work, 700
+  double one;
+  const int split = best_split(tiles, steps, 600, nt, sms, &one);
+  if (T > 128 && (double)((pairs + sms / 2 - 1) / (sms / 2)) * steps * 700 + 3500 <= one)
+    return launch_tiles<FMT, 256, true>(a, w, alpha, dtype, y, 1, stream);
   switch (nt) {
     case 32: return launch_tiles<FMT, 32, false>(a, w, alpha, dtype, y, split, stream);
     case 64: return launch_tiles<FMT, 64, false>(a, w, alpha, dtype, y, split, stream);

@@ -87,24 +87,60 @@ __device__ __forceinline__ void umma_bf16(uint32_t d, uint64_t ad, uint64_t bd, 
                  : "memory");
 }
 
-// Sums the partial tiles of a cluster of at most eight CTAs ([token][128 rows] float32 at the same place of every CTA's
-// shared memory) in rank order; this CTA takes its share of the tokens.
+// Sums the partial tiles of a cluster of at most eight CTAs ([token][128 rows] float32 at the same place of
+// every CTA's shared memory) in rank order; this CTA takes its share of the tokens, a thread four rows
+// at a time: the loads across the cluster are what this costs.
 __device__ __forceinline__ void join_partials(const void* part, int rank, int split, int cols, int64_t row0, int64_t t0,
                                               int64_t rows, float alpha, int dtype, void* y) {
   const int c0 = cols * rank / split, c1 = cols * (rank + 1) / split;
   const uint32_t at = smem_u32(part);
-  for (int i = threadIdx.x + c0 * 128; i < c1 * 128; i += blockDim.x) {
-    const int64_t row = row0 + (i & 127);
+  const int size = dtype == kMxF32 ? 4 : 2;
+  const bool four = rows % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & (4 * size - 1)) == 0;
+  for (int i = threadIdx.x + c0 * 32; i < c1 * 32; i += blockDim.x) {
+    const int64_t row = row0 + (i & 31) * 4;
     if (row >= rows) continue;
-    float w[8], v = 0.0f;   // all loads ahead of the sum
+    float4 w[8], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // all loads ahead of the sum
 #pragma unroll
     for (int p = 0; p < 8; p++)
-      if (p < split) w[p] = ld_cluster_f32(peer_addr(at + 4 * i, p));
+      if (p < split) w[p] = ld_cluster_f32x4(peer_addr(at + 16 * i, p));
 #pragma unroll
     for (int p = 0; p < 8; p++)
-      if (p < split) v += w[p];
-    put_out(y, dtype, (t0 + (i >> 7)) * rows + row, alpha * v);
+      if (p < split) v.x += w[p].x, v.y += w[p].y, v.z += w[p].z, v.w += w[p].w;
+    v = make_float4(alpha * v.x, alpha * v.y, alpha * v.z, alpha * v.w);
+    const int64_t to = (t0 + (i >> 5)) * rows + row;
+    if (four) {
+      if (dtype == kMxF32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(y) + to) = v;
+      } else {
+        uint2 o;
+        if (dtype == kMxBF16) {
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o.x) : "f"(v.y), "f"(v.x));
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o.y) : "f"(v.w), "f"(v.z));
+        } else {
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(o.x) : "f"(v.y), "f"(v.x));
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(o.y) : "f"(v.w), "f"(v.z));
+        }
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(y) + to) = o;
+      }
+    } else {
+      const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (row + k < rows) put_out(y, dtype, to + k, e[k]);
+    }
   }
+}
+
+// The split of the reduction (1, 2, 4 or 8 CTAs to a tile) with the shortest estimate, in clocks: rounds of
+// `tiles` x split CTAs over the SMs, each its share of `steps`, the join of a partial tile of nt tokens
+// (measured 3600 to 5400 clocks for 128 tokens, 14 bytes a clock across the cluster) and the start.
+inline int best_split(int64_t tiles, int steps, double step, int nt, int sms, double* clocks) {
+  int best = 1;
+  for (int s = 1; s <= 8 && s <= steps; s *= 2) {
+    const double c = (double)((tiles * s + sms - 1) / sms) * ((steps + s - 1) / s * step + (s > 1 ? 1000 + 36.0 * nt : 0)) + 3500;
+    if (s == 1 || c < *clocks) *clocks = c, best = s;
+  }
+  return best;
 }
 
 // Lets a kernel use all of an SM's shared memory (launches ask for what they need), once per device.

@@ -157,12 +157,11 @@ __device__ __forceinline__ void fail_pair(volatile int* abort, uint32_t peer_abo
 __device__ __forceinline__ void umma_commit(uint32_t mbar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar) : "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t a) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
   return v;
 }
-
 // N accumulator columns of this warp's lanes into registers, one wait for all of them.
 template <int N> __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float (&v)[N]) {
   static_assert(N % 16 == 0, "loaded 16 columns at a time");

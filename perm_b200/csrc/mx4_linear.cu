@@ -528,9 +528,19 @@ int launch_form(const XView& x, int parts, int64_t T, const Mx4View& w, float al
 }
 
 // Whether the weights are decoded to the workspace first.  Measured, MXFP4, bf16, decoded first / in the
-// product: 4096 -> 4096 with 512 tokens 32 / 27 us, 1024 tokens 33 / 43, 4096 tokens 96 / 148;
+// product: 4096 -> 4096 with 512 tokens 32 / 27 us, 640 tokens 33 / 43, 4096 tokens 96 / 148;
 // 4096 -> 14336 with 256 tokens 57 / 43, 512 tokens 78 / 77, 4096 tokens 420 / 476.
-bool use_dense(int64_t T) { return T > 640; }
+bool use_dense(int64_t T) { return T > 544; }
+
+// The device address of this unit's status word (looked up once per device).
+int* status_word() {
+  static std::atomic<int*> at[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  int* p = at[dev].load();
+  if (!p && cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_status) == cudaSuccess) at[dev].store(p);
+  return p;
+}
 
 int launch_dense(const XView& x, int parts, int64_t T, const Mx4View& w, float alpha, int dtype, int transpose, void* y,
                  void* wbuf, cudaStream_t stream) {
@@ -540,7 +550,8 @@ int launch_dense(const XView& x, int parts, int64_t T, const Mx4View& w, float a
   if (!bf16_map(&mw, wbuf, w.rows, w.n, ld, transpose ? 64 : 128) || !bf16_map(&mx, x.p, x.rows, x.K, x.ld, 128)) return 5;
   dense::Params p;
   p.y = y;
-  if (cudaGetSymbolAddress((void**)&p.status, g_status) != cudaSuccess) return 6;
+  p.status = status_word();
+  if (!p.status) return 6;
   p.T = T;
   p.out = transpose ? w.n : w.rows;
   p.alpha = alpha;

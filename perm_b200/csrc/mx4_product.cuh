@@ -131,13 +131,19 @@ __device__ __forceinline__ void join_partials(const void* part, int rank, int sp
   }
 }
 
+// Clusters of `size` CTAs, one CTA to an SM, that fit the device at once: the SMs of a GPC do not divide evenly
+// (the occupancy query gives 74, 33 and 15 on a B200).
+inline int64_t cluster_slots(int size, int sms) {
+  return size == 8 ? sms * 15 / 148 : size == 4 ? sms * 33 / 148 : sms / size;
+}
 // The split of the reduction (1, 2, 4 or 8 CTAs to a tile) with the shortest estimate, in clocks: rounds of
-// `tiles` x split CTAs over the SMs, each its share of `steps`, the join of a partial tile of nt tokens
-// (measured 3600 to 5400 clocks for 128 tokens, 14 bytes a clock across the cluster) and the start.
+// `tiles` clusters, each CTA its share of `steps`, the join of a partial tile of nt tokens (measured 3600 to
+// 5400 clocks for 128 tokens, 14 bytes a clock across the cluster) and the start.
 inline int best_split(int64_t tiles, int steps, double step, int nt, int sms, double* clocks) {
   int best = 1;
   for (int s = 1; s <= 8 && s <= steps; s *= 2) {
-    const double c = (double)((tiles * s + sms - 1) / sms) * ((steps + s - 1) / s * step + (s > 1 ? 1000 + 36.0 * nt : 0)) + 3500;
+    const int64_t fit = cluster_slots(s, sms) > 0 ? cluster_slots(s, sms) : 1;
+    const double c = (double)((tiles + fit - 1) / fit) * ((steps + s - 1) / s * step + (s > 1 ? 1000 + 36.0 * nt : 0)) + 3500;
     if (s == 1 || c < *clocks) *clocks = c, best = s;
   }
   return best;

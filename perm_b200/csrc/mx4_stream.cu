@@ -505,10 +505,10 @@ bool stream_plan(int dtype, int64_t T, int64_t rows, int64_t n, StreamPlan* plan
   const bool convert = dtype != kMxF16 && T * n * wt > 2000000;
   const int parts = dtype == kMxF32 ? 2 : 1;
   const int most = T <= 8 ? 3 : 2;   // CTAs to an SM, by registers
-  const int64_t slots = (int64_t)device_sm_count() * most;
+  const int sms = device_sm_count();
   const int steps = (int)(mx4_pitch(n) / 128), stage = 128 * 128 + 4 * 512;   // NVFP4's; MXFP4's is smaller
   int split = 1;
-  while (split < 8 && wt * split * 2 <= slots && split * 2 <= steps) split *= 2;
+  while (split < 8 && wt <= most * cluster_slots(split * 2, sms) && split * 2 <= steps) split *= 2;
   // x's slice stays in shared memory beside at least two stages
   auto x_bytes = [&](int sp) { return T * ((int64_t)(steps + sp - 1) / sp * 512 * parts + 64); };
   const int64_t room = 222 * 1024;

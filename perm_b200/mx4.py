@@ -225,7 +225,7 @@ def _product(x, w, transpose, what):
         else:
             ld = x.stride(0)
     L, p = nat.lib(), x.data_ptr()
-    key = (dt, T, ld, w.rows, w.n, transpose, p & 15)
+    key = (dev, dt, T, ld, w.rows, w.n, transpose, p & 15)
     need = _workspace.get(key)
     if need is None:
         if len(_workspace) > 4096:

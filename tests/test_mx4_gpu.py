@@ -277,6 +277,84 @@ def test_linear_and_its_gradient(fmt, dtype, T, out, n):
     mx4.status()
 
 
+# every launch variant: few tokens with x converted ahead, SM pairs, and weights decoded first
+VARIANTS = [(16, 8200, 2048), (3, 14400, 4100), (130, 14336, 256), (512, 14340, 200), (600, 300, 200), (545, 1030, 530)]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,out,n", VARIANTS)
+def test_products_in_every_variant(fmt, dtype, T, out, n):
+    dt = DTYPES[dtype]
+    w, wv = operand(out, n, fmt, out + n)
+    x = make_x(T, n, T + out, dt, 0.5)
+    check_product(mx4.linear(x, w), f64(x), wv, dt)
+    dy = make_x(T, out, T * 3 + out, dt, 0.5)
+    check_product(mx4.linear_grad(dy, w), f64(dy), wv.T, dt)
+    a, av = operand(T, n, fmt, T + n, 2.0 ** -10 if fmt == "NVFP4" else 1.0)
+    check_product(mx4.matmul(a, w, dt), av, wv, dt)
+    mx4.status()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_variants_in_a_graph_on_another_stream(dtype):
+    dt = DTYPES[dtype]
+    w, wv = operand(8200, 2048, "MXFP4", 3)
+    xs = [make_x(T, 2048, T, dt, 0.5) for T in (16, 130, 600)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for x in xs:
+            mx4.linear_grad(mx4.linear(x, w), w)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            ys = [mx4.linear(x, w) for x in xs]
+            zs = [mx4.linear_grad(y, w) for y in ys]
+    side.synchronize()
+    for rep in range(2):
+        for x in xs:
+            x.copy_(make_x(x.shape[0], 2048, 70 + rep, dt, 0.5))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            g.replay()
+            g.replay()
+        side.synchronize()
+        for x, y, z in zip(xs, ys, zs):
+            check_product(y, f64(x), wv, dt)
+            check_product(z, f64(y), wv.T, dt)
+
+
+def test_gradient_from_a_thread_without_a_context():
+    """The first CUDA call of a thread that has made no context current is a product's launch."""
+    import threading
+    w, wv = operand(600, 256, "MXFP4", 4)
+    x = make_x(600, 256, 1, torch.bfloat16)
+    out = []
+    torch.cuda.synchronize()
+    t = threading.Thread(target=lambda: out.extend([mx4.linear(x[:40], w), mx4.linear(x, w), mx4.matmul(w, w, torch.float32)]))
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    check_product(out[0], f64(x[:40]), wv, torch.bfloat16)
+    check_product(out[1], f64(x), wv, torch.bfloat16)
+    check_product(out[2], wv, wv, torch.float32)
+
+
+@pytest.mark.parametrize("T", [40, 600])
+def test_undefined_scales_of_padding_rows(T):
+    """The scale bytes of rows past the last may hold anything: they reach no result."""
+    w, wv = operand(130, 200, "NVFP4", 5)
+    s = w.scales.clone()
+    rows = torch.arange(256, device="cuda").view(2, 4, 32).permute(0, 2, 1).view(2, 1, 32, 4, 1).expand_as(s)
+    s = torch.where(rows >= 130, torch.full_like(s, 0x7F), s).contiguous()
+    w2 = mx4.Mx4Tensor(w.codes, s, "NVFP4", 130, 200, w.tensor_scale)
+    x, dy = make_x(T, 200, 1, torch.bfloat16), make_x(T, 130, 2, torch.bfloat16)
+    check_product(mx4.linear(x, w2), f64(x), wv, torch.bfloat16)
+    check_product(mx4.linear_grad(dy, w2), f64(dy), wv.T, torch.bfloat16)
+    check_product(mx4.matmul(mx4.Mx4Tensor(w.codes, s, "NVFP4", 130, 200, w.tensor_scale), w2, torch.float32), wv, wv, torch.float32)
+    assert np.array_equal(f64(mx4.dequantize(w2)), wv)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T", [3, 150])
 def test_linear_strides_and_shapes(dtype, T):

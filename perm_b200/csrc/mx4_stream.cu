@@ -26,7 +26,7 @@
 // A CTA holds 128 rows (16 for each of eight warps) and a slice of the columns; a cluster of up to eight
 // shares a row tile and joins the partial sums through distributed shared memory in rank order.  Codes
 // and scale tiles arrive by TMA in stages of 256 columns; x is converted into shared memory while the first
-// stages are in flight.  Two CTAs fit an SM, or three for up to 8 tokens.
+// stages are in flight.  Two CTAs fit an SM.
 #include <type_traits>
 #include "mx4_product.cuh"
 
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(512) convert_kernel(const S* __restrict__ x, i
 
 // DONE: x is what convert_kernel left.
 template <int FMT, int NB, typename S, bool DONE>
-__global__ void __launch_bounds__(kThreads, NB == 1 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads, 2)
     mx4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
                       const StreamParams prm, int split) {
   constexpr int NTOK = 8 * NB, P = Parts<S>::k;
@@ -504,11 +504,12 @@ bool stream_plan(int dtype, int64_t T, int64_t rows, int64_t n, StreamPlan* plan
   // tokens 12.7 / 14.7, 16 tokens 18 / 24; 4096 -> 4096 with 8 tokens 7.2 / 7.0.
   const bool convert = dtype != kMxF16 && T * n * wt > 2000000;
   const int parts = dtype == kMxF32 ? 2 : 1;
-  const int most = T <= 8 ? 3 : 2;   // CTAs to an SM, by registers
+  const int most = 2;   // CTAs to an SM, by registers (three of fewer registers were 3 % slower for one token)
   const int sms = device_sm_count();
   const int steps = (int)(mx4_pitch(n) / 128), stage = 128 * 128 + 4 * 512;   // NVFP4's; MXFP4's is smaller
   int split = 1;
-  while (split < 8 && wt <= most * cluster_slots(split * 2, sms) && split * 2 <= steps) split *= 2;
+  // one and a half rounds of shorter CTAs beat one of longer ones (14336 -> 4096, one token: 9.7 / 10.9 us)
+  while (split < 8 && wt <= 3 * most / 2 * cluster_slots(split * 2, sms) && split * 2 <= steps) split *= 2;
   // x's slice stays in shared memory beside at least two stages
   auto x_bytes = [&](int sp) { return T * ((int64_t)(steps + sp - 1) / sp * 512 * parts + 64); };
   const int64_t room = 222 * 1024;

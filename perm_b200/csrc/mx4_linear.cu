@@ -9,10 +9,10 @@
 // x w^T, MN-major for x w, where the packed axis is the output's.  Both are the same bytes: two
 // halves of 64 columns, 128 bytes a row.  Weights are the M side (128 rows of the output per CTA), tokens the N side.
 //
-// Decoding.  cvt turns two codes into two f16 values; f16 holds an e2m1 value in the sign and the
-// top six bits, and the same bits three places lower are the bf16 of the value times 2^-112.  One
-// bf16 product with 2^112 times the block scale makes it whole: five instructions for two
-// weights.  MXFP4 scales above 2^15, where that factor would overflow, take a second product.
+// Decoding.  A conversion turns two codes into two f16 values; widened to float32 they take the block
+// scale, exactly, and go back as a pair of bf16.  (Shifting the f16 bits into a bf16 with another exponent
+// and one bf16 product takes an instruction less, but three of its five are for the pipe that the
+// conversions use too: 4 to 10 % slower.)
 //
 // float16 and float32 activations are cut into bf16 parts (8 significant bits each: two for float16,
 // three for float32, no remainder) by a first kernel, and every decoded weight tile is multiplied
@@ -37,8 +37,10 @@ constexpr int kChunkSteps = 1;  // 128-deep steps of one float32 accumulation ch
 
 template <int FMT, int NT, bool PAIR, bool TR, bool CHUNK> struct Cfg {
   // warps: 0 x loads, 1 MMA, 2 code loads, 3 allocation, 4-7 epilogue, then groups of eight that decode
-  // alternate steps.  float32 results keep NT sums per epilogue thread, which leaves registers for one group.
-  static constexpr int kGroups = CHUNK ? 1 : 2;
+  // steps in turn.  float32 results keep NT sums per epilogue thread, which leaves registers for one group.
+  // A pair has the registers for a third group (512 x 4096 -> 14336: 70 us with two, 61 with three); one-SM
+  // tiles were no faster with it.
+  static constexpr int kGroups = CHUNK ? 1 : PAIR ? 3 : 2;
   static constexpr int kThreads = 256 + 256 * kGroups;
   static constexpr int kXRows = PAIR ? NT / 2 : NT;
   static constexpr int kA = 128 * 256;                     // decoded tile: 128 rows x 128, bf16
@@ -46,13 +48,12 @@ template <int FMT, int NT, bool PAIR, bool TR, bool CHUNK> struct Cfg {
   static constexpr int kAtoms = FMT == kMXFP4 ? 1 : 2;     // scale tiles of 128 x 128 codes
   static constexpr int kCodes = 128 * 64;
   static constexpr int kC = (kCodes + kAtoms * 512 + 1023) / 1024 * 1024;
-  // code stages: as many as the largest number of groups, so that one group sees every use of a stage
-  // (a group that saw every other use could take one phase of its barrier for another)
-  static constexpr int kCS = 2, kMaxStages = 6;
+  // code stages at most; see LinParams::turns
+  static constexpr int kCS = PAIR ? 3 : 2, kMaxStages = 6;
   static constexpr int kRing = (225 * 1024 - kCS * kC) / 1024 * 1024;   // stages of one decoded tile and its x tiles
   static constexpr size_t kSmem = 1024 + (size_t)kRing + kCS * kC + 512;
   static constexpr uint32_t kTmem = 2 * NT < 64 ? 64 : 2 * NT;
-  static_assert(kCS % kGroups == 0, "one group per code stage");
+  static_assert(kCS % kGroups == 0, "code stages for every group");
   static_assert(kB % 1024 == 0 && kRing >= NT * 512, "stages keep the swizzle's alignment, and a partial tile fits");
   // f32 accumulator, A and B bf16, A MN-major in the transposed form, N >> 3, M >> 4
   static constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((TR ? 1u : 0u) << 15) |
@@ -67,39 +68,29 @@ struct LinParams {
   int dtype;
   int parts;
   int nst;              // stages of the ring
+  // The groups that decode, and the code stages.  A wait for a phase of a barrier is answered by its parity, so it
+  // must not come before the phase ahead of the one meant is known to be over.  The ring's stages: a group that
+  // decodes step s waits for the MMAs of s - nst, and has seen those of s - turns - nst complete; the phase
+  // ahead is that of s - 2 nst, so turns <= nst.  The code stages: their number is a multiple of turns,
+  // so that one group sees every use of a stage.
+  int turns, ncs;
   int steps;            // 128-deep steps of the reduction
   int groups;           // scale tiles per 128 rows of w
   int mtiles, tiles;
 };
 
-// bf16 (twice) of 2^112 times a block scale; `more` is a further factor, 1 unless the first would
-// overflow.
-__device__ __forceinline__ uint32_t twice(uint32_t b) { return b | (b << 16); }
-__device__ __forceinline__ uint32_t factor_e8m0(uint32_t byte, uint32_t& more) {
-  more = 0;
-  if (byte > 142) {
-    more = byte == 255 ? twice(0x7FC0) : twice((byte - 142 + 127) << 7);   // byte 254: 2^112, the field's 239
-    byte = 142;
-  }
-  return twice((byte + 112) << 7);
-}
-__device__ __forceinline__ uint32_t factor_e4m3(uint32_t byte) {
-  return twice(__float_as_uint(e4m3_value(byte) * 5.192296858534827628530496329220096e33f) >> 16);   // 2^112; 0x7F stays NaN
-}
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-// Eight codes -> eight bf16 values times 2^-112, in pairs.
-__device__ __forceinline__ void decode8(uint32_t w, uint32_t (&v)[4]) {
+// Eight codes times a block scale -> eight bf16 values in pairs.
+__device__ __forceinline__ void decode8(uint32_t w, float scale, uint32_t (&v)[4]) {
   asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
       "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
       "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
       : "r"(w));
 #pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = ((v[i] >> 3) & 0x0FC00FC0u) | (v[i] & 0x80008000u);
+  for (int i = 0; i < 4; i++) {
+    const float2 f = __fmul2_rn(__half22float2(*reinterpret_cast<const __half2*>(&v[i])), make_float2(scale, scale));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v[i]) : "f"(f.y), "f"(f.x));
+  }
 }
 
 template <int FMT, int NT, bool PAIR, bool TR, bool CHUNK>
@@ -197,13 +188,14 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
     }
   } else if (warp == 2) {
     if (lane == 0) {   // ---- codes and scales of this CTA's rows
+      Ring rc{0, 0};
       int it = 0;
       bool ok = true;
       for (int tile = first; ok && tile < prm.tiles; tile += stride) {
         const int m0 = (int)tile_row(tile);
-        for (int s = s_begin; s < s_end; s++, it++) {
-          const int st = it % C::kCS, round = it / C::kCS;
-          if (round > 0 && !mbar_wait(cempty + 8 * st, (round - 1) & 1, abort, kWaitNs)) {
+        for (int s = s_begin; s < s_end; s++, it++, rc.advance(prm.ncs)) {
+          const int st = rc.st;
+          if (it >= prm.ncs && !mbar_wait(cempty + 8 * st, rc.ph ^ 1, abort, kWaitNs)) {
             ok = false;
             break;
           }
@@ -219,9 +211,10 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
         }
       }
       if (!ok) fail();
-      for (int k = max(0, it - C::kCS); k < it; k++) {
+      for (int k = min(it, prm.ncs); k > 0; k--) {
         int zero = 0;
-        mbar_wait(cfull + 8 * (k % C::kCS), (k / C::kCS) & 1, &zero, kWaitNs);
+        rc.back(prm.ncs);
+        mbar_wait(cfull + 8 * rc.st, rc.ph, &zero, kWaitNs);
       }
     }
   } else if (warp == 1) {
@@ -270,58 +263,48 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
       mbar_wait(done, 0, &zero, kWaitNs);
     }
   } else if (warp >= 8) {
-    // ---- decoding.  Groups take alternate steps, so one group's waits and fences overlap the other's
-    // work; a thread takes 64 codes (32 bytes): half of a row's 128.  It decodes into registers before it
-    // waits for the stage.
+    // ---- decoding.  Groups take steps in turn, so one group's waits and fences overlap the others' work; a
+    // thread takes 64 codes (32 bytes): half of a row's 128.  It decodes into registers before it waits for the
+    // stage.
     const int d = threadIdx.x & 255, g = (threadIdx.x - 256) >> 8;
     const int r = d & 127, h = d >> 7, x7 = r & 7;
     const uint32_t dst0 = h * 16384 + r * 128;
     const uint32_t at0 = r * 64 + (((h * 2) ^ ((r >> 1) & 3)) << 4), at1 = r * 64 + (((h * 2 + 1) ^ ((r >> 1) & 3)) << 4);
     const int srow = (r & 31) * 16 + (r >> 5) * 4;
     const uint32_t lead_full = PAIR ? peer_addr(full0, 0) : full0;
-    Ring rg{0, 0};
+    Ring rg{0, 0}, rc{0, 0}, turn{0, 0};
     int seen = 0;
     bool ok = true;
-    for (int tile = first; ok && tile < prm.tiles; tile += stride)
-      for (int s = s_begin; s < s_end; s++, seen++, rg.advance(nst)) {
-        if (C::kGroups > 1 && (seen & 1) != g) continue;
-        const int cs = seen % C::kCS;
-        if (!mbar_wait_warp(cfull + 8 * cs, (seen / C::kCS) & 1, abort, kWaitNs)) {
+    for (int tile = g < prm.turns ? first : prm.tiles; ok && tile < prm.tiles; tile += stride)
+      for (int s = s_begin; s < s_end; s++, seen++, rg.advance(nst), rc.advance(prm.ncs), turn.advance(prm.turns)) {
+        if (turn.st != g) continue;
+        const int cs = rc.st;
+        if (!mbar_wait_warp(cfull + 8 * cs, rc.ph, abort, kWaitNs)) {
           ok = false;
           break;
         }
-        const uint8_t* codes = base + C::kRing + cs * C::kC;
-        const uint8_t* scales = codes + C::kCodes + srow;
+        const uint32_t codes = ring_c + cs * C::kC, scales = codes + C::kCodes + srow;
         {
-          const uint4 q[2] = {*reinterpret_cast<const uint4*>(codes + at0), *reinterpret_cast<const uint4*>(codes + at1)};
-          uint32_t f[4], more[2] = {0, 0};
+          const uint4 q[2] = {ld_stage_u32x4(codes + at0), ld_stage_u32x4(codes + at1)};
+          float f[4];
           if (FMT == kMXFP4) {
-            const uint32_t two = *reinterpret_cast<const uint16_t*>(scales + h * 2);
-            f[0] = f[1] = factor_e8m0(two & 0xFF, more[0]);
-            f[2] = f[3] = factor_e8m0(two >> 8, more[1]);
+            const uint32_t two = ld_stage_u16(scales + h * 2);
+            f[0] = f[1] = e8m0_value(two & 0xFF);
+            f[2] = f[3] = e8m0_value(two >> 8);
           } else {
-            const uint32_t four = *reinterpret_cast<const uint32_t*>(scales + h * 512);
+            const uint32_t four = ld_stage_u32(scales + h * 512);
 #pragma unroll
-            for (int j = 0; j < 4; j++) f[j] = factor_e4m3((four >> (8 * j)) & 0xFF);
+            for (int j = 0; j < 4; j++) f[j] = e4m3_value((four >> (8 * j)) & 0xFF);
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(cempty + 8 * cs);   // the stage's bytes are in registers
           // rows past the last (their scale bytes are not defined) are part of the reduction: zero
-          if (TR && (int64_t)s * 128 + r >= prm.wrows) {
-            f[0] = f[1] = f[2] = f[3] = 0;
-            more[0] = more[1] = 0;
-          }
+          if (TR && (int64_t)s * 128 + r >= prm.wrows) f[0] = f[1] = f[2] = f[3] = 0.0f;
           uint32_t v[8][4];
 #pragma unroll
           for (int i = 0; i < 8; i++) {
             const uint4& qq = q[i / 4];
-            decode8(i % 4 == 0 ? qq.x : i % 4 == 1 ? qq.y : i % 4 == 2 ? qq.z : qq.w, v[i]);
-#pragma unroll
-            for (int k = 0; k < 4; k++) v[i][k] = mul_bf16x2(v[i][k], f[i / 2]);
-            if (FMT == kMXFP4 && more[i / 4]) {
-#pragma unroll
-              for (int k = 0; k < 4; k++) v[i][k] = mul_bf16x2(v[i][k], more[i / 4]);
-            }
+            decode8(i % 4 == 0 ? qq.x : i % 4 == 1 ? qq.y : i % 4 == 2 ? qq.z : qq.w, f[i / 2], v[i]);
           }
           if (seen >= nst && !mbar_wait_warp(empty0 + 8 * rg.st, rg.ph ^ 1, abort, kWaitNs)) {
             ok = false;
@@ -486,6 +469,8 @@ int launch_tiles(const XView& x, int parts, int64_t T, const Mx4View& w, float a
   p.dtype = dtype;
   p.parts = parts;
   p.nst = std::min(C::kMaxStages, C::kRing / (C::kA + parts * C::kB));
+  p.turns = std::min(C::kGroups, p.nst);   // float16 in a pair: two stages
+  p.ncs = C::kCS / C::kGroups * p.turns;
   p.steps = (int)((x.K + 127) / 128);
   p.groups = (int)groups;
   const int64_t mt = (p.out + 127) / 128;
@@ -504,6 +489,7 @@ int launch_form(const XView& x, int parts, int64_t T, const Mx4View& w, float al
   const int64_t mt = ((TR ? w.n : w.rows) + 127) / 128;
   const int steps = (int)((x.K + 127) / 128);
   // 128-deep steps take about 1350 clocks, the decoding's, for any of these tile widths, and 1750 in a pair
+  // (512 tokens 4096 -> 4096: 27 us in one-SM tiles, 35 in pairs)
   if (dtype == kMxF32) {
     double clocks;
     const int split = best_split(mt * ((T + 63) / 64), steps, 1350, 64, sms, &clocks);
@@ -527,10 +513,15 @@ int launch_form(const XView& x, int parts, int64_t T, const Mx4View& w, float al
   }
 }
 
-// Whether the weights are decoded to the workspace first.  Measured, MXFP4, bf16, decoded first / in the
-// product: 4096 -> 4096 with 512 tokens 32 / 27 us, 640 tokens 33 / 43, 4096 tokens 96 / 148;
-// 4096 -> 14336 with 256 tokens 57 / 43, 512 tokens 78 / 77, 4096 tokens 420 / 476.
-bool use_dense(int64_t T) { return T > 544; }
+// Whether the weights are decoded to the workspace first: for many tokens, where the decoded weights stay in
+// L2 (126 MB) beside x and y, and for float32, whose sums in registers leave the fused form one group that
+// decodes and 64 tokens a tile.  Measured, MXFP4, with L2 flushed, decoded first / in the product, us:
+// bf16 4096 -> 4096 (32 MiB decoded), 512 tokens 37 / 36, 600 42 / 45, 1024 46 / 45, 4096 134 / 151;
+// 4096 -> 8192 (64 MiB), 1024 tokens 87 / 81, 4096 282 / 271; 4096 -> 14336 (112 MiB), 600 tokens 116 / 102,
+// 4096 534 / 462; float32 4096 -> 14336, 1024 tokens 345 / 484.
+bool use_dense(int dtype, int64_t T, int64_t rows, int64_t n) {
+  return T > 544 && (dtype == kMxF32 || rows * n * 2 <= (int64_t)48 << 20);
+}
 
 // The device address of this unit's status word (looked up once per device).
 int* status_word() {
@@ -580,7 +571,7 @@ size_t parts_bytes(int dtype, int64_t T, int64_t K, int aligned) {
 size_t mx4_linear_workspace_bytes(int dtype, int64_t T, int64_t rows, int64_t n, int aligned, int transpose) {
   if (!transpose && mx4_stream_applies(dtype, T, rows, n)) return mx4_stream_workspace_bytes(dtype, T, rows, n);
   return parts_bytes(dtype, T, transpose ? rows : n, aligned) +
-         (use_dense(T) ? (size_t)rows * ((n + 7) / 8 * 8) * 2 : 0);
+         (use_dense(dtype, T, rows, n) ? (size_t)rows * ((n + 7) / 8 * 8) * 2 : 0);
 }
 
 int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, int aligned, const Mx4View& w, float alpha,
@@ -602,7 +593,7 @@ int launch_mx4_linear(int dtype, const void* x, int64_t T, int64_t ld, int align
     note_launch();
     xv = XView{ws, parts * T, K, Kp};
   }
-  if (use_dense(T))
+  if (use_dense(dtype, T, w.rows, w.n))
     return launch_dense(xv, parts, T, w, alpha, dtype, transpose, y, static_cast<uint8_t*>(ws) + pb, stream);
   if (w.fmt == kMXFP4)
     return transpose ? launch_form<kMXFP4, true>(xv, parts, T, w, alpha, dtype, y, stream)

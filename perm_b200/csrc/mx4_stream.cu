@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         break;
       }
       const uint32_t sw = ring + rg.st * kStage;
-      const uint8_t* sc = base + rg.st * kStage + 128 * 128;
+      const uint32_t sc = sw + 128 * 128;
       const uint32_t xcol = (s - s_begin) * (512 * P);
       float c[P][NB][4];
       if (FMT == kNVFP4) {
@@ -384,8 +384,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         float sa[4], sb[4];
         uint32_t ha[4], hb[4];
         if (FMT == kMXFP4) {
-          const uint32_t va = *reinterpret_cast<const uint32_t*>(sc + half * 512 + srow);
-          const uint32_t vb = *reinterpret_cast<const uint32_t*>(sc + half * 512 + srow + 128);
+          const uint32_t va = ld_stage_u32(sc + half * 512 + srow);
+          const uint32_t vb = ld_stage_u32(sc + half * 512 + srow + 128);
           e8m0x2(va, sa[0], sa[1]);
           e8m0x2(va >> 16, sa[2], sa[3]);
           e8m0x2(vb, sb[0], sb[1]);
@@ -394,8 +394,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           const uint32_t sel = t4 < 2 ? 0x1010u : 0x3232u;   // this lane's block of a pair
 #pragma unroll
           for (int j = 0; j < 4; j += 2) {
-            const uint32_t va = *reinterpret_cast<const uint32_t*>(sc + (half * 2 + j / 2) * 512 + srow) & 0x7F7F7F7Fu;
-            const uint32_t vb = *reinterpret_cast<const uint32_t*>(sc + (half * 2 + j / 2) * 512 + srow + 128) & 0x7F7F7F7Fu;
+            const uint32_t va = ld_stage_u32(sc + (half * 2 + j / 2) * 512 + srow) & 0x7F7F7F7Fu;
+            const uint32_t vb = ld_stage_u32(sc + (half * 2 + j / 2) * 512 + srow + 128) & 0x7F7F7F7Fu;
             ha[j] = __byte_perm(e4m3x2(va), 0, sel);
             ha[j + 1] = __byte_perm(e4m3x2(va >> 16), 0, sel);
             hb[j] = __byte_perm(e4m3x2(vb), 0, sel);

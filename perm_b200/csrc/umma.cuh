@@ -153,6 +153,24 @@ __device__ __forceinline__ void fail_pair(volatile int* abort, uint32_t peer_abo
   atomicOr(status, 1);
 }
 
+// Loads from a ring's stage.  Volatile: a plain load may be done again (where registers are scarce) or moved
+// behind the arrive that hands the stage back, when the next TMA load has overwritten it.
+__device__ __forceinline__ uint32_t ld_stage_u32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_stage_u16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.volatile.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 ld_stage_u32x4(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.volatile.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
 // Arrive on this CTA's barrier once the MMAs issued so far complete.
 __device__ __forceinline__ void umma_commit(uint32_t mbar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar) : "memory");

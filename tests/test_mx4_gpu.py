@@ -296,6 +296,49 @@ def test_products_in_every_variant(fmt, dtype, T, out, n):
     mx4.status()
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("out,n", [(2050, 12300), (12800, 2048)])
+def test_many_tokens_with_weights_too_large_to_decode_first(fmt, dtype, out, n):
+    dt, T = DTYPES[dtype], 560
+    w, wv = operand(out, n, fmt, out + n)
+    x = make_x(T, n, T + out, dt, 0.5)
+    check_product(mx4.linear(x, w), f64(x), wv, dt)
+    dy = make_x(T, out, T * 3 + out, dt, 0.5)
+    check_product(mx4.linear_grad(dy, w), f64(dy), wv.T, dt)
+    mx4.status()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [5, 300, 700])
+def test_captured_forward_and_backward(dtype, T):
+    dt = DTYPES[dtype]
+    w, wv = operand(520, 320, "MXFP4", T)
+    x, dy = make_x(T, 320, T, dt, 0.5), make_x(T, 520, T + 1, dt, 0.5)
+
+    def step():
+        leaf = x.detach().requires_grad_(True)
+        y = mx4.linear(leaf, w)
+        return y.detach(), torch.autograd.grad(y, leaf, dy)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        y, dx = step()
+    for rep in range(2):
+        x.copy_(make_x(T, 320, 40 + rep, dt, 0.5))
+        dy.copy_(make_x(T, 520, 50 + rep, dt, 0.5))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        check_product(y, f64(x), wv, dt)
+        check_product(dx, f64(dy), wv.T, dt)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_variants_in_a_graph_on_another_stream(dtype):
     dt = DTYPES[dtype]

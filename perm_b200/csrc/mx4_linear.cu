@@ -489,7 +489,7 @@ int launch_form(const XView& x, int parts, int64_t T, const Mx4View& w, float al
   const int64_t mt = ((TR ? w.n : w.rows) + 127) / 128;
   const int steps = (int)((x.K + 127) / 128);
   // 128-deep steps take about 1350 clocks, the decoding's, for any of these tile widths, and 1750 in a pair
-  // (512 tokens 4096 -> 4096: 27 us in one-SM tiles, 35 in pairs)
+  // (512 tokens 4096 -> 4096: 27 us in one-SM tiles, 35 in pairs; 256 tokens 4096 -> 14336: 48 and 36)
   if (dtype == kMxF32) {
     double clocks;
     const int split = best_split(mt * ((T + 63) / 64), steps, 1350, 64, sms, &clocks);

@@ -20,6 +20,7 @@ Calls only enqueue work on the current stream of the tensors' device, and every 
 is on that device.  Products accumulate in float32 and round once.  Their kernels bound every
 wait; status() raises if one ran out.
 """
+import copy
 import math
 
 import torch
@@ -99,6 +100,19 @@ class Mx4Tensor:
     @property
     def device(self):
         return (self._codes if self._buf is None else self._buf).device
+
+    # Copies are made through __init__, so that the addresses are those of their own tensors.
+    def _rest(self):
+        return self.fmt, self.rows, self.n, self.tensor_scale
+
+    def __copy__(self):
+        return Mx4Tensor(self.codes, self.scales, *self._rest())
+
+    def __deepcopy__(self, memo):
+        return Mx4Tensor(copy.deepcopy(self.codes, memo), copy.deepcopy(self.scales, memo), *self._rest())
+
+    def __reduce__(self):   # clones: a view is written with all that shares its storage
+        return Mx4Tensor, (self.codes.clone(), self.scales.clone(), *self._rest())
 
     def __repr__(self):
         return f"Mx4Tensor({self.fmt}, [{self.rows}, {self.n}], tensor_scale={self.tensor_scale}, device={self.device})"

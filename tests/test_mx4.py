@@ -1,6 +1,9 @@
 """Microscaled 4-bit operands without a GPU: the oracle against the GGUF container's own decoder,
 operand checks, and the refusals of the C entry points (perm_b200/mx4.py)."""
+import copy
 import ctypes
+import io
+import pickle
 
 import numpy as np
 import pytest
@@ -45,6 +48,38 @@ def test_operand_checks():
                dict(scales=torch.zeros((2, 4, 32, 4, 4), dtype=torch.uint8))):
         with pytest.raises(ValueError):
             make(**kw)
+
+
+def _saved(q):
+    f = io.BytesIO()
+    torch.save({"w": q}, f)
+    f.seek(0)
+    return torch.load(f, weights_only=False)["w"]
+
+
+@pytest.mark.parametrize("rows", [0, 3, 130])
+@pytest.mark.parametrize("fmt", mo.BLOCK)
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy, lambda q: pickle.loads(pickle.dumps(q)), _saved],
+                         ids=["copy", "deepcopy", "pickle", "save"])
+def test_copies_of_an_operand_point_to_their_own_tensors(how, fmt, rows):
+    """The addresses that the kernels get are those of the copy's codes and scales, for operands of two
+    tensors and of one buffer."""
+    c = torch.randint(0, 256, (rows, 256), dtype=torch.uint8)
+    s = torch.randint(0, 256, ((rows + 127) // 128, 512 // (4 * mo.BLOCK[fmt]), 32, 4, 4), dtype=torch.uint8)
+    g = 0.5 if fmt == "NVFP4" else 1.0
+    two = mx4.Mx4Tensor(c.clone(), s.clone(), fmt, rows, 300, g)
+    one = mx4.Mx4Tensor._new(torch.empty(0), fmt, rows, 300, g)
+    one.codes.copy_(c)
+    one.scales.copy_(s)
+    for q in (two, one):
+        k = how(q)
+        assert k._cp == k.codes.data_ptr() and k._sp == k.scales.data_ptr() and k.dev == q.dev
+        assert torch.equal(k.codes, c) and torch.equal(k.scales, s)
+        assert (k.fmt, k.shape, k.tensor_scale) == (fmt, (rows, 300), g)
+        if how is not copy.copy:
+            q.codes.fill_(0x11)                       # a copy has storage of its own
+            q.scales.fill_(0x11)
+            assert torch.equal(k.codes, c) and torch.equal(k.scales, s)
 
 
 def test_host_tensors_are_refused():

@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int64_t left = prm.K - k0 - (int64_t)c * 8;   // values of the row from here on
         const S* src = static_cast<const S*>(prm.x) + u.t * prm.ld + k0 + c * 8;
         uint8_t* dst = xs + u.t * xpitch + c * (16 * P);
-        if (prm.vec || left <= 0) {
+        if (prm.vec) {   // 16 bytes at a time: sources past the row's end stay at x, which is aligned as its rows are
 #pragma unroll
           for (int p = 0; p < P; p++) {
             const int64_t bytes = (left - p * (8 / P)) * (int64_t)sizeof(S);

@@ -36,9 +36,11 @@ def row_bytes(ttype, n):
 
 def quantize_dev(ttype, x, qw=None, out=None, stream=None):
     """x: torch f32 CUDA [nrow, n] (contiguous); qw: torch f32 CUDA [n] or None."""
-    torch = nat.torch_cuda()
     nrow, n = x.shape
     _check_shape(ttype, n)
+    if qw is not None and qw.numel() != n:
+        raise ValueError(f"qw must hold {n} column weights, not {qw.numel()}")
+    torch = nat.torch_cuda()
     if out is None:
         out = torch.empty((nrow, row_bytes(ttype, n)), dtype=torch.uint8, device=x.device)
     nat.check(nat.lib().cp_kquant_encode(TYPE_ID[ttype], nat.ptr(x), nrow, n, nat.ptr(qw), nat.ptr(out),
@@ -47,9 +49,11 @@ def quantize_dev(ttype, x, qw=None, out=None, stream=None):
 
 
 def dequantize_dev(ttype, raw, n, out=None, stream=None):
-    torch = nat.torch_cuda()
     nrow = raw.shape[0]
     _check_shape(ttype, n)
+    if raw.numel() < nrow * row_bytes(ttype, n):
+        raise ValueError(f"raw holds {raw.numel()} bytes; {nrow} rows of {n} {ttype} values take {nrow * row_bytes(ttype, n)}")
+    torch = nat.torch_cuda()
     if out is None:
         out = torch.empty((nrow, n), dtype=torch.float32, device=raw.device)
     nat.check(nat.lib().cp_kquant_decode(TYPE_ID[ttype], nat.ptr(raw), nrow, n, nat.ptr(out),

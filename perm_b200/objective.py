@@ -70,6 +70,8 @@ def tensor_err(x, ttype, qw, perm=None, wvec=None, rows_sample=None, seed=0):
     qd = None
     if qw is not None:
         qd = _dev_f32(torch, qw)
+        if qd.numel() != n:
+            raise ValueError(f"qw must hold {n} column weights, not {qd.numel()}")
         if pi is not None:
             qd = _gather(torch, qd, n, None, 1, pi, n).view(n)
     raw = kq.quantize_dev(ttype, xd, qd)

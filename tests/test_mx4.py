@@ -147,3 +147,16 @@ def test_c_entry_points_refuse():
     assert L.cp_kquant_encode(NV, p, 2, 64, None, p, None) == nat.CP_ERR_TYPE
     assert L.cp_grid_params(MX, p, 2, 256, p, p, None) == nat.CP_ERR_TYPE
     assert L.cp_block_bytes(MX) == 17
+
+
+@pytest.mark.parametrize("tt", ["MXFP4", "Q8_0", "Q2_K"])
+def test_codec_refuses_buffers_that_are_too_small(tt):
+    """Fewer container bytes than the rows take, and column weights of another length, would be read past their end."""
+    from perm_b200 import kquant as kq
+    per = kq.row_bytes(tt, 512)
+    for raw in (torch.zeros((3, per - 1), dtype=torch.uint8), torch.zeros(3 * per, dtype=torch.uint8)):
+        with pytest.raises(ValueError):
+            kq.dequantize_dev(tt, raw, 512)
+    for qw in (torch.ones(511), torch.ones(1), torch.ones(1024)):
+        with pytest.raises(ValueError):
+            kq.quantize_dev(tt, torch.zeros(3, 512), qw)

@@ -282,7 +282,8 @@ int cp_xtx_status(void* workspace, void* stream);
  *
  * An operand is two arrays.  codes: [rows][P/2], P = n rounded up to 256, element 2j of a row in
  * the low half of byte j.  scales: tiles of 128 rows x 4 blocks, [rows/128][blocks of P/4][512],
- * byte 16 r + 4 j + k of a tile for row 32 j + r and block k.  Both are zero past n. */
+ * byte 16 r + 4 j + k of a tile for row 32 j + r and block k.  Both are zero past n, and so are
+ * the scale bytes that fill the last tile past the last row (no product uses those). */
 #define CP_MXFP4 39
 #define CP_NVFP4 40
 #define CP_MX4_BF16 0

@@ -9,7 +9,7 @@
 // group][32][4][4]: byte 16 r + 4 j + k of a tile is row 32 j + r, block k.  That is the order in
 // which the block-scaled MMA wants a tile's scales in tensor memory (lane r, column j, byte k), so
 // they go there by plain copies.  Codes and scales past n are zero; the scale bytes of rows past
-// the last are never used.
+// the last are written as zeros and never used.
 #pragma once
 #include <cstdint>
 #include <cuda_bf16.h>

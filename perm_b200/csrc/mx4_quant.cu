@@ -382,13 +382,20 @@ __global__ void __launch_bounds__(256) weighted_err_kernel(const uint8_t* __rest
   }
 }
 
-// Container -> operand: one thread per block of the padded row (blocks past n: zero).
+__host__ __device__ inline int64_t tile_rows(int64_t rows) { return (rows + 127) / 128 * 128; }
+
+// Container -> operand: one thread per block of the padded row (blocks past n, and the scale bytes of the rows
+// that fill the last tile: zero).
 __global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* __restrict__ raw, int64_t nrow, int nb_row, int nb_pad,
                                                      uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   const int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x;
-  if (i >= nrow * nb_pad) return;
   const int64_t row = i / nb_pad;
+  if (row >= tile_rows(nrow)) return;
   const int b = (int)(i - row * nb_pad);
+  if (row >= nrow) {
+    scales[mx_scale_offset(row, b, nb_pad / 4)] = 0;
+    return;
+  }
   uint32_t o[4] = {0, 0, 0, 0};
   uint8_t s = 0;
   if (b < nb_row) {
@@ -405,6 +412,7 @@ __global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* __restrict__
   scales[mx_scale_offset(row, b, nb_pad / 4)] = s;
 }
 
+// Row lanes that hold a row.
 int64_t row_lanes(int64_t rows) { return rows / 128 * 32 + (rows % 128 < 32 ? rows % 128 : 32); }
 
 template <typename T, int FMT, bool IMAT>
@@ -415,7 +423,7 @@ int quantize_typed(const T* x, int64_t rows, int64_t n, int64_t ld, const float*
   constexpr int H = sizeof(T) == 2 && FMT == kMXFP4 && !IMAT ? 8 : 4;
   const int64_t pitch = (n + 255) / 256 * 256;
   const int chunks = (int)((pitch + 64 * H - 1) / (64 * H));
-  const int64_t units = row_lanes(rows) * chunks;
+  const int64_t units = tile_rows(rows) / 4 * chunks;   // all row lanes of a tile: their scale bytes are zero past the last row
   const unsigned grid = (unsigned)((units + kWarps - 1) / kWarps);
   const bool vec = ((uintptr_t)x & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
   quantize_kernel<T, FMT, IMAT, H><<<grid, 32 * kWarps, 0, stream>>>(x, rows, n, ld, qw, scale, 1.0f / scale, chunks, pitch,
@@ -497,7 +505,7 @@ int launch_mx4_unpack(const uint8_t* raw, int64_t nrow, int64_t n, uint8_t* code
                       cudaStream_t stream) {
   if (nrow == 0) return 0;
   const int nb = (int)(n / 32), nbp = (int)((n + 255) / 256 * 8);
-  const int64_t total = nrow * nbp;
+  const int64_t total = tile_rows(nrow) * nbp;
   unpack_kernel<<<(unsigned)((total + 255) / 256), 256, 0, stream>>>(raw, nrow, nb, nbp, codes, scales);
   note_launch();
   return 0;

@@ -43,7 +43,8 @@ class Mx4Tensor:
     codes   uint8 [rows, P/2], P = n rounded up to 256: element 2j of a row in the low half of
             byte j, zero past n
     scales  uint8, tiles of 128 rows x 4 blocks, [ceil(rows/128), P/(4 block), 32, 4, 4]: entry
-            [i, g, r, j, k] is the scale of row 128 i + 32 j + r, block 4 g + k; zero past n
+            [i, g, r, j, k] is the scale of row 128 i + 32 j + r, block 4 g + k; zero past n and
+            past the last row
     tensor_scale  a positive float that multiplies every value"""
     __slots__ = ("fmt", "rows", "n", "tensor_scale", "dev", "_codes", "_scales", "_buf", "_cp", "_sp")
 

@@ -28,3 +28,38 @@ def test_few_tokens_at_every_alignment_of_x(fmt, dtype, T):
             x = base[at:at + T * (n + 3)].view(T, n + 3)[:, :n]
             check_product(mx4.linear(x, w), f64(x), wv, dt)
     mx4.status()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows,n", [(1, 40), (5, 256), (33, 300), (127, 64), (130, 1000)])
+def test_padding_is_written_and_nothing_behind_it(fmt, rows, n):
+    """Every byte of an operand is defined, whatever its memory held: codes and scales past n and the scales of
+    rows past the last are zero.  Bytes behind the arrays stay."""
+    L, s = nat.lib(), nat.stream_ptr(torch)
+    nc, ns = L.cp_mx4_codes_bytes(rows, n), L.cp_mx4_scales_bytes(nat.MX4_ID[fmt], rows, n)
+
+    def run(call):
+        codes = torch.full((nc + 512,), 0xA5, dtype=torch.uint8, device="cuda")
+        scales = torch.full((ns + 512,), 0xA5, dtype=torch.uint8, device="cuda")
+        nat.check(call(codes.data_ptr(), scales.data_ptr()))
+        assert (codes[nc:] == 0xA5).all() and (scales[ns:] == 0xA5).all()
+        return codes[:nc].view(rows, -1).cpu().numpy(), scales[:ns].view(-1, nc // rows // (2 * mo.BLOCK[fmt]), 32, 4, 4).cpu().numpy()
+
+    for dt, kind in ((torch.bfloat16, nat.CP_MX4_BF16), (torch.float32, nat.CP_MX4_F32)):
+        x = make_x(rows, n, rows + n, dt)
+        for qw in (None, torch.linspace(0.5, 2.0, n, device="cuda")):
+            codes, byte = mo.quantize(f64(x), fmt, 1.0, None if qw is None else f64(qw))
+            want = mo.pack(np.where(codes == 8, 0, codes), byte, fmt, n)
+            got = run(lambda c, p: L.cp_mx4_quantize(nat.MX4_ID[fmt], kind, x.data_ptr(), rows, n, n,
+                                                     None if qw is None else qw.data_ptr(), 1.0, c, p, s))
+            assert np.array_equal(got[1], want[1])
+            gc, _ = mo.unpack(got[0], got[1], fmt, rows, n)
+            wc, _ = mo.unpack(want[0], want[1], fmt, rows, n)
+            assert np.array_equal(np.where(gc == 8, 0, gc), wc)
+    if fmt == "MXFP4" and n % 32 == 0:
+        x = f64(make_x(rows, n, 1))
+        codes, byte = mo.quantize(x, fmt)
+        raw = torch.from_numpy(mo.container(codes, byte)).cuda()
+        got = run(lambda c, p: L.cp_mx4_from_gguf(raw.data_ptr(), rows, n, c, p, s))
+        want = mo.pack(codes, byte, fmt, n)
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])

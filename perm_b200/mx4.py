@@ -315,6 +315,16 @@ class Linear(torch.nn.Module):
     def weight4(self):
         return Mx4Tensor(self.codes, self.scales, self.fmt, self.out_features, self.in_features, self.tensor_scale)
 
+    def get_extra_state(self):
+        """What a saved state holds beside codes, scales and bias: the format's id and the tensor scale."""
+        return torch.tensor([_ID[self.fmt], self.tensor_scale], dtype=torch.float64)
+
+    def set_extra_state(self, state):
+        fmt, scale = state.tolist()
+        if fmt != _ID[self.fmt]:
+            raise ValueError(f"the saved weights are not {self.fmt}")
+        self.tensor_scale = scale
+
     def forward(self, x):
         y = linear(x, self.weight4)
         return y if self.bias is None else y + self.bias.to(y.dtype)

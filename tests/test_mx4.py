@@ -160,3 +160,35 @@ def test_codec_refuses_buffers_that_are_too_small(tt):
     for qw in (torch.ones(511), torch.ones(1), torch.ones(1024)):
         with pytest.raises(ValueError):
             kq.quantize_dev(tt, torch.zeros(3, 512), qw)
+
+
+def _module(fmt, g, seed):
+    rng = np.random.default_rng(seed)
+    c, s = mo.pack(*mo.quantize(rng.standard_normal((5, 70)), fmt, g), fmt, 70)
+    return mx4.Linear(mx4.Mx4Tensor(torch.from_numpy(c), torch.from_numpy(s), fmt, 5, 70, g), torch.full((5,), float(seed)))
+
+
+def test_a_saved_module_keeps_its_tensor_scale():
+    a, b = _module("NVFP4", 0.25, 1), _module("NVFP4", 1.0, 2)
+    f = io.BytesIO()
+    torch.save(a.state_dict(), f)
+    f.seek(0)
+    assert not any(b.load_state_dict(torch.load(f))), "all keys match"
+    assert b.tensor_scale == 0.25 and b.weight4.tensor_scale == 0.25
+    assert torch.equal(b.codes, a.codes) and torch.equal(b.scales, a.scales) and torch.equal(b.bias, a.bias)
+    nested = torch.nn.Sequential(_module("NVFP4", 2.0, 3))
+    nested.load_state_dict(torch.nn.Sequential(a).state_dict())
+    assert nested[0].tensor_scale == 0.25
+    assert copy.deepcopy(a).tensor_scale == 0.25 and pickle.loads(pickle.dumps(a)).weight4.tensor_scale == 0.25
+
+
+def test_a_saved_module_of_another_format_or_without_its_scale_is_refused():
+    a = _module("NVFP4", 0.25, 1)
+    with pytest.raises((ValueError, RuntimeError)):
+        _module("MXFP4", 1.0, 2).load_state_dict(a.state_dict())
+    part = {k: v for k, v in a.state_dict().items() if "extra" not in k}
+    with pytest.raises(RuntimeError):
+        _module("NVFP4", 1.0, 2).load_state_dict(part)
+    one = _module("MXFP4", 1.0, 2)
+    with pytest.raises(ValueError):
+        one.set_extra_state(a.get_extra_state())

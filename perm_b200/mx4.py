@@ -24,6 +24,7 @@ import copy
 import math
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import _native as nat
 
@@ -262,22 +263,31 @@ class _Product(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        if torch.is_grad_enabled():   # create_graph: the gradient has one itself
+        if torch.is_grad_enabled() or _forward._current_level >= 0:   # create_graph, or dy has a tangent: a gradient itself
             return _Product.apply(dy, ctx.w, 1 - ctx.transpose), None, None
         return _product(dy, ctx.w, 1 - ctx.transpose, "mx4.linear (backward)"), None, None
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        return _Product.apply(tangent, ctx.w, ctx.transpose)
+
+
+def _differentiated(x):
+    return _forward._current_level >= 0 or x.requires_grad and torch.is_grad_enabled()
 
 
 def linear(x, w):
     """x w^T: x [..., n] (bf16, f16 or f32, taken at its own precision), w [out, n] -> [..., out] in
-    x's type.  x gets a gradient; the weights are frozen."""
-    if x.requires_grad and torch.is_grad_enabled():
+    x's type.  x gets a gradient (reverse and forward mode, also of second order; torch.func and vmap
+    raise); the weights are frozen."""
+    if _differentiated(x):
         return _Product.apply(x, w, 0)
     return _product(x, w, 0, "mx4.linear")
 
 
 def linear_grad(dy, w):
     """The gradient of linear(x, w) with respect to x: dy w, dy [..., out] -> [..., n]."""
-    if dy.requires_grad and torch.is_grad_enabled():
+    if _differentiated(dy):
         return _Product.apply(dy, w, 1)
     return _product(dy, w, 1, "mx4.linear_grad")
 

@@ -192,3 +192,27 @@ def test_a_saved_module_of_another_format_or_without_its_scale_is_refused():
     one = _module("MXFP4", 1.0, 2)
     with pytest.raises(ValueError):
         one.set_extra_state(a.get_extra_state())
+
+
+def test_forward_mode_derivatives(monkeypatch):
+    """linear's tangent, the tangent of its gradient (forward over reverse), and differences, with a plain
+    product in the place of the kernels'."""
+    import torch.autograd.forward_ad as fw
+    W = torch.randn(5, 7, dtype=torch.float64)
+    monkeypatch.setattr(mx4, "_product", lambda x, w, t, what: x.detach() @ (W if t else W.T))
+    x, t = torch.randn(3, 7, dtype=torch.float64), torch.randn(3, 7, dtype=torch.float64)
+    v, u = torch.randn(3, 5, dtype=torch.float64), torch.randn(3, 5, dtype=torch.float64)
+    with fw.dual_level():
+        assert torch.equal(fw.unpack_dual(mx4.linear(fw.make_dual(x, t), None)).tangent, t @ W.T)
+        assert torch.equal(fw.unpack_dual(mx4.linear_grad(fw.make_dual(v, u), None)).tangent, u @ W)
+        assert fw.unpack_dual(mx4.linear(x, None)).tangent is None
+        d = x.clone().requires_grad_(True)
+        g, = torch.autograd.grad(mx4.linear(d, None), d, fw.make_dual(v, u))
+        assert torch.equal(fw.unpack_dual(g).tangent, u @ W)
+    leaf = x.clone().requires_grad_(True)
+    assert torch.autograd.gradcheck(lambda z: mx4.linear(z, None), (leaf,), check_forward_ad=True)
+    assert torch.autograd.gradgradcheck(lambda z: mx4.linear(z, None), (leaf,), check_fwd_over_rev=True)
+    for f in (lambda: torch.func.jvp(lambda z: mx4.linear(z, None), (x,), (t,)),
+              lambda: torch.func.grad(lambda z: mx4.linear(z, None).sum())(x)):
+        with pytest.raises(RuntimeError):
+            f()

@@ -63,3 +63,25 @@ def test_padding_is_written_and_nothing_behind_it(fmt, rows, n):
         got = run(lambda c, p: L.cp_mx4_from_gguf(raw.data_ptr(), rows, n, c, p, s))
         want = mo.pack(codes, byte, fmt, n)
         assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [2, 40])
+def test_forward_mode(dtype, T):
+    import torch.autograd.forward_ad as fw
+    dt = DTYPES[dtype]
+    w, wv = operand(96, 200, "MXFP4", 3)
+    x, t = make_x(T, 200, 1, dt, 0.5), make_x(T, 200, 2, dt, 0.5)
+    dy, u = make_x(T, 96, 3, dt, 0.5), make_x(T, 96, 4, dt, 0.5)
+    with fw.dual_level():
+        y = fw.unpack_dual(mx4.linear(fw.make_dual(x, t), w))
+        check_product(y.primal, f64(x), wv, dt)
+        check_product(y.tangent, f64(t), wv, dt)
+        leaf = x.clone().requires_grad_(True)
+        g, = torch.autograd.grad(mx4.linear(leaf, w), leaf, fw.make_dual(dy, u))
+        g = fw.unpack_dual(g)
+        check_product(g.primal, f64(dy), wv.T, dt)
+        check_product(g.tangent, f64(u), wv.T, dt)
+    x3 = x.view(1, T, 200)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda z: mx4.linear(z, w))(x3)

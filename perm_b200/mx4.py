@@ -68,13 +68,13 @@ class Mx4Tensor:
         self._cp, self._sp = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
-    def _new(cls, like, fmt, rows, n, tensor_scale):
-        """An operand on like's device, not yet filled: one allocation, of which codes and scales are
-        views made when they are asked for."""
+    def _new(cls, like, fmt, rows, n, tensor_scale, buf=None):
+        """An operand on like's device, not yet filled: one allocation (or `buf`, which is one), of which
+        codes and scales are views made when they are asked for."""
         q = cls.__new__(cls)
         pitch = (n + 255) // 256 * 128
         at = (rows * pitch + 255) // 256 * 256
-        q._buf = like.new_empty((at + (rows + 127) // 128 * (256 // BLOCK[fmt]) * pitch,), dtype=torch.uint8)
+        q._buf = buf if buf is not None else like.new_empty((at + (rows + 127) // 128 * (256 // BLOCK[fmt]) * pitch,), dtype=torch.uint8)
         q.fmt, q.rows, q.n, q.tensor_scale, q.dev = fmt, rows, n, tensor_scale, like.get_device()
         q._codes = q._scales = None
         q._cp = q._buf.data_ptr()
@@ -115,6 +115,17 @@ class Mx4Tensor:
 
     def __reduce__(self):   # clones: a view is written with all that shares its storage
         return Mx4Tensor, (self.codes.clone(), self.scales.clone(), *self._rest())
+
+    def _tensors(self):
+        return (self._codes, self._scales) if self._buf is None else (self._buf,)
+
+    def _over(self, tensors):
+        """This operand over tensors in the place of its own."""
+        if tensors[0] is self._tensors()[0]:
+            return self
+        if self._buf is None:
+            return Mx4Tensor(*tensors, *self._rest())
+        return Mx4Tensor._new(tensors[0], *self._rest(), buf=tensors[0])
 
     def __repr__(self):
         return f"Mx4Tensor({self.fmt}, [{self.rows}, {self.n}], tensor_scale={self.tensor_scale}, device={self.device})"
@@ -259,13 +270,18 @@ class _Product(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, transpose):
         ctx.w, ctx.transpose = w, transpose
+        own = w._tensors()
+        ctx.saved = not own[0].is_inference()   # those have no version and cannot be saved
+        if ctx.saved:
+            ctx.save_for_backward(*own)
         return _product(x, w, transpose, "mx4.linear_grad" if transpose else "mx4.linear")
 
     @staticmethod
     def backward(ctx, dy):
+        w = ctx.w._over(ctx.saved_tensors) if ctx.saved else ctx.w   # raises if the weights were written since
         if torch.is_grad_enabled() or _forward._current_level >= 0:   # create_graph, or dy has a tangent: a gradient itself
-            return _Product.apply(dy, ctx.w, 1 - ctx.transpose), None, None
-        return _product(dy, ctx.w, 1 - ctx.transpose, "mx4.linear (backward)"), None, None
+            return _Product.apply(dy, w, 1 - ctx.transpose), None, None
+        return _product(dy, w, 1 - ctx.transpose, "mx4.linear (backward)"), None, None
 
     @staticmethod
     def jvp(ctx, tangent, *_):

@@ -200,19 +200,49 @@ def test_forward_mode_derivatives(monkeypatch):
     import torch.autograd.forward_ad as fw
     W = torch.randn(5, 7, dtype=torch.float64)
     monkeypatch.setattr(mx4, "_product", lambda x, w, t, what: x.detach() @ (W if t else W.T))
+    q = mx4.Mx4Tensor._new(torch.empty(0), "MXFP4", 5, 7, 1.0)
     x, t = torch.randn(3, 7, dtype=torch.float64), torch.randn(3, 7, dtype=torch.float64)
     v, u = torch.randn(3, 5, dtype=torch.float64), torch.randn(3, 5, dtype=torch.float64)
     with fw.dual_level():
-        assert torch.equal(fw.unpack_dual(mx4.linear(fw.make_dual(x, t), None)).tangent, t @ W.T)
-        assert torch.equal(fw.unpack_dual(mx4.linear_grad(fw.make_dual(v, u), None)).tangent, u @ W)
-        assert fw.unpack_dual(mx4.linear(x, None)).tangent is None
+        assert torch.equal(fw.unpack_dual(mx4.linear(fw.make_dual(x, t), q)).tangent, t @ W.T)
+        assert torch.equal(fw.unpack_dual(mx4.linear_grad(fw.make_dual(v, u), q)).tangent, u @ W)
+        assert fw.unpack_dual(mx4.linear(x, q)).tangent is None
         d = x.clone().requires_grad_(True)
-        g, = torch.autograd.grad(mx4.linear(d, None), d, fw.make_dual(v, u))
+        g, = torch.autograd.grad(mx4.linear(d, q), d, fw.make_dual(v, u))
         assert torch.equal(fw.unpack_dual(g).tangent, u @ W)
     leaf = x.clone().requires_grad_(True)
-    assert torch.autograd.gradcheck(lambda z: mx4.linear(z, None), (leaf,), check_forward_ad=True)
-    assert torch.autograd.gradgradcheck(lambda z: mx4.linear(z, None), (leaf,), check_fwd_over_rev=True)
-    for f in (lambda: torch.func.jvp(lambda z: mx4.linear(z, None), (x,), (t,)),
-              lambda: torch.func.grad(lambda z: mx4.linear(z, None).sum())(x)):
+    assert torch.autograd.gradcheck(lambda z: mx4.linear(z, q), (leaf,), check_forward_ad=True)
+    assert torch.autograd.gradgradcheck(lambda z: mx4.linear(z, q), (leaf,), check_fwd_over_rev=True)
+    for f in (lambda: torch.func.jvp(lambda z: mx4.linear(z, q), (x,), (t,)),
+              lambda: torch.func.grad(lambda z: mx4.linear(z, q).sum())(x)):
         with pytest.raises(RuntimeError):
             f()
+
+
+@pytest.mark.parametrize("buffer", [False, True])
+def test_weights_written_between_forward_and_backward(monkeypatch, buffer):
+    """They are saved tensors: a write in place is noticed, hooks see them and what a hook gives back is used."""
+    seen = []
+    monkeypatch.setattr(mx4, "_product", lambda x, w, t, what: seen.append(w) or x.new_zeros(x.shape[0], w.n if t else w.rows))
+    q = mx4.Mx4Tensor._new(torch.empty(0), "MXFP4", 5, 7, 1.0)
+    q.codes.zero_(), q.scales.zero_()
+    if not buffer:
+        q = copy.copy(q)
+    x = torch.zeros(3, 7, requires_grad=True)
+    mx4.linear(x, q).sum().backward()
+    assert seen[-1] is q
+    y = mx4.linear(x, q)
+    q.codes.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(t.clone()) or packed[-1], lambda t: t):
+        y = mx4.linear(x, q)
+        assert sum(p.numel() for p in packed) >= q.codes.numel() + q.scales.numel()
+        y.sum().backward()
+    w = seen[-1]
+    assert w is not q and w._cp == w.codes.data_ptr() != q._cp and torch.equal(w.codes, q.codes) and torch.equal(w.scales, q.scales)
+    with torch.inference_mode():
+        r = mx4.Mx4Tensor._new(torch.empty(0), "MXFP4", 5, 7, 1.0)
+    mx4.linear(x, r).sum().backward()
+    assert seen[-1] is r

@@ -54,6 +54,8 @@ def dequantize_dev(ttype, raw, n, out=None, stream=None):
     if raw.numel() < nrow * row_bytes(ttype, n):
         raise ValueError(f"raw holds {raw.numel()} bytes; {nrow} rows of {n} {ttype} values take {nrow * row_bytes(ttype, n)}")
     torch = nat.torch_cuda()
+    if ttype == "MXFP4" and raw.data_ptr() % 16:   # rows of 17-byte blocks: a slice starts anywhere
+        raw = raw.clone()
     if out is None:
         out = torch.empty((nrow, n), dtype=torch.float32, device=raw.device)
     nat.check(nat.lib().cp_kquant_decode(TYPE_ID[ttype], nat.ptr(raw), nrow, n, nat.ptr(out),

@@ -85,3 +85,14 @@ def test_forward_mode(dtype, T):
     x3 = x.view(1, T, 200)
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda z: mx4.linear(z, w))(x3)
+
+
+@pytest.mark.parametrize("n", [32, 96, 4096])
+def test_container_rows_sliced_on_the_device(n):
+    from perm_b200 import kquant as kq
+    x = make_x(9, n, n)
+    raw = kq.QUANTIZE["MXFP4"](x)
+    want = kq.DEQUANTIZE["MXFP4"](raw, n)
+    for r0 in range(9):
+        assert torch.equal(kq.DEQUANTIZE["MXFP4"](raw[r0:], n), want[r0:])
+        assert torch.equal(mx4.dequantize(mx4.from_gguf(raw[r0:], n)), want[r0:])

@@ -35,6 +35,7 @@ _DTYPE = {torch.bfloat16: nat.CP_MX4_BF16, torch.float16: nat.CP_MX4_F16, torch.
 # stream's address comes from torch directly (a Stream object costs more than the rest of the checks).
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
+_MIN_SCALE, _MAX_SCALE = 2.0 ** -126, (2.0 - 2.0 ** -23) * 2.0 ** 127   # float32's normal numbers
 _workspace = {}   # sizes of a linear call -> workspace bytes
 
 
@@ -60,8 +61,8 @@ class Mx4Tensor:
             raise ValueError(f"scales must be contiguous uint8 tiles of {rows} rows and {pitch * 2 // BLOCK[fmt]} blocks")
         if codes.device != scales.device:
             raise ValueError("codes and scales must be on one device")
-        if not (tensor_scale > 0.0 and math.isfinite(tensor_scale)):
-            raise ValueError("tensor_scale must be positive and finite")
+        if not _MIN_SCALE <= tensor_scale <= _MAX_SCALE:
+            raise ValueError("tensor_scale must be positive and within float32's normal range")
         self.fmt, self.rows, self.n, self.tensor_scale = fmt, rows, n, tensor_scale
         self.dev = codes.get_device()   # CUDA device index, -1 on the host
         self._codes, self._scales, self._buf = codes, scales, None
@@ -216,11 +217,14 @@ def matmul(a, w, dtype=torch.bfloat16):
         raise ValueError(f"mx4.matmul: {a!r} and {w!r} must have one format and one n")
     if a.dev != w.dev:
         raise ValueError("mx4.matmul: operands must be on one device")
+    scale = a.tensor_scale * w.tensor_scale
+    if not _MIN_SCALE <= scale <= _MAX_SCALE:
+        raise ValueError("mx4.matmul: the product of the tensor scales must be within float32's normal range")
     if a.dev < 0:
         _refuse_host("mx4.matmul")
     y = (w._buf if w._codes is None else w._codes).new_empty((a.rows, w.rows), dtype=dtype)
     _call(a.dev, nat.lib().cp_mx4_matmul, "mx4.matmul", _ID[w.fmt], a._cp, a._sp, a.rows, w._cp, w._sp, w.rows, w.n,
-          a.tensor_scale * w.tensor_scale, dt, y.data_ptr())
+          scale, dt, y.data_ptr())
     return y
 
 

@@ -246,3 +246,19 @@ def test_weights_written_between_forward_and_backward(monkeypatch, buffer):
         r = mx4.Mx4Tensor._new(torch.empty(0), "MXFP4", 5, 7, 1.0)
     mx4.linear(x, r).sum().backward()
     assert seen[-1] is r
+
+
+def test_tensor_scales_outside_float32_are_refused():
+    """The kernels take the scale of a result as one float32 number: beyond its range all of a result was infinite,
+    NaN or zero."""
+    def make(g):
+        return mx4.Mx4Tensor(torch.zeros((3, 128), dtype=torch.uint8), torch.zeros((1, 4, 32, 4, 4), dtype=torch.uint8), "NVFP4", 3, 64, g)
+    for g in (1e300, 2.0 ** 128, 2.0 ** -127, 1e-300):
+        with pytest.raises(ValueError):
+            make(g)
+    for a, b in ((2.0 ** 99, 2.0 ** 29), (2.0 ** -100, 2.0 ** -27), (2.0 ** 99, 2.0 ** 99)):
+        with pytest.raises(ValueError, match="product of the tensor scales"):
+            mx4.matmul(make(a), make(b))
+    for a, b in ((2.0 ** 99, 2.0 ** 28), (2.0 ** -100, 2.0 ** -26), (2.0 ** 99, 2.0 ** -99)):
+        with pytest.raises(nat.CudaPathError):   # host operands: all that is wrong with these
+            mx4.matmul(make(a), make(b))

@@ -316,7 +316,9 @@ def status(device=None):
     """Raise CudaPathError if a bounded wait in an earlier product on `device` ran out (its result
     is incomplete); synchronises the current stream."""
     nat.torch_cuda()
-    idx = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    idx = None if device is None else torch.device(device).index
+    if idx is None:   # a device without a number is the current one
+        idx = torch.cuda.current_device()
     _call(idx, nat.lib().cp_mx4_status, "mx4.status")
 
 

@@ -262,3 +262,13 @@ def test_tensor_scales_outside_float32_are_refused():
     for a, b in ((2.0 ** 99, 2.0 ** 28), (2.0 ** -100, 2.0 ** -26), (2.0 ** 99, 2.0 ** -99)):
         with pytest.raises(nat.CudaPathError):   # host operands: all that is wrong with these
             mx4.matmul(make(a), make(b))
+
+
+def test_status_of_a_device_without_a_number_is_the_current_devices(monkeypatch):
+    asked = []
+    monkeypatch.setattr(nat, "torch_cuda", lambda: torch)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    monkeypatch.setattr(mx4, "_call", lambda idx, fn, what: asked.append(idx))
+    for dev in (None, "cuda", torch.device("cuda"), "cuda:1", torch.device("cuda", 0)):
+        mx4.status(dev)
+    assert asked == [3, 3, 3, 1, 0]

@@ -104,6 +104,7 @@ def collect_hessians(model, batches, gguf_ne0, arch, n_layers, layer_lo=0, layer
     Returns ({gguf_name: {"H": float32 [d, d] numpy, "n": int}}, unmapped)."""
     import torch
     import torch.nn as nn
+    from . import mx4
     from .mx4 import Linear as Linear4
     if layer_hi is None:
         layer_hi = n_layers
@@ -205,6 +206,8 @@ def collect_hessians(model, batches, gguf_ne0, arch, n_layers, layer_lo=0, layer
             h.remove()
     for dev in {H.device.index for H in acc.values() if H.is_cuda}:
         xtx_status(dev)
+    for dev in {m.codes.device for m in model.modules() if isinstance(m, Linear4) and m.codes.is_cuda}:
+        mx4.status(dev)   # an incomplete product upstream would make the Hessians wrong
     for gname, first in alias.items():
         acc[gname], cnt[gname] = acc[first].clone(), cnt[first]
     hessians = {}

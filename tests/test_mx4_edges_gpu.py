@@ -96,3 +96,44 @@ def test_container_rows_sliced_on_the_device(n):
     for r0 in range(9):
         assert torch.equal(kq.DEQUANTIZE["MXFP4"](raw[r0:], n), want[r0:])
         assert torch.equal(mx4.dequantize(mx4.from_gguf(raw[r0:], n)), want[r0:])
+
+
+def test_collected_hessians_ask_for_the_products_status(monkeypatch):
+    """A product whose wait ran out is incomplete, and so is what later layers saw: collection ends with the error."""
+    from perm_b200 import hessians
+
+    class Mlp(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.up_proj, self.down_proj = torch.nn.Linear(64, 96), torch.nn.Linear(96, 64)
+
+        def forward(self, x):
+            return self.down_proj(self.up_proj(x))
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.model = torch.nn.Module()
+            self.model.embed_tokens = torch.nn.Embedding(16, 64)
+            self.model.layers = torch.nn.ModuleList([torch.nn.Module()])
+            self.model.layers[0].mlp = Mlp()
+
+        def forward(self, ids):
+            return self.model.layers[0].mlp(self.model.embed_tokens(ids))
+
+    net = Net().cuda().to(torch.bfloat16)
+    mlp = net.model.layers[0].mlp
+    mlp.up_proj = mx4.Linear.from_linear(mlp.up_proj)
+    ne0 = {"blk.0.ffn_up.weight": 64, "blk.0.ffn_down.weight": 96}
+    collect = lambda: hessians.collect_hessians(net, [torch.arange(16)], ne0, "qwen3", 1, log=lambda *_: None)  # noqa: E731
+    asked = []
+    real = mx4.status
+    monkeypatch.setattr(mx4, "status", lambda dev=None: asked.append(dev) or real(dev))
+    H, _ = collect()
+    assert set(H) == set(ne0) and asked == [torch.device("cuda", 0)]
+
+    def ran_out(dev=None):
+        raise nat.CudaPathError("a bounded wait ran out")
+    monkeypatch.setattr(mx4, "status", ran_out)
+    with pytest.raises(nat.CudaPathError):
+        collect()

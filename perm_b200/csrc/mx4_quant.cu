@@ -102,8 +102,12 @@ __device__ __forceinline__ void quantize_block(float2 (&v)[H], uint32_t top, con
     constexpr int C = mx_candidates<FMT>();
     const int first = byte;
     // values and steps in units of the block's maximum (a power of two), so that squares neither vanish
-    // nor overflow
-    const float unit = __uint_as_float((uint32_t)min(max(254 - (int)(m >> 23), 1), 253) << 23);
+    // nor overflow.  Not searched, and not in such units, are a block with scale byte 0 (all but empty: NVFP4's
+    // step in units of so small a maximum may be infinite) and one of NVFP4 that is past 2^100 tensor
+    // scales (saturated throughout; its step may vanish).
+    float unit = __uint_as_float((uint32_t)min(max(254 - (int)(m >> 23), 1), 253) << 23);
+    const bool search = finite && first > 0 && (FMT == kMXFP4 || __fmul_rn(tensor_scale, unit) >= 0x1p-100f);
+    unit = search ? unit : 1.0f;
     const float times = __fmul_rn(tensor_scale, unit);
     float err[C];
     const MxStep step0 = mx_step<FMT>(first, times);
@@ -131,7 +135,7 @@ __device__ __forceinline__ void quantize_block(float2 (&v)[H], uint32_t top, con
     bool near = !(best > 1e-30f && best < 1e30f);
 #pragma unroll
     for (int c = 0; c < C; c++) near |= c != pick && err[c] <= best * 1.0000153f;
-    near = near && first > 0 && finite;
+    near = near && search;
     if (__any_sync(0xffffffffu, near)) {
       double bd = 0.0;
       int pd = 0;
@@ -151,7 +155,7 @@ __device__ __forceinline__ void quantize_block(float2 (&v)[H], uint32_t top, con
       }
       if (near) pick = pd;
     }
-    if (first == 0 || !finite) pick = 0;   // scale byte 0 (an all but empty block) is not searched
+    if (!search) pick = 0;
     if (pick > 0) byte = mx_candidate<FMT>(first, pick);
     mx_codes<FMT, H>(v, mx_step<FMT>(byte, times), code);
   }

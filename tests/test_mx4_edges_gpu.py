@@ -137,3 +137,18 @@ def test_collected_hessians_ask_for_the_products_status(monkeypatch):
     monkeypatch.setattr(mx4, "status", ran_out)
     with pytest.raises(nat.CudaPathError):
         collect()
+
+
+@pytest.mark.parametrize("g", [2.0 ** -100, 2.0 ** -30, 1.0, 4.0, 2.0 ** 40, 2.0 ** 99])
+def test_weighted_blocks_far_from_the_tensor_scale(g):
+    """Blocks of zeros, far below and far above what the tensor scale's e4m3 scales reach: codes as without weights."""
+    rng = np.random.default_rng(7)
+    x = np.zeros((12, 64))
+    for r, e in enumerate((0, 20, -8, -12, -40, -120, 60, 90, 104, 127)):
+        x[r] = rng.standard_normal(64) * np.exp2(np.clip(np.log2(g) + e, -140, 126))
+    x[10, :16] = 1.5 * g
+    xt = torch.from_numpy(x).float().cuda()
+    assert torch.isfinite(xt).all()
+    check_operand(mx4.quantize(xt, "NVFP4", tensor_scale=g), xt, g)
+    for qw in (torch.ones(64, device="cuda"), torch.exp(torch.linspace(-3, 3, 64, device="cuda"))):
+        check_operand(mx4.quantize(xt, "NVFP4", qw, g), xt, g, qw)

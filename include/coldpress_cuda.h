@@ -311,7 +311,8 @@ int cp_mx4_matmul(int format, const uint8_t* a_codes, const uint8_t* a_scales, i
 
 /* transpose == 0: y[t][r] = alpha * sum_k x[t][k] w[r][k], x [T, n], y [T, rows].
  * transpose == 1: y[t][k] = alpha * sum_r x[t][r] w[r][k], x [T, rows], y [T, n] (the first
- * form's gradient with respect to x).  x and y are of `dtype`, x's rows ld elements apart.
+ * form's gradient with respect to x).  x and y are of `dtype`, x's rows ld elements apart.  x is taken as it
+ * is, but for float32 with transpose == 0 and T <= 16, whose values may be off by 2^-23 of themselves.
  * workspace >= cp_mx4_linear_workspace_bytes of the same arguments (it may be 0). */
 size_t cp_mx4_linear_workspace_bytes(int dtype, const void* x, int64_t T, int64_t ld, int64_t rows, int64_t n,
                                      int transpose);

@@ -417,8 +417,7 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
   }
 }
 
-// x [T, K] -> bf16 parts [parts][T][Kp] that sum to x exactly: each part takes the next 8 significant
-// bits (truncated, so no part overflows); of a NaN or infinity the first part holds it all.
+// x [T, K] -> bf16 parts [parts][T][Kp] that sum to x exactly.
 template <typename S>
 __global__ void __launch_bounds__(256) parts_kernel(const S* __restrict__ x, int64_t T, int64_t K, int64_t ld, int64_t Kp,
                                                     int parts, __nv_bfloat16* __restrict__ out) {
@@ -428,19 +427,11 @@ __global__ void __launch_bounds__(256) parts_kernel(const S* __restrict__ x, int
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) v[e] = k + e < K ? float(x[t * ld + k + e]) : 0.0f;
-    for (int p = 0; p < parts; p++) {
-      uint32_t w[4];
+    uint32_t w[3][4];
+    cut_bf16<3>(v, w);
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        uint32_t b = __float_as_uint(v[e]);
-        const bool odd = (b & 0x7F800000u) == 0x7F800000u;
-        if (odd && (b & 0x007FFFFFu)) b |= 0x00400000u;
-        b >>= 16;
-        v[e] = odd ? 0.0f : __fsub_rn(v[e], __uint_as_float(b << 16));
-        w[e / 2] = e & 1 ? w[e / 2] | b << 16 : b;
-      }
-      *reinterpret_cast<uint4*>(out + (p * T + t) * Kp + k) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+    for (int p = 0; p < 3; p++)
+      if (p < parts) *reinterpret_cast<uint4*>(out + (p * T + t) * Kp + k) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
   }
 }
 

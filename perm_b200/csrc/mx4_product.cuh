@@ -15,6 +15,23 @@ __device__ __forceinline__ void put_out(void* y, int dtype, int64_t i, float v) 
   else static_cast<float*>(y)[i] = v;
 }
 
+// Eight values as P bf16 parts each, in pairs: a part takes the next 8 significant bits (truncated, so no part
+// overflows), so that three sum to a float32 exactly and two to an f16; of a NaN or infinity the first part
+// holds it all.
+template <int P> __device__ __forceinline__ void cut_bf16(float (&v)[8], uint32_t (&w)[P][4]) {
+#pragma unroll
+  for (int p = 0; p < P; p++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      uint32_t b = __float_as_uint(v[e]);
+      const bool odd = (b & 0x7F800000u) == 0x7F800000u;
+      if (odd && (b & 0x007FFFFFu)) b |= 0x00400000u;
+      b >>= 16;
+      v[e] = odd ? 0.0f : __fsub_rn(v[e], __uint_as_float(b << 16));
+      w[p][e / 2] = e & 1 ? w[p][e / 2] | b << 16 : b;
+    }
+}
+
 // Stores N accumulator columns of a warp: lane = output row (row0 + lane of rows), register = token
 // (t0 + c of T); y is [T, rows].  Two-byte types: neighbouring lanes swap halves of a packed pair of
 // columns, so that a lane holds two rows of one token and stores four bytes; a store instruction
@@ -87,25 +104,30 @@ __device__ __forceinline__ void umma_bf16(uint32_t d, uint64_t ad, uint64_t bd, 
                  : "memory");
 }
 
-// Sums the partial tiles of a cluster of at most eight CTAs ([token][128 rows] float32 at the same place of
-// every CTA's shared memory) in rank order; this CTA takes its share of the tokens, a thread four rows
+// Sums the partial tiles of a cluster of at most eight CTAs ([part][token][128 rows] float32 at the same place of
+// every CTA's shared memory) in rank order, the smallest parts first; this CTA takes its share of the tokens, a thread four rows
 // at a time: the loads across the cluster are what this costs.
-__device__ __forceinline__ void join_partials(const void* part, int rank, int split, int cols, int64_t row0, int64_t t0,
+template <int P = 1>
+__device__ __forceinline__ void join_partials(const void* tile, int rank, int split, int cols, int64_t row0, int64_t t0,
                                               int64_t rows, float alpha, int dtype, void* y) {
   const int c0 = cols * rank / split, c1 = cols * (rank + 1) / split;
-  const uint32_t at = smem_u32(part);
+  const uint32_t at = smem_u32(tile);
   const int size = dtype == kMxF32 ? 4 : 2;
   const bool four = rows % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & (4 * size - 1)) == 0;
   for (int i = threadIdx.x + c0 * 32; i < c1 * 32; i += blockDim.x) {
     const int64_t row = row0 + (i & 31) * 4;
     if (row >= rows) continue;
-    float4 w[8], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // all loads ahead of the sum
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int p = 0; p < 8; p++)
-      if (p < split) w[p] = ld_cluster_f32x4(peer_addr(at + 16 * i, p));
+    for (int part = P - 1; part >= 0; part--) {
+      float4 w[8];   // all loads ahead of the sum
 #pragma unroll
-    for (int p = 0; p < 8; p++)
-      if (p < split) v.x += w[p].x, v.y += w[p].y, v.z += w[p].z, v.w += w[p].w;
+      for (int p = 0; p < 8; p++)
+        if (p < split) w[p] = ld_cluster_f32x4(peer_addr(at + 16 * (i + part * cols * 32), p));
+#pragma unroll
+      for (int p = 0; p < 8; p++)
+        if (p < split) v.x += w[p].x, v.y += w[p].y, v.z += w[p].z, v.w += w[p].w;
+    }
     v = make_float4(alpha * v.x, alpha * v.y, alpha * v.z, alpha * v.w);
     const int64_t to = (t0 + (i >> 5)) * rows + row;
     if (four) {

@@ -297,9 +297,10 @@ def _differentiated(x):
 
 
 def linear(x, w):
-    """x w^T: x [..., n] (bf16, f16 or f32, taken at its own precision), w [out, n] -> [..., out] in
-    x's type.  x gets a gradient (reverse and forward mode, also of second order; torch.func and vmap
-    raise); the weights are frozen."""
+    """x w^T: x [..., n] (bf16, f16 or f32), w [out, n] -> [..., out] in x's type.  x is taken as it is; only
+    float32 values of up to 16 rows may be off by a unit in the last place (2^-23).  NVFP4's sums are formed
+    before the tensor scale: |x| up to 2^100 keeps them finite.  x gets a gradient (reverse and forward mode,
+    also of second order; torch.func and vmap raise); the weights are frozen."""
     if _differentiated(x):
         return _Product.apply(x, w, 0)
     return _product(x, w, 0, "mx4.linear")

@@ -152,3 +152,107 @@ def test_weighted_blocks_far_from_the_tensor_scale(g):
     check_operand(mx4.quantize(xt, "NVFP4", tensor_scale=g), xt, g)
     for qw in (torch.ones(64, device="cuda"), torch.exp(torch.linspace(-3, 3, 64, device="cuda"))):
         check_operand(mx4.quantize(xt, "NVFP4", qw, g), xt, g, qw)
+
+
+# ------------------------------------------------------------------------------- activations at their own precision
+
+def picker(out, n, fmt, code, byte):
+    """Weights of one code in every row, each in another column, and zero elsewhere; the columns."""
+    b = mo.BLOCK[fmt]
+    nb = -(-n // b)
+    codes, col = np.zeros((out, nb, b), np.int64), np.random.default_rng(out + n).permutation(n)[np.arange(out) % n]
+    codes[np.arange(out), col // b, col % b] = code
+    c, s = mo.pack(codes, np.full((out, nb), byte), fmt, n)
+    return mx4.Mx4Tensor(torch.from_numpy(c).cuda(), torch.from_numpy(s).cuda(), fmt, out, n), torch.from_numpy(col).cuda()
+
+
+def wide(T, n, dtype, seed, span):
+    """Values of random significands with exponents spread over 2^-span .. 2^span."""
+    g = torch.Generator().manual_seed(seed)
+    e = torch.randint(-span, span + 1, (T, n), generator=g)
+    return (torch.randn(T, n, generator=g).double() * torch.exp2(e.double())).to(dtype).cuda()
+
+
+ONE = {"MXFP4": 127, "NVFP4": 0x38}     # the scale byte of 1
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,out,n", [(1, 300, 520), (2, 300, 520), (8, 300, 520), (16, 300, 520), (17, 300, 520), (130, 300, 520),
+                                     (600, 300, 520), (16, 8200, 2048), (3, 15000, 4096), (12, 130, 12000)])
+def test_every_value_of_x_counts(fmt, dtype, T, out, n):
+    """Each result is one value of x times one: what a row's large values take from its small ones, or a part of
+    a value that is left out, shows at once.  float32 rows of a narrow range with up to 16 tokens may be off
+    by a unit in the last place, 2^-23; all else is exact."""
+    dt = DTYPES[dtype]
+    w, col = picker(out, n, fmt, 2, ONE[fmt])
+    wide_span, narrow_span = (8, 3) if dt == torch.float16 else (55, 5)
+    x, z = wide(T, n, dt, T, wide_span), wide(T, n, dt, T + 1, narrow_span)
+    z = torch.where(z.abs() < 2.0 ** -7, torch.ones_like(z), z)      # narrow: 2^-7 to about 2^8
+    assert torch.equal(mx4.linear(x, w), x[:, col])
+    y = mx4.linear(z, w)
+    if dt == torch.float32 and T <= 16:
+        assert ((y.double() - z[:, col].double()).abs() <= 2.0 ** -23 * z[:, col].double().abs()).all()
+    else:
+        assert torch.equal(y, z[:, col])
+    for scale in (2.0 ** -90, 2.0 ** 90) if dt != torch.float16 else ():       # a narrow range far from 1
+        assert torch.equal(mx4.linear(z * scale, w), z[:, col] * scale)
+    if T > 1:                                                          # one wide row among narrow ones
+        m = z.clone()
+        m[T - 1] = x[T - 1]
+        assert torch.equal(mx4.linear(m, w)[T - 1], x[T - 1, col])
+    if out <= n:
+        dy = wide(T, out, dt, T + 2, wide_span)
+        want = torch.zeros((T, n), dtype=dt, device="cuda").index_copy(1, col, dy)
+        assert torch.equal(mx4.linear_grad(dy, w), want)
+    mx4.status()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("T", [1, 16, 17, 600])
+def test_products_near_the_end_of_float32(fmt, dtype, T):
+    """x at float32's end times a small weight is finite, for any number of tokens."""
+    dt = DTYPES[dtype]
+    w, col = picker(64, 256, fmt, 7, 127 - 6 if fmt == "MXFP4" else 8)           # 6 x 2^-6
+    x = torch.full((T, 256), 3e38, device="cuda").to(dt)
+    want = f64(x[:, :1]) * 6 * 2.0 ** -6
+    for v in (x, -x, x * 2.0 ** -245):
+        got = f64(mx4.linear(v, w))
+        want = f64(v[:, :1]) * 6 * 2.0 ** -6
+        # one rounding to the type; float32 values of one significand are as in the test above
+        assert (np.abs(got - want) <= (HALF[dt] + 2.0 ** -22) * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("T,out,n", [(1, 130, 600), (5, 130, 600), (16, 130, 600), (16, 8200, 2048)])
+def test_wide_rows_against_dense_weights(fmt, dtype, T, out, n):
+    """Rows that their units do not hold, with every weight set; a NaN and infinities among them."""
+    dt = DTYPES[dtype]
+    w, wv = operand(out, n, fmt, 11)
+    x = wide(T, n, dt, T, 40)
+    check_product(mx4.linear(x, w), f64(x), wv, dt)
+    x[0, 5] = float("inf")
+    y = f64(mx4.linear(x, w))
+    c = wv[:, 5]
+    assert (y[0][c > 0] == np.inf).all() and (y[0][c < 0] == -np.inf).all() and np.isnan(y[0][c == 0]).all()
+    check_product(mx4.linear(x, w)[1:], f64(x[1:]), wv, dt)
+    x[T - 1, 7] = float("nan")
+    assert torch.isnan(mx4.linear(x, w)[T - 1]).all()
+
+
+@pytest.mark.parametrize("T", [1, 16, 200])
+def test_small_values_beside_a_large_one_that_has_no_weight(T):
+    """The large value's column is zero in every row of the weights, so the tolerance knows the small ones only."""
+    for fmt in FMTS:
+        codes, byte = mo.quantize(0.05 * np.random.default_rng(7).standard_normal((64, 256)), fmt, 2.0 ** -12 if fmt == "NVFP4" else 1.0)
+        b = mo.BLOCK[fmt]
+        codes[:, 100 // b, 100 % b] = 0
+        c, s = mo.pack(codes, byte, fmt, 256)
+        w = mx4.Mx4Tensor(torch.from_numpy(c).cuda(), torch.from_numpy(s).cuda(), fmt, 64, 256)
+        for dt in DTYPES.values():
+            for big in (1e3, 6e4) if dt == torch.float16 else (1e3, 1e13, 1e30):
+                x = make_x(T, 256, 3, dt) * 2.0 ** -6
+                x[:, 100] = big
+                check_product(mx4.linear(x, w), f64(x), mo.values(codes, byte, fmt, 1.0, 256), dt)

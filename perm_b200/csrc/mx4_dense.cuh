@@ -9,8 +9,10 @@
 // kind::f16.  Each CTA loads, by TMA, its 128 rows of W and, for each part of x, half of the tokens,
 // 64 deep per stage; both CTAs' loads complete on the even CTA's barrier.  Two accumulators
 // alternate: eight epilogue warps read a finished one into registers while the MMAs go on in the other.
-// float32 results take a new accumulator every few steps and sum the chunks in those registers, because the
-// tensor core's own accumulation truncates.
+// float32 results take a new accumulator every step (12 MMAs, the smallest part of x first) and sum the
+// chunks in those registers, because the tensor core's own accumulation truncates: sums of positive products
+// come out low by 2^-24 on average; with three steps to a chain and the largest part first it was 2^-19
+// (4096 x 4096 -> 4096 348 us, was 340).
 #pragma once
 #include "mx4_product.cuh"
 
@@ -134,11 +136,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t ad = TR ? sw128_desc(sw, kBox / 2, 1024) : sw128_desc(sw, 16, 1024);
             const uint64_t bd = sw128_desc(sw + kBox, 16, 1024);
             if (elected) {
-              for (int p = 0; p < prm.parts; p++)
+              for (int p = prm.parts - 1; p >= 0; p--)   // the smallest part first: what truncation takes goes by the sum
 #pragma unroll
                 for (int kk = 0; kk < 4; kk++)   // 16 deep: 32 bytes of a K-major row, or 16 rows of 128
                   umma_bf16<true>(tmem + b * 256, ad + (TR ? 128 : 2) * kk, bd + p * (kBox / 16) + 2 * kk, kIdesc,
-                                  (uint32_t)(s - g0) | p | kk);
+                                  (uint32_t)(s - g0) | (p ^ (prm.parts - 1)) | kk);
               umma_commit_group<true>(empty0 + 8 * rg.st);
             }
             __syncwarp();

@@ -22,8 +22,9 @@
 // Work split, joins and bounded waits are those of the 4-bit products: SM pairs on 256 x 256 tiles
 // for many tokens, clusters over the reduction where there are few tiles (mx4_matmul.cu).  Two
 // accumulators alternate, so storing one tile overlaps the MMAs of the next.  float32 results restart the
-// accumulation every few steps and sum the chunks in round-to-nearest registers, because the tensor core's own
-// accumulation truncates.
+// accumulation every step (24 MMAs, the smallest part of x first) and sum the chunks in round-to-nearest
+// registers, because the tensor core's own accumulation truncates: sums of positive products come out low by 2^-24 on
+// average (2^-19 with the largest part first, which has the other parts' MMAs truncate the whole sum too).
 #include "mx4_dense.cuh"
 #include "mx4_product.cuh"
 
@@ -33,7 +34,7 @@ namespace {
 __device__ int g_status;
 
 constexpr unsigned long long kWaitNs = 1000000000ull;
-constexpr int kChunkSteps = 1;  // 128-deep steps of one float32 accumulation chain (24 MMAs with three parts)
+constexpr int kChunkSteps = 1;  // 128-deep steps of one float32 accumulation chain
 
 template <int FMT, int NT, bool PAIR, bool TR, bool CHUNK> struct Cfg {
   // warps: 0 x loads, 1 MMA, 2 code loads, 3 allocation, 4-7 epilogue, then groups of eight that decode
@@ -241,12 +242,12 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
             const uint64_t ad = TR ? sw128_desc(sa, 16384, 1024) : sw128_desc(sa, 16, 1024);
             const uint64_t bd = sw128_desc(sa + C::kA, 16, 1024);
             if (elected) {
-              for (int p = 0; p < prm.parts; p++)
+              for (int p = prm.parts - 1; p >= 0; p--)   // the smallest part first: what truncation takes goes by the sum
 #pragma unroll
                 for (int kk = 0; kk < 8; kk++)   // 16 deep: 32 bytes of a K-major row (four to a half), or 16 rows
                   umma_bf16<PAIR>(acc, ad + (TR ? 128 * kk : kk / 4 * 1024 + kk % 4 * 2),
                                   bd + p * (C::kB / 16) + kk / 4 * (C::kB / 32) + kk % 4 * 2, C::kIdesc,
-                                  (uint32_t)(s - g0) | p | kk);
+                                  (uint32_t)(s - g0) | (p ^ (prm.parts - 1)) | kk);
               umma_commit_group<PAIR>(empty0 + 8 * rg.st);
             }
             __syncwarp();
@@ -541,7 +542,7 @@ int launch_dense(const XView& x, int parts, int64_t T, const Mx4View& w, float a
   p.parts = parts;
   p.nst = dense::kRing / ((1 + parts) * dense::kBox);
   p.steps = (int)((x.K + 63) / 64);
-  p.chunk = dtype == kMxF32 ? 3 : p.steps;
+  p.chunk = dtype == kMxF32 ? 1 : p.steps;
   p.mtiles = (int)((p.out + 255) / 256);
   p.tiles = p.mtiles * (int)((T + 255) / 256);
   const int grid = 2 * std::min(p.tiles, device_sm_count() / 2);

@@ -256,3 +256,22 @@ def test_small_values_beside_a_large_one_that_has_no_weight(T):
                 x = make_x(T, 256, 3, dt) * 2.0 ** -6
                 x[:, 100] = big
                 check_product(mx4.linear(x, w), f64(x), mo.values(codes, byte, fmt, 1.0, 256), dt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("T", [1, 16, 40, 300, 600])
+def test_float32_sums_keep_their_size(fmt, T):
+    """Sums of positive products: truncation, which the tensor core's accumulation does, does not cancel here.  A chain
+    ends with at most 16 MMAs of x's largest part, each of which takes half a unit (2^-24) of a sum that is on
+    average half grown; chains are added with rounding.  16 2^-25 = 2^-21."""
+    rng = np.random.default_rng(T)
+    b, n, out = mo.BLOCK[fmt], 1024, 256
+    codes = rng.integers(1, 8, (out, n // b, b))
+    byte = rng.integers(125, 130, (out, n // b)) if fmt == "MXFP4" else rng.integers(0x30, 0x48, (out, n // b))
+    c, s = mo.pack(codes, byte, fmt, n)
+    w = mx4.Mx4Tensor(torch.from_numpy(c).cuda(), torch.from_numpy(s).cuda(), fmt, out, n)
+    wv = mo.values(codes, byte, fmt)
+    x = torch.from_numpy(0.5 + rng.random((T, n))).float().cuda()
+    dy = torch.from_numpy(0.5 + rng.random((T, out))).float().cuda()
+    for got, want in ((mx4.linear(x, w), f64(x) @ wv.T), (mx4.linear_grad(dy, w), f64(dy) @ wv)):
+        assert abs((f64(got) / want - 1).mean()) <= 2.0 ** -21

@@ -18,6 +18,13 @@
 // 14336 (NVFP4) took 288 us with one-SM tiles.  Both CTAs need the scales of all the tile's
 // tokens.  The loads of both complete on the even CTA's barrier; its MMA warp issues for both.
 //
+// float32 results take the whole reduction in one chain of accumulations too, although each truncates: a product
+// of two 4-bit values and their scales has few bits, so most additions are exact, and a chain has a quarter of the
+// steps that it has with bf16.  Sums of positive products with block scales spread over 2^16 come out low
+// by 2^-22 (4096 columns) to 2^-20 (14336) on average, which is what a float32 sum in another order is off by at
+// its worst places.  Restarting every 16 MMAs made that 2^-22 for any length and cost 55 -> 149 us (2048 x 14336
+// -> 4096): there is no room for a second accumulator, and the sums take all registers.
+//
 // The accumulator (256 columns) and the scales do not fit into tensor memory twice, so there is one
 // accumulator: eight epilogue warps read it into registers at once and hand it back before they
 // convert and store, while the next tile's MMAs run.

@@ -320,6 +320,13 @@ int cp_mx4_linear(int format, int dtype, const void* x, int64_t T, int64_t ld, c
                   const uint8_t* scales, int64_t rows, int64_t n, float alpha, int transpose, void* y,
                   void* workspace, size_t ws_bytes, void* stream);
 
+/* Failure-path testing of the products' bounded waits: arms the calling thread's NEXT cp_mx4_matmul or
+ * cp_mx4_linear so that each CTA leaves out its load step `skip_step` (counted from 0; 256 columns of both
+ * operands, 128 of x, 64 of both or 256 of the weights, by kernel) and every wait gives up after wait_ns
+ * (1 ms .. 2 s).  The kernel then stops, drains the loads that it issued, frees its tensor memory and sets
+ * the status word; the device stays usable.  One call only. */
+int cp_mx4_inject_stall(int skip_step, int64_t wait_ns);
+
 /* Synchronises `stream`, reads and clears the current device's status word: CP_OK, or
  * CP_ERR_TIMEOUT when a wait inside an earlier cp_mx4_matmul or cp_mx4_linear ran out (its
  * result is then incomplete). */

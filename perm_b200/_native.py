@@ -128,6 +128,7 @@ def lib():
         "cp_mx4_matmul": ([I, P, P, I64, P, P, I64, I64, F, I, P, P], I),
         "cp_mx4_linear_workspace_bytes": ([I, P, I64, I64, I64, I64, I], SZ),
         "cp_mx4_linear": ([I, I, P, I64, I64, P, P, I64, I64, F, I, P, P, SZ, P], I),
+        "cp_mx4_inject_stall": ([I, I64], I),
         "cp_mx4_status": ([P], I),
     }
     for name, (args, res) in sig.items():

@@ -22,6 +22,9 @@ thread_local char g_err[512] = "";
 // cp_xtx_inject_stall: armed for the calling thread's next cp_xtx_accumulate only
 thread_local int g_xtx_stall_step = -1;
 thread_local int64_t g_xtx_stall_wait_ns = 0;
+// cp_mx4_inject_stall: armed for the calling thread's next 4-bit product only
+constexpr cpk::Mx4Waits kMx4Waits{1000000000ull, -1};
+thread_local cpk::Mx4Waits g_mx4_waits = kMx4Waits;
 
 int set_err(int code, const char* msg) {
   std::snprintf(g_err, sizeof(g_err), "%s", msg);
@@ -118,6 +121,12 @@ EfLayout ef_layout(int t, int64_t nrow, int64_t n) {
 }
 
 }  // namespace
+
+cpk::Mx4Waits cpk::mx4_take_waits() {
+  const Mx4Waits w = g_mx4_waits;
+  g_mx4_waits = kMx4Waits;
+  return w;
+}
 
 extern "C" {
 
@@ -772,6 +781,13 @@ int cp_mx4_linear(int fmt, int dtype, const void* x, int64_t T, int64_t ld, cons
   return mx4_rc(cpk::launch_mx4_linear(dtype, x, T, ld, mx4_x_aligned(dtype, x, T, ld), w, alpha, transpose, y, workspace,
                                        (cudaStream_t)stream),
                 "cp_mx4_linear");
+}
+
+int cp_mx4_inject_stall(int skip_step, int64_t wait_ns) {
+  if (skip_step < 0 || wait_ns < 1000000 || wait_ns > 2000000000LL)
+    return set_err(CP_ERR_ARG, "cp_mx4_inject_stall: skip_step >= 0 and 1 ms <= wait_ns <= 2 s");
+  g_mx4_waits = cpk::Mx4Waits{(unsigned long long)wait_ns, skip_step};
+  return CP_OK;
 }
 
 int cp_mx4_status(void* stream) {

@@ -19,7 +19,6 @@
 namespace cpk {
 namespace dense {
 
-constexpr unsigned long long kWaitNs = 1000000000ull;
 constexpr int kThreads = 320;   // warps: 0 loads, 1 MMA, 2-9 epilogue (two per lane quarter, 128 columns each)
 constexpr int kBox = 128 * 128;                 // 128 rows x 64, or 64 rows x 128 as two boxes: bf16
 constexpr int kRing = 7 * 2 * kBox;
@@ -35,6 +34,7 @@ struct Params {
   int parts, nst;
   int steps, chunk;     // 64-deep steps; steps of one accumulation chain
   int mtiles, tiles;
+  Mx4Waits waits;
 };
 
 template <bool TR>
@@ -85,20 +85,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int tile = first; ok && tile < prm.tiles; tile += stride) {
         const int m0 = tile % prm.mtiles * 256 + rank * 128, t0 = tile / prm.mtiles * 256 + rank * 128;
         for (int s = 0; s < prm.steps; s++, loads++) {
-          if (loads >= nst && !mbar_wait(empty0 + 8 * rg.st, rg.ph ^ 1, abort, kWaitNs)) {
+          if (loads >= nst && !mbar_wait(empty0 + 8 * rg.st, rg.ph ^ 1, abort, prm.waits.ns)) {
             ok = false;
             break;
           }
-          const uint32_t fb = lead_full + 8 * rg.st, sw = ring + rg.st * stage_bytes;
-          if (leader) mbar_expect_tx(full0 + 8 * rg.st, 2 * stage_bytes);
-          if (TR) {
-            tma_load_pair(sw, &map_w, m0, s * 64, fb);
-            tma_load_pair(sw + kBox / 2, &map_w, m0 + 64, s * 64, fb);
-          } else {
-            tma_load_pair(sw, &map_w, s * 64, m0, fb);
+          if (loads != prm.waits.skip) {
+            const uint32_t fb = lead_full + 8 * rg.st, sw = ring + rg.st * stage_bytes;
+            if (leader) mbar_expect_tx(full0 + 8 * rg.st, 2 * stage_bytes);
+            if (TR) {
+              tma_load_pair(sw, &map_w, m0, s * 64, fb);
+              tma_load_pair(sw + kBox / 2, &map_w, m0 + 64, s * 64, fb);
+            } else {
+              tma_load_pair(sw, &map_w, s * 64, m0, fb);
+            }
+            for (int p = 0; p < prm.parts; p++)
+              tma_load_pair(sw + (1 + p) * kBox, &map_x, s * 64, (int)(p * prm.T) + t0, fb);
           }
-          for (int p = 0; p < prm.parts; p++)
-            tma_load_pair(sw + (1 + p) * kBox, &map_x, s * 64, (int)(p * prm.T) + t0, fb);
           rg.advance(nst);
         }
       }
@@ -108,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = min(loads, nst); k > 0; k--) {
         rg.back(nst);
         int zero = 0;
-        mbar_wait((leader ? full0 : empty0) + 8 * rg.st, rg.ph, &zero, kWaitNs);
+        mbar_wait((leader ? full0 : empty0) + 8 * rg.st, rg.ph, &zero, prm.waits.ns);
       }
     }
   } else if (warp == 1) {
@@ -122,12 +124,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int tile = first; ok && tile < prm.tiles; tile += stride)
         for (int g0 = 0; ok && g0 < prm.steps; cg++) {
           const int b = cg & 1, g1 = min(prm.steps, g0 + prm.chunk);
-          if (cg >= 2 && !mbar_wait_warp(acce + 8 * b, ((cg >> 1) - 1) & 1, abort, kWaitNs)) {
+          if (cg >= 2 && !mbar_wait_warp(acce + 8 * b, ((cg >> 1) - 1) & 1, abort, prm.waits.ns)) {
             ok = false;
             break;
           }
           for (int s = g0; s < g1; s++) {
-            if (!mbar_wait_warp(full0 + 8 * rg.st, rg.ph, abort, kWaitNs)) {
+            if (!mbar_wait_warp(full0 + 8 * rg.st, rg.ph, abort, prm.waits.ns)) {
               ok = false;
               break;
             }
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) fail_pair(abort, peer_abort, prm.status);
       if (elected) umma_commit_group<true>(done);   // all MMAs complete before tensor memory is freed
       int zero = 0;
-      mbar_wait(done, 0, &zero, kWaitNs);
+      mbar_wait(done, 0, &zero, prm.waits.ns);
     }
   } else {
     const int q = warp & 3, hh = (warp - 2) >> 2;
@@ -165,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m[128];
       for (int g0 = 0; g0 < prm.steps; g0 += prm.chunk, cg++) {
         const int b = cg & 1;
-        if (!mbar_wait_warp(accf + 8 * b, (cg >> 1) & 1, abort, kWaitNs)) {
+        if (!mbar_wait_warp(accf + 8 * b, (cg >> 1) & 1, abort, prm.waits.ns)) {
           ok = false;
           break;
         }

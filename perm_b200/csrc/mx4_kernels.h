@@ -50,6 +50,14 @@ size_t mx4_stream_workspace_bytes(int dtype, int64_t T, int64_t rows, int64_t n)
 int launch_mx4_stream(int dtype, const void* x, int64_t T, int64_t ld, int aligned, const Mx4View& w, float alpha, void* y,
                       void* ws, cudaStream_t stream);
 
+// Bound of every wait of the calling thread's next product, and (failure-path tests) the load step that each CTA
+// leaves out of it; -1: none.
+struct Mx4Waits {
+  unsigned long long ns;
+  int skip;
+};
+Mx4Waits mx4_take_waits();
+
 // Status words of the products' bounded waits (read and cleared; synchronises the stream).
 int mx4_matmul_status(cudaStream_t stream, int* status);
 int mx4_linear_status(cudaStream_t stream, int* status);

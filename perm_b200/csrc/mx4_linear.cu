@@ -33,7 +33,6 @@ namespace {
 
 __device__ int g_status;
 
-constexpr unsigned long long kWaitNs = 1000000000ull;
 constexpr int kChunkSteps = 1;  // 128-deep steps of one float32 accumulation chain
 
 template <int FMT, int NT, bool PAIR, bool TR, bool CHUNK> struct Cfg {
@@ -78,6 +77,7 @@ struct LinParams {
   int steps;            // 128-deep steps of the reduction
   int groups;           // scale tiles per 128 rows of w
   int mtiles, tiles;
+  Mx4Waits waits;
 };
 
 // Eight codes times a block scale -> eight bf16 values in pairs.
@@ -160,17 +160,19 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
       for (int tile = first; ok && tile < prm.tiles; tile += stride) {
         const int t0 = tile / prm.mtiles * NT + (PAIR ? rank * C::kXRows : 0);
         for (int s = s_begin; s < s_end; s++, loads++) {
-          if (loads >= nst && !mbar_wait(empty0 + 8 * rg.st, rg.ph ^ 1, abort, kWaitNs)) {
+          if (loads >= nst && !mbar_wait(empty0 + 8 * rg.st, rg.ph ^ 1, abort, prm.waits.ns)) {
             ok = false;
             break;
           }
-          if (leader) mbar_expect_tx(full0 + 8 * rg.st, (PAIR ? 2 : 1) * prm.parts * C::kB);
-          const uint32_t sx = ring + rg.st * stage_bytes + C::kA;
-          for (int p = 0; p < prm.parts; p++)
+          if (loads != prm.waits.skip) {
+            if (leader) mbar_expect_tx(full0 + 8 * rg.st, (PAIR ? 2 : 1) * prm.parts * C::kB);
+            const uint32_t sx = ring + rg.st * stage_bytes + C::kA;
+            for (int p = 0; p < prm.parts; p++)
 #pragma unroll
-            for (int k = 0; k < 2; k++)
-              tma_load_group<PAIR>(sx + p * C::kB + k * (C::kB / 2), &map_x, s * 128 + k * 64, (int)(p * prm.T) + t0,
-                                   lead_full + 8 * rg.st);
+              for (int k = 0; k < 2; k++)
+                tma_load_group<PAIR>(sx + p * C::kB + k * (C::kB / 2), &map_x, s * 128 + k * 64, (int)(p * prm.T) + t0,
+                                     lead_full + 8 * rg.st);
+          }
           rg.advance(nst);
         }
       }
@@ -180,7 +182,7 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
       // full barriers, so wait as long as a load could take.
       for (int k = min(loads, nst); ok && k > 0; k--) {
         rg.back(nst);
-        ok = mbar_wait(empty0 + 8 * rg.st, rg.ph, abort, kWaitNs);
+        ok = mbar_wait(empty0 + 8 * rg.st, rg.ph, abort, prm.waits.ns);
       }
       if (!ok) {
         const unsigned long long t0 = gtime();
@@ -196,7 +198,7 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
         const int m0 = (int)tile_row(tile);
         for (int s = s_begin; s < s_end; s++, it++, rc.advance(prm.ncs)) {
           const int st = rc.st;
-          if (it >= prm.ncs && !mbar_wait(cempty + 8 * st, rc.ph ^ 1, abort, kWaitNs)) {
+          if (it >= prm.ncs && !mbar_wait(cempty + 8 * st, rc.ph ^ 1, abort, prm.waits.ns)) {
             ok = false;
             break;
           }
@@ -215,7 +217,7 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
       for (int k = min(it, prm.ncs); k > 0; k--) {
         int zero = 0;
         rc.back(prm.ncs);
-        mbar_wait(cfull + 8 * rc.st, rc.ph, &zero, kWaitNs);
+        mbar_wait(cfull + 8 * rc.st, rc.ph, &zero, prm.waits.ns);
       }
     }
   } else if (warp == 1) {
@@ -228,12 +230,12 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
         for (int g0 = s_begin; ok && g0 < s_end; cg++) {
           const int b = cg & 1, g1 = CHUNK ? min(s_end, g0 + kChunkSteps) : s_end;
           const uint32_t acc = tmem + b * NT;
-          if (cg >= 2 && !mbar_wait_warp(acce + 8 * b, ((cg >> 1) - 1) & 1, abort, kWaitNs)) {
+          if (cg >= 2 && !mbar_wait_warp(acce + 8 * b, ((cg >> 1) - 1) & 1, abort, prm.waits.ns)) {
             ok = false;
             break;
           }
           for (int s = g0; s < g1; s++) {
-            if (!mbar_wait_warp<PAIR>(full0 + 8 * rg.st, rg.ph, abort, kWaitNs)) {
+            if (!mbar_wait_warp<PAIR>(full0 + 8 * rg.st, rg.ph, abort, prm.waits.ns)) {
               ok = false;
               break;
             }
@@ -261,7 +263,7 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
       if (!ok) fail();
       if (elected) umma_commit_group<PAIR>(done);   // all MMAs complete before tensor memory is freed
       int zero = 0;
-      mbar_wait(done, 0, &zero, kWaitNs);
+      mbar_wait(done, 0, &zero, prm.waits.ns);
     }
   } else if (warp >= 8) {
     // ---- decoding.  Groups take steps in turn, so one group's waits and fences overlap the others' work; a
@@ -280,7 +282,7 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
       for (int s = s_begin; s < s_end; s++, seen++, rg.advance(nst), rc.advance(prm.ncs), turn.advance(prm.turns)) {
         if (turn.st != g) continue;
         const int cs = rc.st;
-        if (!mbar_wait_warp(cfull + 8 * cs, rc.ph, abort, kWaitNs)) {
+        if (!mbar_wait_warp(cfull + 8 * cs, rc.ph, abort, prm.waits.ns)) {
           ok = false;
           break;
         }
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
             const uint4& qq = q[i / 4];
             decode8(i % 4 == 0 ? qq.x : i % 4 == 1 ? qq.y : i % 4 == 2 ? qq.z : qq.w, f[i / 2], v[i]);
           }
-          if (seen >= nst && !mbar_wait_warp(empty0 + 8 * rg.st, rg.ph ^ 1, abort, kWaitNs)) {
+          if (seen >= nst && !mbar_wait_warp(empty0 + 8 * rg.st, rg.ph ^ 1, abort, prm.waits.ns)) {
             ok = false;
             break;
           }
@@ -352,7 +354,7 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
           for (int e = 0; e < 16; e++) m[c][e] = 0.0f;
         for (int g0 = s_begin; g0 < s_end; g0 += kChunkSteps, cg++) {
           const int b = cg & 1;
-          if (!mbar_wait_warp(accf + 8 * b, (cg >> 1) & 1, abort, kWaitNs)) {
+          if (!mbar_wait_warp(accf + 8 * b, (cg >> 1) & 1, abort, prm.waits.ns)) {
             ok = false;
             break;
           }
@@ -377,7 +379,7 @@ __global__ void __launch_bounds__((Cfg<FMT, NT, PAIR, TR, CHUNK>::kThreads), 1)
         }
       } else {
         const int b = cg & 1;
-        if (!mbar_wait_warp(accf + 8 * b, (cg >> 1) & 1, abort, kWaitNs)) {
+        if (!mbar_wait_warp(accf + 8 * b, (cg >> 1) & 1, abort, prm.waits.ns)) {
           ok = false;
           break;
         }
@@ -468,6 +470,7 @@ int launch_tiles(const XView& x, int parts, int64_t T, const Mx4View& w, float a
   const int64_t mt = (p.out + 127) / 128;
   p.mtiles = (int)(PAIR ? (mt + 1) / 2 : mt);
   p.tiles = p.mtiles * (int)((T + NT - 1) / NT);
+  p.waits = mx4_take_waits();
   const int sms = device_sm_count();
   const int grid = PAIR ? 2 * std::min(p.tiles, sms / 2) : split > 1 ? p.tiles * split : std::min(p.tiles, sms);
   return launch_cluster<mx4_linear_kernel<FMT, NT, PAIR, TR, CHUNK>>(grid, C::kThreads, C::kSmem, PAIR ? 2 : split, stream, mw,
@@ -545,6 +548,7 @@ int launch_dense(const XView& x, int parts, int64_t T, const Mx4View& w, float a
   p.chunk = dtype == kMxF32 ? 1 : p.steps;
   p.mtiles = (int)((p.out + 255) / 256);
   p.tiles = p.mtiles * (int)((T + 255) / 256);
+  p.waits = mx4_take_waits();
   const int grid = 2 * std::min(p.tiles, device_sm_count() / 2);
   return transpose ? launch_cluster<dense::dense_kernel<true>>(grid, dense::kThreads, dense::kSmem, 2, stream, mw, mx, p)
                    : launch_cluster<dense::dense_kernel<false>>(grid, dense::kThreads, dense::kSmem, 2, stream, mw, mx, p);

@@ -45,7 +45,6 @@ namespace {
 
 __device__ int g_status;
 
-constexpr unsigned long long kWaitNs = 1000000000ull;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 
@@ -75,6 +74,7 @@ struct MmParams {
   int dtype;
   int steps;            // 256-column steps
   int mtiles, tiles;    // weight tiles; weight tiles x token tiles
+  Mx4Waits waits;
 };
 
 // Shared-memory descriptor of a scale tile for tcgen05.cp: no swizzle, 8 x 16-byte cores 128 bytes apart.
@@ -167,10 +167,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int row = (int)tile_row(tile), t0 = tile / prm.mtiles * NT;
         for (int s = s_begin; s < s_end; s++, it++) {
           const int st = it % C::kStages, round = it / C::kStages;
-          if (round > 0 && !mbar_wait(empty0 + 8 * st, (round - 1) & 1, abort, kWaitNs)) {
+          if (round > 0 && !mbar_wait(empty0 + 8 * st, (round - 1) & 1, abort, prm.waits.ns)) {
             ok = false;
             break;
           }
+          if (it == prm.waits.skip) continue;
           const uint32_t fb = lead_full0 + 8 * st, sw = ring + st * C::kStage, sx = sw + C::kWBytes, ss = sx + C::kXBytes;
           // boxes past the arrays' ends arrive as zeros and count in full
           if (leader) mbar_expect_tx(full0 + 8 * st, (PAIR ? 2 : 1) * C::kStage);
@@ -187,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // odd one the MMAs that consumed its loads (or the wait's bound)
       for (int k = max(0, it - C::kStages); k < it; k++) {
         int zero = 0;
-        mbar_wait((leader ? full0 : empty0) + 8 * (k % C::kStages), (k / C::kStages) & 1, &zero, kWaitNs);
+        mbar_wait((leader ? full0 : empty0) + 8 * (k % C::kStages), (k / C::kStages) & 1, &zero, prm.waits.ns);
       }
     }
   } else if (warp == 1) {
@@ -196,13 +197,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       int it = 0, n = 0;
       bool ok = true;
       for (int tile = first; ok && tile < prm.tiles; tile += stride, n++) {
-        if (n > 0 && !mbar_wait_warp(acce, (n - 1) & 1, abort, kWaitNs)) {
+        if (n > 0 && !mbar_wait_warp(acce, (n - 1) & 1, abort, prm.waits.ns)) {
           ok = false;
           break;
         }
         for (int s = s_begin; s < s_end; s++, it++) {
           const int st = it % C::kStages;
-          if (!mbar_wait_warp(full0 + 8 * st, (it / C::kStages) & 1, abort, kWaitNs)) {
+          if (!mbar_wait_warp(full0 + 8 * st, (it / C::kStages) & 1, abort, prm.waits.ns)) {
             ok = false;
             break;
           }
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // all MMAs complete before tensor memory is freed and before the other CTA may exit
       if (elected) umma_commit_group<PAIR>(done);
       int zero = 0;
-      mbar_wait(done, 0, &zero, kWaitNs);
+      mbar_wait(done, 0, &zero, prm.waits.ns);
     }
   } else {
     const int q = warp & 3, hh = (warp - 2) >> 2;
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lead_acce = PAIR ? peer_addr(acce, 0) : acce;
     int n = 0;
     for (int tile = first; tile < prm.tiles; tile += stride, n++) {
-      if (!mbar_wait_warp(accf, n & 1, abort, kWaitNs)) {
+      if (!mbar_wait_warp(accf, n & 1, abort, prm.waits.ns)) {
         fail();
         break;
       }
@@ -304,6 +305,7 @@ int launch_tiles(const Mx4View& a, const Mx4View& w, float alpha, int dtype, voi
   p.steps = (int)steps;
   p.mtiles = (int)(PAIR ? (wt + 1) / 2 : wt);
   p.tiles = p.mtiles * (int)((a.rows + NT - 1) / NT);
+  p.waits = mx4_take_waits();
   const int sms = device_sm_count();
   const int grid = PAIR ? 2 * std::min(p.tiles, sms / 2) : split > 1 ? p.tiles * split : std::min(p.tiles, sms);
   return launch_cluster<mx4_matmul_kernel<FMT, NT, PAIR>>(grid, kThreads, C::kSmem, PAIR ? 2 : split, stream, mw, mx, msw,

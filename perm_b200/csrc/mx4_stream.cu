@@ -42,7 +42,6 @@ namespace {
 
 __device__ int g_status;
 
-constexpr unsigned long long kWaitNs = 1000000000ull;
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * (kWarps + 1);   // the last warp loads
 constexpr int kMaxStages = 6;
@@ -60,6 +59,7 @@ struct StreamParams {
   const void* units;    // x as convert_kernel left it
   const uint32_t* top;  // its rows' largest magnitudes
   int64_t pitch;        // and its bytes per row
+  Mx4Waits waits;
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t a, uint32_t (&r)[4]) {
@@ -332,21 +332,23 @@ __global__ void __launch_bounds__(kThreads, 2)
       bool ok = true;
       int loads = 0;
       for (int s = s_begin; s < s_end; s++, loads++) {
-        if (loads >= nst && !mbar_wait(empty0 + 8 * rg.st, rg.ph ^ 1, abort, kWaitNs)) {
+        if (loads >= nst && !mbar_wait(empty0 + 8 * rg.st, rg.ph ^ 1, abort, prm.waits.ns)) {
           ok = false;
           break;
         }
         const uint32_t fb = full0 + 8 * rg.st, sw = ring + rg.st * kStage;
-        mbar_expect_tx(fb, kStage);
-        tma_load(sw, &map_w, s * 128, tile * 128, fb);
-        tma_load(sw + 128 * 128, &map_s, 0, tile * prm.groups + s * kAtoms, fb);
+        if (loads != prm.waits.skip) {
+          mbar_expect_tx(fb, kStage);
+          tma_load(sw, &map_w, s * 128, tile * 128, fb);
+          tma_load(sw + 128 * 128, &map_s, 0, tile * prm.groups + s * kAtoms, fb);
+        }
         rg.advance(nst);
       }
       if (!ok) fail_cta(abort, &g_status);
       for (int k = min(loads, nst); k > 0; k--) {   // every load issued lands before the CTA goes on
         rg.back(nst);
         int zero = 0;
-        mbar_wait(full0 + 8 * rg.st, rg.ph, &zero, kWaitNs);
+        mbar_wait(full0 + 8 * rg.st, rg.ph, &zero, prm.waits.ns);
       }
     }
   } else {
@@ -447,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       constexpr bool kBlocks = !EXACT && FMT == kMXFP4;   // sums of one block
       constexpr int Q = EXACT && P > 1 ? 3 : 1, NBX = EXACT ? (NB + P - 1) / P : NB;
       for (int s = s_begin; s < s_end; s++) {
-        if (!mbar_wait_warp(full0 + 8 * rg.st, rg.ph, abort, kWaitNs)) return false;
+        if (!mbar_wait_warp(full0 + 8 * rg.st, rg.ph, abort, prm.waits.ns)) return false;
         const uint32_t sw = ring + rg.st * kStage;
         const uint32_t sc = sw + 128 * 128;
         const uint32_t xcol = (s - s_begin) * 512;
@@ -694,6 +696,7 @@ int launch_mx4_stream(int dtype, const void* x, int64_t T, int64_t ld, int align
   p.slice = plan.slice;
   p.groups = steps * (w.fmt == kMXFP4 ? 2 : 4);
   p.vec = aligned;
+  p.waits = mx4_take_waits();
   if (w.fmt == kMXFP4) {
     if (dtype == kMxBF16) return launch_type<kMXFP4, __nv_bfloat16>(p, w, plan.split, plan.convert, ws, stream);
     if (dtype == kMxF16) return launch_type<kMXFP4, __half>(p, w, plan.split, plan.convert, ws, stream);

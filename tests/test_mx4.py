@@ -272,3 +272,9 @@ def test_status_of_a_device_without_a_number_is_the_current_devices(monkeypatch)
     for dev in (None, "cuda", torch.device("cuda"), "cuda:1", torch.device("cuda", 0)):
         mx4.status(dev)
     assert asked == [3, 3, 3, 1, 0]
+
+
+def test_inject_stall_checks_its_arguments():
+    L = nat.lib()
+    for skip, wait in ((-1, 5_000_000), (0, 10), (0, 999_999), (0, 2_000_000_001)):
+        assert L.cp_mx4_inject_stall(skip, wait) == nat.CP_ERR_ARG

@@ -275,3 +275,36 @@ def test_float32_sums_keep_their_size(fmt, T):
     dy = torch.from_numpy(0.5 + rng.random((T, out))).float().cuda()
     for got, want in ((mx4.linear(x, w), f64(x) @ wv.T), (mx4.linear_grad(dy, w), f64(dy) @ wv)):
         assert abs((f64(got) / want - 1).mean()) <= 2.0 ** -21
+
+
+# ------------------------------------------------------------------------------- waits that run out
+
+STALLS = [("matmul", "MXFP4", "bf16", 5, 300, 2048, 0), ("matmul", "NVFP4", "f32", 100, 300, 2048, 0),
+          ("matmul", "NVFP4", "bf16", 600, 4000, 4096, 11),
+          ("linear", "MXFP4", "bf16", 1, 300, 2048, 0), ("linear", "NVFP4", "f32", 16, 8200, 2048, 1), ("linear", "MXFP4", "f16", 9, 130, 512, 0),
+          ("linear", "MXFP4", "bf16", 40, 520, 2048, 0), ("linear", "NVFP4", "f32", 40, 520, 2048, 1),
+          ("linear", "MXFP4", "bf16", 512, 14340, 1024, 7), ("linear", "NVFP4", "f16", 512, 14340, 1024, 0),
+          ("linear", "MXFP4", "bf16", 600, 1030, 2048, 9), ("linear", "NVFP4", "f32", 600, 1030, 2048, 0),
+          ("grad", "MXFP4", "bf16", 3, 520, 2048, 0), ("grad", "NVFP4", "bf16", 200, 2048, 520, 1), ("grad", "MXFP4", "bf16", 600, 1030, 2048, 8)]
+
+
+@pytest.mark.parametrize("call,fmt,dtype,T,out,n,skip", STALLS)
+def test_a_wait_that_runs_out_is_reported(call, fmt, dtype, T, out, n, skip):
+    """The failure paths of the products' bounded waits, made on the host: the next call leaves out one step of its
+    loads and every wait gives up after 5 ms.  The kernel stops, status() says so once, and the next call is right."""
+    dt = DTYPES[dtype]
+    w, wv = operand(out, n, fmt, out + n)
+    if call == "matmul":
+        a, av = operand(T, n, fmt, T + n, 2.0 ** -10 if fmt == "NVFP4" else 1.0)
+        run, x, m = (lambda: mx4.matmul(a, w, dt)), av, wv
+    else:
+        xt = make_x(T, n if call == "linear" else out, T + out, dt, 0.5)
+        run, x, m = (lambda: (mx4.linear if call == "linear" else mx4.linear_grad)(xt, w)), f64(xt), wv if call == "linear" else wv.T
+    check_product(run(), x, m, dt)
+    mx4.status()
+    assert nat.lib().cp_mx4_inject_stall(skip, 5_000_000) == nat.CP_OK
+    run()
+    with pytest.raises(nat.CudaPathError, match="ran out"):
+        mx4.status()
+    check_product(run(), x, m, dt)
+    mx4.status()

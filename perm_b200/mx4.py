@@ -121,10 +121,8 @@ class Mx4Tensor:
         return (self._codes, self._scales) if self._buf is None else (self._buf,)
 
     def _over(self, tensors):
-        """This operand over tensors in the place of its own."""
-        if tensors[0] is self._tensors()[0]:
-            return self
-        if self._buf is None:
+        """This operand over tensors in the place of its own (all of _tensors())."""
+        if len(tensors) == 2:
             return Mx4Tensor(*tensors, *self._rest())
         return Mx4Tensor._new(tensors[0], *self._rest(), buf=tensors[0])
 
@@ -274,15 +272,16 @@ class _Product(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, transpose):
         ctx.w, ctx.transpose = w, transpose
-        own = w._tensors()
-        ctx.saved = not own[0].is_inference()   # those have no version and cannot be saved
-        if ctx.saved:
-            ctx.save_for_backward(*own)
+        own = w._buf if w._codes is None else w._codes
+        if not own.is_inference():   # those have no version and cannot be saved
+            ctx.save_for_backward(*w._tensors())
         return _product(x, w, transpose, "mx4.linear_grad" if transpose else "mx4.linear")
 
     @staticmethod
     def backward(ctx, dy):
-        w = ctx.w._over(ctx.saved_tensors) if ctx.saved else ctx.w   # raises if the weights were written since
+        w, saved = ctx.w, ctx.saved_tensors   # raises if the weights were written since
+        if saved and saved[0] is not (w._codes if w._buf is None else w._buf):
+            w = w._over(saved)
         if torch.is_grad_enabled() or _forward._current_level >= 0:   # create_graph, or dy has a tangent: a gradient itself
             return _Product.apply(dy, w, 1 - ctx.transpose), None, None
         return _product(dy, w, 1 - ctx.transpose, "mx4.linear (backward)"), None, None
@@ -292,23 +291,19 @@ class _Product(torch.autograd.Function):
         return _Product.apply(tangent, ctx.w, ctx.transpose)
 
 
-def _differentiated(x):
-    return _forward._current_level >= 0 or x.requires_grad and torch.is_grad_enabled()
-
-
 def linear(x, w):
     """x w^T: x [..., n] (bf16, f16 or f32), w [out, n] -> [..., out] in x's type.  x is taken as it is; only
     float32 values of up to 16 rows may be off by a unit in the last place (2^-23).  NVFP4's sums are formed
     before the tensor scale: |x| up to 2^100 keeps them finite.  x gets a gradient (reverse and forward mode,
     also of second order; torch.func and vmap raise); the weights are frozen."""
-    if _differentiated(x):
+    if x.requires_grad and torch.is_grad_enabled() or _forward._current_level >= 0:
         return _Product.apply(x, w, 0)
     return _product(x, w, 0, "mx4.linear")
 
 
 def linear_grad(dy, w):
     """The gradient of linear(x, w) with respect to x: dy w, dy [..., out] -> [..., n]."""
-    if _differentiated(dy):
+    if dy.requires_grad and torch.is_grad_enabled() or _forward._current_level >= 0:
         return _Product.apply(dy, w, 1)
     return _product(dy, w, 1, "mx4.linear_grad")
 

@@ -38,8 +38,8 @@ constexpr int kChunkSteps = 1;  // 128-deep steps of one float32 accumulation ch
 template <int FMT, int NT, bool PAIR, bool TR, bool CHUNK> struct Cfg {
   // warps: 0 x loads, 1 MMA, 2 code loads, 3 allocation, 4-7 epilogue, then groups of eight that decode
   // steps in turn.  float32 results keep NT sums per epilogue thread, which leaves registers for one group.
-  // A pair has the registers for a third group (512 x 4096 -> 14336: 70 us with two, 61 with three); one-SM
-  // tiles were no faster with it.
+  // A pair has the registers for a third group (MXFP4, bf16, 4096 -> 14336: 512 tokens 78 us with
+  // two, 62 with three, 4096 tokens 474 and 420); one-SM tiles were no faster with it.
   static constexpr int kGroups = CHUNK ? 1 : PAIR ? 3 : 2;
   static constexpr int kThreads = 256 + 256 * kGroups;
   static constexpr int kXRows = PAIR ? NT / 2 : NT;
@@ -483,8 +483,11 @@ int launch_form(const XView& x, int parts, int64_t T, const Mx4View& w, float al
   const int sms = device_sm_count();
   const int64_t mt = ((TR ? w.n : w.rows) + 127) / 128;
   const int steps = (int)((x.K + 127) / 128);
-  // 128-deep steps take about 1350 clocks, the decoding's, for any of these tile widths, and 1750 in a pair
-  // (512 tokens 4096 -> 4096: 27 us in one-SM tiles, 35 in pairs; 256 tokens 4096 -> 14336: 48 and 36)
+  // Clocks of a 128-deep step, from 4096 and 8192 columns with one round of tiles and cold weights: bf16 1320 to 1460
+  // for any of the widths, which is the decoding's time, and 1750 in a pair.  (Float16's two parts take 1370, 1600
+  // and 1880 for 32, 64 and 128 tokens and 3300 in a pair, float32's three with 64 tokens 2100; with these in the
+  // estimates no case of 30 was faster and 300 tokens 4096 -> 14336 took 108 us for 99, so one pair of numbers
+  // serves all.)
   if (dtype == kMxF32) {
     double clocks;
     const int split = best_split(mt * ((T + 63) / 64), steps, 1350, 64, sms, &clocks);
@@ -510,10 +513,18 @@ int launch_form(const XView& x, int parts, int64_t T, const Mx4View& w, float al
 
 // Whether the weights are decoded to the workspace first: for many tokens, where the decoded weights stay in
 // L2 (126 MB) beside x and y, and for float32, whose sums in registers leave the fused form one group that
-// decodes and 64 tokens a tile.  Measured, MXFP4, with L2 flushed, decoded first / in the product, us:
-// bf16 4096 -> 4096 (32 MiB decoded), 512 tokens 37 / 36, 600 42 / 45, 1024 46 / 45, 4096 134 / 151;
-// 4096 -> 8192 (64 MiB), 1024 tokens 87 / 81, 4096 282 / 271; 4096 -> 14336 (112 MiB), 600 tokens 116 / 102,
-// 4096 534 / 462; float32 4096 -> 14336, 1024 tokens 345 / 484.
+// decodes and 64 tokens a tile.  Measured, decoded first / in the product, us, cold weights:
+//                             512 tokens   600          1024         4096
+// 4096 -> 4096 (32 MiB)       33 / 29      34 / 37      34 / 38      99 / 124     MXFP4, bf16
+//                             33 / 29      33 / 37      34 / 37      105 / 127    NVFP4, bf16
+//                             33 / 29                   34 / 38      102 / 131    MXFP4, bf16, gradient
+//                             56 / 39      58 / 59      62 / 62      222 / 233    MXFP4, f16
+//                             56 / 39      57 / 59      62 / 62      228 / 238    NVFP4, f16
+//                             57 / 39                   61 / 62      227 / 238    NVFP4, f16, gradient
+// 4096 -> 14336 (112 MiB)                               129 / 120    433 / 425    MXFP4, bf16
+//                                                       137 / 116    458 / 432    NVFP4, bf16
+//                                                       227 / 206    748 / 718    MXFP4, f16
+// float32 4096 -> 4096, 512 tokens 76 / 78; 4096 -> 14336, 1024 tokens 321 / 484.
 bool use_dense(int dtype, int64_t T, int64_t rows, int64_t n) {
   return T > 544 && (dtype == kMxF32 || rows * n * 2 <= (int64_t)48 << 20);
 }

@@ -15,7 +15,7 @@
 // Many tokens: SM pairs (cta_group::2) take 256 x 256 tiles.  Each CTA loads its 128 weight rows
 // and half of the tokens, so an SM fetches 32 KB of codes per 256 columns where a one-SM 128 x 256
 // tile fetches 48, and its tensor core reads two thirds of the shared memory: 8192 x 4096 ->
-// 14336 (NVFP4) took 288 us with one-SM tiles.  Both CTAs need the scales of all the tile's
+// 14336 (NVFP4) takes 258 us with one-SM tiles, 192 with pairs.  Both CTAs need the scales of all the tile's
 // tokens.  The loads of both complete on the even CTA's barrier; its MMA warp issues for both.
 //
 // float32 results take the whole reduction in one chain of accumulations too, although each truncates: a product

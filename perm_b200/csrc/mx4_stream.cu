@@ -606,8 +606,8 @@ struct StreamPlan {
   bool convert;         // x is converted by a kernel of its own
 };
 // False where the kernel does not take these sizes: more tokens than it is good for (MXFP4, bf16, here / decoded
-// to bf16 for tcgen05: 4096 -> 14336 with 16 tokens 18 / 23 us, with 24 tokens 33 / 23 us), or slices of x
-// that would leave no room in shared memory.
+// to bf16 for tcgen05: 4096 -> 14336 with 16 tokens 16 / 24 us; a third tile of columns would take 17 tokens at
+// 20 / 24 and 24 tokens at 26 / 24), or slices of x that would leave no room in shared memory.
 bool stream_plan(int dtype, int64_t T, int64_t rows, int64_t n, StreamPlan* plan) {
   if (T > 16) return false;
   const int64_t wt = (rows + 127) / 128;
@@ -616,11 +616,12 @@ bool stream_plan(int dtype, int64_t T, int64_t rows, int64_t n, StreamPlan* plan
   // 15.9; 4096 -> 4096, bf16, 8 tokens 7.5 / 7.2; float32, 4 tokens 7.7 / 7.7, 12 tokens 11.4 / 13.1.
   const bool convert = dtype != kMxF16 && T * n * wt > (dtype == kMxF32 ? 600000 : 2000000);
   const int parts = dtype == kMxF32 ? Parts<float>::k : 1;
-  const int most = 2;   // CTAs to an SM, by registers (three of fewer registers were 3 % slower for one token)
+  const int most = 2;   // CTAs to an SM, by registers (three of fewer: one token 4096 -> 14336 12.6 us for 10.3, 16 tokens 24 for 16)
   const int sms = device_sm_count();
   const int steps = (int)(mx4_pitch(n) / 128), stage = 128 * 128 + 4 * 512;   // NVFP4's; MXFP4's is smaller
   int split = 1;
-  // one and a half rounds of shorter CTAs beat one of longer ones (14336 -> 4096, one token: 9.7 / 10.9 us)
+  // one and a half rounds of shorter CTAs beat one of longer ones (14336 -> 4096, bf16: one token 9.6 / 10.6 us, 8
+  // tokens 13.0 / 14.1)
   while (split < 8 && wt <= 3 * most / 2 * cluster_slots(split * 2, sms) && split * 2 <= steps) split *= 2;
   // x's slice stays in shared memory beside at least two stages
   auto x_bytes = [&](int sp) { return T * parts * ((int64_t)(steps + sp - 1) / sp * 512 + 64); };

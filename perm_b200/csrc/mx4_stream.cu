@@ -19,9 +19,9 @@
 // 2^-31 of the largest.  A float32 value is the sum of two f16 parts, the second 2^11 times finer: 23 bits
 // and a sign, so that it is off by a unit in the last place (2^-23 of itself) at most if it is at least 2^-26 of the
 // largest.  (A third part makes it exact, and 8 tokens 4096 -> 14336 28 us for 16.5.)  A part is a column of B of
-// its own.  Units of 2^-77 to 2^49 keep every step inside float32's range unless the result is outside.
+// its own.  Units of 2^-126 to 2^49 keep every step inside float32's range unless the result is outside.
 //
-// Where a row has smaller values, or another unit, the CTA takes all its rows as they are instead, in bf16: weights
+// Where a row has smaller values, or a larger unit, the CTA takes all its rows as they are instead, in bf16: weights
 // times scales, exact as in the products for more tokens, against bf16 values or the three bf16 parts that a
 // float32 is cut into, so that nothing is lost beside a large value.  Four more instructions for two weights, and
 // the cutting, make that the slower way (one token 4096 -> 14336: bf16 14.0 us for 10.1, float32 27 for 12).
@@ -126,10 +126,10 @@ __device__ __forceinline__ float as_f32(float v) { return v; }
 __device__ __forceinline__ float as_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float as_f32(__half v) { return __half2float(v); }
 
-// k: parts.  span: a value of at least 2^-span of its row's largest is held in the row's unit.
-template <typename S> struct Parts { static constexpr int k = 1, span = 31; static constexpr bool scaled = true; };
-template <> struct Parts<__half> { static constexpr int k = 1, span = 0; static constexpr bool scaled = false; };
-template <> struct Parts<float> { static constexpr int k = 2, span = 26; static constexpr bool scaled = true; };
+// k: parts.  least: the exponent, in the row's unit, from which a value is held.
+template <typename S> struct Parts { static constexpr int k = 1, least = -17; static constexpr bool scaled = true; };
+template <> struct Parts<__half> { static constexpr int k = 1, least = 0; static constexpr bool scaled = false; };
+template <> struct Parts<float> { static constexpr int k = 2, least = -12; static constexpr bool scaled = true; };
 
 // Unit c of a row t, `units` to a row.
 struct Unit {
@@ -187,18 +187,20 @@ template <typename S> __device__ __forceinline__ void take_x8(const uint8_t* at,
 #pragma unroll
   for (int e = 0; e < 8; e++) r.take(v[e]);
 }
+// The exponent of one over a row's unit, for a largest magnitude (as bits) with the exponent field e: the largest
+// goes to [2^14, 2^15), or as far as 2^126 takes it.
+__device__ __forceinline__ int unit_shift(uint32_t top) { return min(141 - (int)(top >> 23), 126); }
 // Whether a row's unit holds all its values.
 template <typename S> __device__ __forceinline__ bool in_unit(uint32_t top, uint32_t low) {
   const int e = (int)(top >> 23), least = (int)((low + 1) >> 23);
-  return top == 0 || (e >= 127 - 63 && e <= 127 + 63 && least >= e - Parts<S>::span);
+  return top == 0 || (e <= 127 + 63 && least > 0 && least - 127 + unit_shift(top) >= Parts<S>::least);
 }
-
-// 2^(14 - e) for a largest magnitude (as bits) of exponent e, -63 to 63, and its inverse.  1 for no magnitude.
+// One over the unit of a row that its unit holds, and the unit.  1 for no magnitude.
 __device__ __forceinline__ float scale_up(uint32_t top) {
-  return top ? __uint_as_float((268 - (top >> 23)) << 23) : 1.0f;
+  return top ? __uint_as_float((uint32_t)(127 + unit_shift(top)) << 23) : 1.0f;
 }
 __device__ __forceinline__ float scale_down(uint32_t top) {
-  return top ? __uint_as_float(((top >> 23) - 14) << 23) : 1.0f;
+  return top ? __uint_as_float((uint32_t)(127 - unit_shift(top)) << 23) : 1.0f;
 }
 // Eight values in their row's unit (`up`) as f16, the parts of a value `apart` bytes from one another.
 template <typename S> __device__ __forceinline__ void write_x8(uint8_t* at, int64_t apart, const float (&v)[8], float up) {

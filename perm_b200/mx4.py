@@ -293,7 +293,8 @@ class _Product(torch.autograd.Function):
 
 def linear(x, w):
     """x w^T: x [..., n] (bf16, f16 or f32), w [out, n] -> [..., out] in x's type.  x is taken as it is; only
-    float32 values of up to 16 rows may be off by a unit in the last place (2^-23).  NVFP4's sums are formed
+    float32 values of up to 16 rows may be off by a unit in the last place (2^-23), and values below 2^-110
+    are taken as multiples of 2^-133.  NVFP4's sums are formed
     before the tensor scale: |x| up to 2^100 keeps them finite.  x gets a gradient (reverse and forward mode,
     also of second order; torch.func and vmap raise); the weights are frozen."""
     if x.requires_grad and torch.is_grad_enabled() or _forward._current_level >= 0:

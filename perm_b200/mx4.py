@@ -159,7 +159,7 @@ def tensor_scale_for(x):
 
 def quantize(x, fmt, qw=None, tensor_scale=1.0):
     """x [rows, n] (bf16, f16 or f32; any row stride) -> Mx4Tensor.  qw: non-negative column
-    weights [n], or None.  tensor_scale: a power of two (1 for MXFP4)."""
+    weights [n], or None.  tensor_scale: a power of two (1 for MXFP4).  x gets no gradient."""
     if fmt not in BLOCK:
         raise ValueError(f"unknown 4-bit format {fmt!r}")
     if not x.is_cuda:
@@ -207,7 +207,7 @@ def from_gguf(raw, n):
 
 
 def matmul(a, w, dtype=torch.bfloat16):
-    """a w^T for two operands of one format: a [T, n], w [out, n] -> [T, out] in `dtype`."""
+    """a w^T for two operands of one format: a [T, n], w [out, n] -> [T, out] in `dtype` (no gradient)."""
     dt = _DTYPE.get(dtype)
     if dt is None:
         raise ValueError("mx4.matmul: dtype must be bf16, f16 or f32")

@@ -356,8 +356,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   } else {
     // ---- x into shared memory: asynchronous copies of the rows as they are (float32: a group of eight
     // values in its two parts' places), then (scaled types) a pass for their ranges and, if the rows' units hold
-    // them, one that converts each group in place.  A warp takes units of 256 columns of one row; a thread reads back only what it
-    // copied itself.
+    // them, one that converts each group in place.  A warp takes units of 256 columns of one row; a thread
+    // reads back only what it copied itself.
     const int units = s_end - s_begin;   // a row's
     const int64_t k0 = (int64_t)s_begin * 256;
     bool odd = false;   // x has an infinity or NaN
